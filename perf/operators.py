@@ -166,11 +166,12 @@ def prepare(case, seed):
         if case["op"] == "cache":
             s["k"], s["v"] = k, v
         else:
-            s["k8"], s["k_scale"] = _kv8(k, s["lengths"])
+            k8, s["k_scale"] = _kv8(k, s["lengths"])
+            s["k8"] = k8.contiguous()
             v8, s["v_scale"] = _kv8(v, s["lengths"])
             del k, v
             # [B, H, blocks, 64, D] -> values with the tokens of a block innermost
-            s["v8"] = v8.view(torch.uint8).transpose(-1, -2).contiguous().view(torch.float8_e4m3fn)
+            s["v8"] = v8.contiguous().view(torch.uint8).transpose(-1, -2).contiguous().view(torch.float8_e4m3fn)
             s["q"] = torch.randn(B, case["Lq"], case["H"], D, generator=g, device="cuda").to(torch.bfloat16)
     return s
 
