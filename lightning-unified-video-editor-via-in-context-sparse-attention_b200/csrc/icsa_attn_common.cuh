@@ -91,6 +91,23 @@ ICSA_DEV void tmem_load_row128(uint32_t taddr, float (&s)[128]) {
     for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(r[c][e]);
 }
 
+// The dense kernels come in two forms: the attention of this library's sparse
+// call, whose key count is the same for every batch element (read from the
+// parameters where it is needed), and RAGGED, with a key count per batch
+// element and query heads that share key/value heads.
+template <bool RAGGED>
+ICSA_DEV int key_count(const AttnParams& p, int b) {
+  return RAGGED && p.kv_lens ? min(max(p.kv_lens[b], 0), p.tkv) : p.tkv;
+}
+// Steps of 128 keys (one even without keys: the softmax masks it whole).
+template <bool RAGGED>
+ICSA_DEV int key_steps(const AttnParams& p, int keys) {
+  return RAGGED ? max(1, (keys + 127) / 128) : (p.nkv + 1) / 2;
+}
+template <bool RAGGED>
+ICSA_DEV int key_head(const AttnParams& p, int h) { return RAGGED ? h / p.kv_group : h; }
+inline bool is_ragged(const AttnParams& p) { return p.kv_lens != nullptr || p.kv_group > 1; }
+
 ICSA_DEV float load_alpha(const AttnParams& p, int b, int token, int h, int d) {
   const long long off = b * p.alpha_strides[0] + token * p.alpha_strides[1] + h * p.alpha_strides[2] +
                         d * p.alpha_strides[3];

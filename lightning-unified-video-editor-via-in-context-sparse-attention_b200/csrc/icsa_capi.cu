@@ -181,6 +181,26 @@ int encode_pooled_map(CUtensorMap* m, const void* base, int BH, int n, int D) {
 
 }  // namespace
 
+namespace icsa {
+int encode_rows_tensor_map(CUtensorMap* m, const void* base, int B, int rows, int H, int D, int64_t row_stride) {
+  return encode_rows_map(m, base, B, rows, H, D, row_stride);
+}
+
+int encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t cols, uint64_t rows,
+                         uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return fail(ICSA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ICSA_ERR_CUDA, "cuTensorMapEncodeTiled (2-D map) failed with %d", int(r));
+  return ICSA_OK;
+}
+}  // namespace icsa
+
 // ===========================================================================
 // Stage drivers
 // ===========================================================================
@@ -683,7 +703,7 @@ int icsa_dit_linear_residual(const void* a, int64_t lda, const void* w, int64_t 
 }
 
 int icsa_last_status(cudaStream_t stream, int clear) {
-  constexpr int kUnits = 6;
+  constexpr int kUnits = 7;
   static std::mutex mu;
   static int* addr[kMaxDevices][kUnits] = {};
   cudaError_t e = cudaStreamSynchronize(stream);
@@ -695,7 +715,8 @@ int icsa_last_status(cudaStream_t stream, int clear) {
   if (addr[dev][0] == nullptr) {
     cudaError_t (*const get[kUnits])(int**) = {icsa::sticky_status_dense_pair, icsa::sticky_status_flat,
                                                icsa::sticky_status_sparse, icsa::sticky_status_selftest,
-                                               icsa::sticky_status_gemm, icsa::sticky_status_scores};
+                                               icsa::sticky_status_gemm, icsa::sticky_status_scores,
+                                               icsa::sticky_status_fp4};
     int* a[kUnits] = {};
     for (int i = 0; i < kUnits; ++i)
       if ((e = get[i](&a[i])) != cudaSuccess) return cuda_fail(e, "sticky status address");

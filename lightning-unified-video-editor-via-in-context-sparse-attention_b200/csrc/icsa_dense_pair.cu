@@ -72,9 +72,11 @@ struct PTile {
   int blk[2];    // query blocks of rows [0,64) and [64,128) of this CTA
   int write[2];  // 0 for a duplicate filling an incomplete group
   int n_steps;   // key steps of 128 rows
+  int keys, kvh;  // valid keys and key/value head
   uint32_t rank;
 };
 
+template <bool RAGGED>
 ICSA_DEV PTile decode_pair_tile(const AttnParams& p) {
   PTile t;
   t.rank = pair::cluster_rank();
@@ -93,7 +95,9 @@ ICSA_DEV PTile decode_pair_tile(const AttnParams& p) {
     const int rr = t.write[i] ? r : p.num_flat - 1;
     t.blk[i] = order ? order[rr] : rr;
   }
-  t.n_steps = (p.nkv + 1) / 2;
+  t.keys = key_count<RAGGED>(p, t.b);
+  t.n_steps = key_steps<RAGGED>(p, t.keys);
+  t.kvh = key_head<RAGGED>(p, t.h);
   return t;
 }
 
@@ -122,11 +126,11 @@ ICSA_DEV void pair_producer(const AttnParams& p, const AttnMaps& maps, const PTi
     const int rk = t.rank ? r1 : r0;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      pair::tma_load_4d(sm.kv[s] + c * (kPKBytes / 2), &maps.k, kv_full, c * 64, t.h, rk, t.b);
+      pair::tma_load_4d(sm.kv[s] + c * (kPKBytes / 2), &maps.k, kv_full, c * 64, t.kvh, rk, t.b);
     // values: all 128 keys, this CTA's 64 of the 128 d (N split)
     uint8_t* vdst = sm.kv[s] + kPKBytes;
-    pair::tma_load_4d(vdst, &maps.v, kv_full, int(t.rank) * 64, t.h, r0, t.b);
-    pair::tma_load_4d(vdst + kPVBytes / 2, &maps.v, kv_full, int(t.rank) * 64, t.h, r1, t.b);
+    pair::tma_load_4d(vdst, &maps.v, kv_full, int(t.rank) * 64, t.kvh, r0, t.b);
+    pair::tma_load_4d(vdst + kPVBytes / 2, &maps.v, kv_full, int(t.rank) * 64, t.kvh, r1, t.b);
   }
 }
 
@@ -208,6 +212,7 @@ ICSA_DEV void pair_mma(const AttnParams& p, const PTile& t, PSmem& sm, uint32_t 
 // epilogue's named barriers pair them): after a failed wait the abort flag
 // is set, every later wait returns at once, the loop runs on over stale
 // data, and the error code marks the result invalid.
+template <bool RAGGED>
 ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTile& t, PSmem& sm, uint32_t tmem) {
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -244,7 +249,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
     if (lane == 0) pair::arrive_cluster_relaxed(s_free);
     __syncwarp();
 
-    const int hi = p.tkv - j * 128;  // extended-KV rows beyond tkv are not keys
+    const int hi = (RAGGED ? t.keys : p.tkv) - j * 128;  // extended-KV rows beyond tkv are not keys
     if (hi < 128) {
 #pragma unroll
       for (int c = 0; c < 128; ++c)
@@ -317,6 +322,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
   const float f1 = (!has1 || m1 == -INFINITY) ? 0.f : ex2((m1 - m_fin) * sl2);
   const float lt = sm.lsum[0][row] * f0 + (has1 ? sm.lsum[1][row] * f1 : 0.f);
   const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  const bool none = RAGGED && t.keys == 0;  // no valid key: the accumulators hold NaN, the output is zero
   const int hb = row >> 6;
   const int blk = hb ? t.blk[1] : t.blk[0];  // (no dynamic indexing: keeps the tile in registers)
   const int token = blk * kBlock + (row & 63);
@@ -343,7 +349,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
       float o[32], x[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e)
-        o[e] = (__uint_as_float(r[e]) * f0 + (has1 ? __uint_as_float(r1[e]) * f1 : 0.f)) * inv;
+        o[e] = none ? 0.f : (__uint_as_float(r[e]) * f0 + (has1 ? __uint_as_float(r1[e]) * f1 : 0.f)) * inv;
       if (valid_row && scalar) residual32_ca(oc, 64 * w + 32 * c, o, x);
       else if (valid_row) residual32(p, t.b, token, t.h, oc, 64 * w + 32 * c, o, x);
       else
@@ -388,7 +394,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
     float o[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e)
-      o[e] = (__uint_as_float(r[e]) * f0 + (has1 ? __uint_as_float(r1[e]) * f1 : 0.f)) * inv;
+      o[e] = none ? 0.f : (__uint_as_float(r[e]) * f0 + (has1 ? __uint_as_float(r1[e]) * f1 : 0.f)) * inv;
     if (!write) continue;
     if (scalar) {
       float x[32];
@@ -415,12 +421,13 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
     }
   }
 }
+template <bool RAGGED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
     dense_pair_kernel(const AttnParams p, const __grid_constant__ AttnMaps maps) {
   extern __shared__ uint8_t smem_raw[];
   PSmem& sm = *reinterpret_cast<PSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const PTile t = decode_pair_tile(p);
+  const PTile t = decode_pair_tile<RAGGED>(p);
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 1);
@@ -460,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
   // a warpgroup.
   if (warp < 8) {
     tc::reg_alloc<216>();
-    pair_softmax(p, maps, t, sm, tmem);
+    pair_softmax<RAGGED>(p, maps, t, sm, tmem);
   } else {
     tc::reg_dealloc<72>();
   }
@@ -498,9 +505,10 @@ cudaError_t launch_dense_pair_attention(const AttnParams& p, const AttnMaps& map
   const int pairs = p.B * p.H * ((p.num_flat + 3) / 4);
   if (pairs == 0) return cudaSuccess;
   const size_t smem = sizeof(PSmem) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  const auto kernel = is_ragged(p) ? dense_pair_kernel<true> : dense_pair_kernel<false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
-  dense_pair_kernel<<<2 * pairs, kPThreads, smem, stream>>>(p, maps);
+  kernel<<<2 * pairs, kPThreads, smem, stream>>>(p, maps);
   return cudaGetLastError();
 }
 

@@ -62,8 +62,10 @@ struct FTile {
   int blk[4];    // query blocks of rows [0,64), [64,128) of tile 0 and of tile 1
   int write[4];  // 0 for a duplicate filling an incomplete group
   int n_steps;   // KV steps of 128 rows
+  int keys, kvh;  // valid keys and key/value head
 };
 
+template <bool RAGGED>
 ICSA_DEV FTile decode_flat_tile(const AttnParams& p, int cta) {
   FTile t;
   const int groups = (p.num_flat + 3) / 4;
@@ -80,7 +82,9 @@ ICSA_DEV FTile decode_flat_tile(const AttnParams& p, int cta) {
     const int rr = t.write[i] ? r : p.num_flat - 1;
     t.blk[i] = order ? order[rr] : rr;
   }
-  t.n_steps = (p.nkv + 1) / 2;
+  t.keys = key_count<RAGGED>(p, t.b);
+  t.n_steps = key_steps<RAGGED>(p, t.keys);
+  t.kvh = key_head<RAGGED>(p, t.h);
   return t;
 }
 
@@ -105,16 +109,16 @@ ICSA_DEV void flat_producer(const AttnParams& p, const AttnMaps& maps, const FTi
     mbar_arrive_expect_tx(&sm.k_full[ks], C::kOpBytes);
     for (int c = 0; c < C::kChunks; ++c) {
       uint8_t* dst = sm.k[ks] + c * kChunkBytes;
-      tma_load_4d(dst, &maps.k, &sm.k_full[ks], c * 64, t.h, r0, t.b);
-      tma_load_4d(dst + kChunkBytes / 2, &maps.k, &sm.k_full[ks], c * 64, t.h, r1, t.b);
+      tma_load_4d(dst, &maps.k, &sm.k_full[ks], c * 64, t.kvh, r0, t.b);
+      tma_load_4d(dst + kChunkBytes / 2, &maps.k, &sm.k_full[ks], c * 64, t.kvh, r1, t.b);
     }
     const int vs = j % C::kVStages;
     if (!mbar_wait(&sm.v_empty[vs], (uint32_t(j / C::kVStages) & 1u) ^ 1u, p.err, kErrVEmpty, abort_flag)) return;
     mbar_arrive_expect_tx(&sm.v_full[vs], C::kOpBytes);
     for (int c = 0; c < C::kChunks; ++c) {
       uint8_t* dst = sm.v[vs] + c * kChunkBytes;
-      tma_load_4d(dst, &maps.v, &sm.v_full[vs], c * 64, t.h, r0, t.b);
-      tma_load_4d(dst + kChunkBytes / 2, &maps.v, &sm.v_full[vs], c * 64, t.h, r1, t.b);
+      tma_load_4d(dst, &maps.v, &sm.v_full[vs], c * 64, t.kvh, r0, t.b);
+      tma_load_4d(dst + kChunkBytes / 2, &maps.v, &sm.v_full[vs], c * 64, t.kvh, r1, t.b);
     }
   }
 }
@@ -206,7 +210,7 @@ ICSA_DEV void flat_mma(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32
 // ---------------------------------------------------------------------------
 // Softmax warpgroups (warps 0-3: tile 0, warps 4-7: tile 1) and epilogue.
 // ---------------------------------------------------------------------------
-template <int D>
+template <int D, bool RAGGED>
 ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32_t tmem) {
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5;
@@ -224,7 +228,7 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
     tc::fence_after_sync();
     float s[128];
     tmem_load_row128(s_col, s);
-    const int hi = p.tkv - j * 128;  // extended-KV rows beyond tkv are not keys
+    const int hi = (RAGGED ? t.keys : p.tkv) - j * 128;  // extended-KV rows beyond tkv are not keys
     if (hi < 128) {
 #pragma unroll
       for (int c = 0; c < 128; ++c)
@@ -287,6 +291,7 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
   const int token = blk * kBlock + (row & 63);
   const bool write = wr && token < p.S;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const bool none = RAGGED && t.keys == 0;  // no valid key: the accumulators hold NaN, the output is zero
   const float* oc = p.outc ? p.outc + (size_t(t.bh) * p.NB + blk) * D : nullptr;  // nullptr: no residual term
   const size_t out_row = ((size_t(t.b) * p.S + token) * p.H + t.h) * D;
 #pragma unroll 1
@@ -297,18 +302,18 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
     tc::tmem_wait_ld();
     float o[32];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(r[e]) * inv;
+    for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : __uint_as_float(r[e]) * inv;
     if (write) store_out32(p, t.b, token, t.h, oc, c * 32, o, out_row);
   }
 }
 
-template <int D>
+template <int D, bool RAGGED>
 __global__ void __launch_bounds__(kFThreads, 1) flat_kernel(const AttnParams p, const __grid_constant__ AttnMaps maps) {
   extern __shared__ uint8_t smem_raw[];
   FSmem<D>& sm = *reinterpret_cast<FSmem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using C = FCfg<D>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const FTile t = decode_flat_tile(p, blockIdx.x);
+  const FTile t = decode_flat_tile<RAGGED>(p, blockIdx.x);
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 1);
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(kFThreads, 1) flat_kernel(const AttnParams p, 
   // a warpgroup.
   if (warp < 8) {
     tc::reg_alloc<216>();
-    flat_softmax<D>(p, t, sm, tmem);
+    flat_softmax<D, RAGGED>(p, t, sm, tmem);
   } else {
     tc::reg_dealloc<72>();  // one instance for all four warps of warpgroup 2
     if (warp == kFProducerWarp && lane == 0) {
@@ -385,14 +390,16 @@ cudaError_t launch_flat_attention(const AttnParams& p, const AttnMaps& maps, int
   if (D == 128) return launch_dense_pair_attention(p, maps, stream);
   if (D == 128) {
     const size_t smem = sizeof(FSmem<128>) + 1024;
-    cudaError_t e = cudaFuncSetAttribute(flat_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    const auto kernel = is_ragged(p) ? flat_kernel<128, true> : flat_kernel<128, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return e;
-    flat_kernel<128><<<ctas, kFThreads, smem, stream>>>(p, maps);
+    kernel<<<ctas, kFThreads, smem, stream>>>(p, maps);
   } else if (D == 64) {
     const size_t smem = sizeof(FSmem<64>) + 1024;
-    cudaError_t e = cudaFuncSetAttribute(flat_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    const auto kernel = is_ragged(p) ? flat_kernel<64, true> : flat_kernel<64, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return e;
-    flat_kernel<64><<<ctas, kFThreads, smem, stream>>>(p, maps);
+    kernel<<<ctas, kFThreads, smem, stream>>>(p, maps);
   } else {
     return cudaErrorInvalidValue;
   }

@@ -1,0 +1,317 @@
+// Microscaled 4-bit floating point: quantisation of rows into the storage form
+// of icsa_lowp.cuh, and back.
+//
+// Quantisation of one block of n elements (n = 16: nvfp4, n = 32: mxfp4):
+//   amax = max |x|
+//   nvfp4: s = e4m3(amax / (6 g)), step d = s g    (g: the tensor's global scale)
+//   mxfp4: s = 2^(floor(log2 amax) - 2) (exponent in [-127, 127]), d = s
+//   code = e2m1(x / d), rounded to nearest even, largest magnitude 6; 0 where d = 0
+// Quotients are those of IEEE float32 division, so a host computation in
+// float32 gives the same bytes.  A block that holds a NaN or an infinity gets
+// the format's NaN scale (0x7f / 0xff).
+//
+// One pass over memory: a thread owns 16 elements of a row (32 bytes of bf16:
+// one 256-bit load), writes their 8 code bytes, and each group of four scales
+// is gathered by shuffles into one 32-bit store.  The eight warps of a CTA
+// take eight rows of one scale tile whose scale words share 32-byte sectors
+// (rows r, r + 1 and those 32, 64, 96 further), so that the scattered words
+// reach memory as whole sectors.
+#include "icsa_lowp.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+namespace icsa {
+
+namespace {
+
+constexpr int kQThreads = 256;
+constexpr int kQChunk = 512;  // elements of a row that one warp takes at a time
+
+struct alignas(32) Words8 {
+  uint32_t w[8];
+};
+
+// 32-byte global accesses (the address is a multiple of 32)
+ICSA_DEV Words8 load32(const void* p) {
+  Words8 r;
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                 "=r"(r.w[7])
+               : "l"(p));
+  return r;
+}
+ICSA_DEV void store32(void* p, const Words8& r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+               "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+               : "memory");
+}
+
+template <typename T>
+ICSA_DEV float to_float(T v);
+template <>
+ICSA_DEV float to_float<float>(float v) {
+  return v;
+}
+template <>
+ICSA_DEV float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+
+// 16 consecutive elements of a row from column k0; zeros from column K on
+template <typename T, bool VEC>
+ICSA_DEV void load16(const T* row, int k0, int K, float (&v)[16]) {
+  if (VEC && k0 + 16 <= K) {
+    if constexpr (sizeof(T) == 2) {
+      const Words8 r = load32(row + k0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[2 * i] = __uint_as_float(r.w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Words8 r = load32(row + k0 + 8 * h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(r.w[i]);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = k0 + i < K ? to_float<T>(row[k0 + i]) : 0.f;
+}
+
+// eight floats to e2m1 (nearest even, saturating), the first in the low half of byte 0
+ICSA_DEV uint32_t e2m1x8(const float* v) {
+  uint32_t o;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(o)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return o;
+}
+
+// four code bytes to eight floats
+ICSA_DEV void e2m1x8_floats(uint32_t w, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+ICSA_DEV float e4m3_float(uint32_t byte) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
+  return __half2float(__half(h));
+}
+
+// byte offset of the scale tile row of row r, and of K tile / scale c in it
+ICSA_DEV size_t scale_row(int r, int k_tiles, int atoms) {
+  return size_t(r >> 7) * k_tiles * atoms * kScaleAtomBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+}
+
+// rows of CTA blockIdx.x: warp w of pair-group i
+ICSA_DEV int tile_row(int cta, int warp) {
+  return (cta >> 4) * kFp4TileRows + (cta & 15) * 2 + (warp & 1) + 32 * (warp >> 1);
+}
+
+// The 16 codes of x / d: nearest to the float32 quotient.
+ICSA_DEV void quotient_codes(const float (&v)[16], float d, uint32_t (&code)[2]) {
+  float q[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) q[i] = __fdiv_rn(v[i], d);
+  code[0] = e2m1x8(q);
+  code[1] = e2m1x8(q + 8);
+}
+
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantParams p, int chunks_per_cta) {
+  constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = tile_row(blockIdx.x, warp);
+  const int k_tiles = (p.K + kFp4TileK - 1) / kFp4TileK;
+  const int k_end = k_tiles * kFp4TileK;
+  const int row_bytes = (p.K + 31) / 32 * 16;
+  uint8_t* srow = p.scales + scale_row(r, k_tiles, kAtoms);
+  const T* xrow = static_cast<const T*>(p.x) + int64_t(r) * p.ldx;
+  uint8_t* drow = p.data + int64_t(r) * row_bytes;
+  const bool row_ok = r < p.rows;
+  const int c0 = blockIdx.y * chunks_per_cta;
+  for (int c = c0; c < c0 + chunks_per_cta; ++c) {
+    const int k0 = c * kQChunk + lane * 16;
+    if (c * kQChunk >= k_end) break;
+    float v[16];
+    if (row_ok && k0 < p.K) {
+      load16<T, VEC>(xrow, k0, p.K, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    }
+    // largest magnitude as bits: NaN and infinity stay above every number
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    uint32_t code[2] = {0u, 0u};
+    uint32_t sbyte;
+    if (FMT == ICSA_NVFP4) {
+      const float t = __fdiv_rn(__uint_as_float(top), 6.0f * p.global_scale);
+      sbyte = top >= 0x7F800000u ? 0x7Fu : uint32_t(__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3));
+      const float d = e4m3_float(sbyte) * p.global_scale;
+      if (d > 0.f && top < 0x7F800000u) quotient_codes(v, d, code);
+    } else {
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      // floor(log2 amax): the exponent field; subnormal magnitudes clamp to 2^-127
+      const int e = min(max(int(top >> 23) - 127 - 2, -127), 127);
+      sbyte = top >= 0x7F800000u ? 0xFFu : uint32_t(e + 127);
+      if (top < 0x7F800000u) {
+        const float inv = __uint_as_float(uint32_t(127 - e) << 23);  // 2^-e, exact products
+        float q[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q[i] = v[i] * inv;
+        code[0] = e2m1x8(q);
+        code[1] = e2m1x8(q + 8);
+      }
+    }
+    if (row_ok && k0 / 2 < row_bytes) *reinterpret_cast<uint2*>(drow + k0 / 2) = make_uint2(code[0], code[1]);
+    // four scales to one word
+    if (FMT == ICSA_NVFP4) {
+      uint32_t w = sbyte << (8 * (lane & 3));
+      w |= __shfl_xor_sync(0xffffffffu, w, 1);
+      w |= __shfl_xor_sync(0xffffffffu, w, 2);
+      if ((lane & 3) == 0 && k0 < k_end) *reinterpret_cast<uint32_t*>(srow + size_t(k0 / 64) * kScaleAtomBytes) = w;
+    } else {
+      uint32_t w = (lane & 1) ? 0u : sbyte << (8 * ((lane >> 1) & 3));
+      w |= __shfl_xor_sync(0xffffffffu, w, 2);
+      w |= __shfl_xor_sync(0xffffffffu, w, 4);
+      if ((lane & 7) == 0 && k0 < k_end) *reinterpret_cast<uint32_t*>(srow + size_t(k0 / 128) * kScaleAtomBytes) = w;
+    }
+  }
+}
+
+template <typename T, int FMT, bool VEC>
+__global__ void __launch_bounds__(kQThreads) fp4_dequantize_kernel(const Fp4DequantParams p, int chunks_per_cta) {
+  constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = tile_row(blockIdx.x, warp);
+  if (r >= p.rows) return;
+  const int k_tiles = (p.K + kFp4TileK - 1) / kFp4TileK;
+  const int row_bytes = (p.K + 31) / 32 * 16;
+  const uint8_t* srow = p.scales + scale_row(r, k_tiles, kAtoms);
+  const uint8_t* drow = p.data + int64_t(r) * row_bytes;
+  T* orow = static_cast<T*>(p.out) + int64_t(r) * p.ldo;
+  const int c0 = blockIdx.y * chunks_per_cta;
+  for (int c = c0; c < c0 + chunks_per_cta; ++c) {
+    const int k0 = c * kQChunk + lane * 16;
+    if (k0 >= p.K) break;
+    const uint2 code = __ldg(reinterpret_cast<const uint2*>(drow + k0 / 2));
+    float d;
+    if (FMT == ICSA_NVFP4) {
+      d = e4m3_float(srow[size_t(k0 / 64) * kScaleAtomBytes + (k0 / 16) % 4]) * p.global_scale;
+    } else {
+      const uint32_t e = srow[size_t(k0 / 128) * kScaleAtomBytes + (k0 / 32) % 4];
+      // 2^(e - 127): the subnormal 2^-127 for 0, NaN for 255
+      d = __uint_as_float(e == 255u ? 0x7FC00000u : e == 0u ? 0x00400000u : e << 23);
+    }
+    float v[16];
+    float h[8];
+    e2m1x8_floats(code.x, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = h[i] * d;
+    e2m1x8_floats(code.y, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 + i] = h[i] * d;
+    if (VEC && k0 + 16 <= p.K) {
+      if constexpr (sizeof(T) == 2) {
+        Words8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        store32(orow + k0, o);
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          Words8 o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.w[i] = __float_as_uint(v[8 * half + i]);
+          store32(orow + k0 + 8 * half, o);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + i < p.K) {
+          if constexpr (sizeof(T) == 2) orow[k0 + i] = __float2bfloat16_rn(v[i]);
+          else orow[k0 + i] = v[i];
+        }
+    }
+  }
+}
+
+bool rows_aligned32(const void* base, int64_t ld, int elem) {
+  return (reinterpret_cast<uintptr_t>(base) & 31u) == 0 && (ld * elem) % 32 == 0;
+}
+
+// CTAs cover `chunks` row chunks in grid.y; four chunks per CTA once the rows
+// alone fill the GPU, one where they do not (a few rows, latency).
+void quant_grid(int rows, int k_elems, dim3* grid, int* chunks_per_cta) {
+  const int row_ctas = (rows + kFp4TileRows - 1) / kFp4TileRows * 16;
+  const int chunks = (k_elems + kQChunk - 1) / kQChunk;
+  *chunks_per_cta = row_ctas >= 1024 ? std::min(chunks, 4) : 1;
+  *grid = dim3(row_ctas, (chunks + *chunks_per_cta - 1) / *chunks_per_cta);
+}
+
+template <typename T, int FMT>
+cudaError_t quantize_as(const Fp4QuantParams& p, cudaStream_t stream) {
+  dim3 grid;
+  int per;
+  quant_grid(p.rows, (p.K + kFp4TileK - 1) / kFp4TileK * kFp4TileK, &grid, &per);
+  if (rows_aligned32(p.x, p.ldx, sizeof(T))) fp4_quantize_kernel<T, FMT, true><<<grid, kQThreads, 0, stream>>>(p, per);
+  else fp4_quantize_kernel<T, FMT, false><<<grid, kQThreads, 0, stream>>>(p, per);
+  return cudaGetLastError();
+}
+
+template <typename T, int FMT>
+cudaError_t dequantize_as(const Fp4DequantParams& p, cudaStream_t stream) {
+  dim3 grid;
+  int per;
+  quant_grid(p.rows, p.K, &grid, &per);
+  if (rows_aligned32(p.out, p.ldo, sizeof(T))) fp4_dequantize_kernel<T, FMT, true><<<grid, kQThreads, 0, stream>>>(p, per);
+  else fp4_dequantize_kernel<T, FMT, false><<<grid, kQThreads, 0, stream>>>(p, per);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, int x_dtype, int format, cudaStream_t stream) {
+  if (x_dtype == ICSA_BF16)
+    return format == ICSA_NVFP4 ? quantize_as<__nv_bfloat16, ICSA_NVFP4>(p, stream)
+                                : quantize_as<__nv_bfloat16, ICSA_MXFP4>(p, stream);
+  return format == ICSA_NVFP4 ? quantize_as<float, ICSA_NVFP4>(p, stream) : quantize_as<float, ICSA_MXFP4>(p, stream);
+}
+
+cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, int out_dtype, int format, cudaStream_t stream) {
+  if (out_dtype == ICSA_BF16)
+    return format == ICSA_NVFP4 ? dequantize_as<__nv_bfloat16, ICSA_NVFP4>(p, stream)
+                                : dequantize_as<__nv_bfloat16, ICSA_MXFP4>(p, stream);
+  return format == ICSA_NVFP4 ? dequantize_as<float, ICSA_NVFP4>(p, stream)
+                              : dequantize_as<float, ICSA_MXFP4>(p, stream);
+}
+
+}  // namespace icsa

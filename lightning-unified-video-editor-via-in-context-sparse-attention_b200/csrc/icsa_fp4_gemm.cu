@@ -1,0 +1,388 @@
+// Linear layer on microscaled 4-bit operands, on SM pairs (tcgen05
+// cta_group::2, block-scaled kinds):
+//
+//   out[r, c] = bf16( act( alpha * sum_k a[r, k] w[c, k] + bias[c] ) )
+//
+// with a and w in the storage form of icsa_lowp.cuh (e2m1 codes, e4m3 scales
+// for 16 elements or e8m0 scales for 32); the tensor core multiplies codes and
+// scales itself and accumulates in float32 in TMEM.  alpha is the product of
+// the two global scales; act is the identity or the tanh form of GELU.
+//
+// Tiles: a cluster of two CTAs computes 256 x 256 outputs, each CTA 128 rows.
+// A K step is 256 elements (128-byte rows, 128-byte swizzle): each CTA loads
+// its 128 rows of a and 128 of the 256 weight rows (16 KB each), the scales
+// of its own rows of a (2 KB nvfp4) and of all 256 weight rows (4 KB, since
+// each SM scales all columns of its half of the tile).  The leader copies
+// both CTAs' scales from shared memory to TMEM (tcgen05.cp, one 512-byte
+// scale tile fills four columns, repeated in the four lane quadrants) and
+// issues four M = 256, N = 256, K = 64 MMAs.  The scale columns are double
+// buffered; copies and MMAs of one thread execute in issue order.
+//
+// TMEM (512 columns): accumulator [0, 256), scale buffers from 256, 48 each.
+//
+// Roles per CTA (320 threads): warps 0-7 epilogue (warpgroup w: columns
+// [128 w, 128 w + 128), thread <-> TMEM lane <-> output row), warp 8 TMA
+// producer, warp 9 TMEM allocation and, in the leader, the MMA issuer.  The
+// epilogue first moves its whole 128-column row into registers, releases the
+// accumulator, and then works from registers while the next tile's MMAs run.
+//
+// Few tiles (few rows, or few outputs): K is split over clusters, each
+// writing float32 partial sums that a second kernel adds in a fixed order.
+//
+// Every wait is bounded (about one second); a wait that gives up records a
+// status code (report_error) and the kernel winds down.
+#include "icsa_attn_common.cuh"
+#include "icsa_lowp.cuh"
+#include "icsa_pair.cuh"
+
+#include <algorithm>
+#include <utility>
+
+namespace icsa {
+
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kStages = 5;
+constexpr int kRows = 128;                  // output rows per CTA
+constexpr int kCols = 256;                  // output columns per pair
+constexpr int kOpBytes = 128 * 128;         // 128 rows x 256 codes
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTmScale = 256, kTmScaleStep = 48, kTmSfb = 16;  // scale buffer: a at 0, w at 16
+constexpr int kGroupM = 8;                  // tile rows per raster group
+
+enum : int { kErrFull = 0x401, kErrEmpty = 0x402, kErrAccFull = 0x403, kErrAccEmpty = 0x404 };
+
+struct __align__(1024) Smem {
+  uint8_t a[kStages][kOpBytes];
+  uint8_t w[kStages][kOpBytes];
+  uint8_t sa[kStages][4 * kScaleAtomBytes];
+  uint8_t sw[kStages][8 * kScaleAtomBytes];
+  uint64_t full[kStages], empty[kStages];
+  uint64_t acc_full, acc_empty;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Smem) + 1024 <= 232448, "fp4 gemm shared memory exceeds 227 KB");
+
+struct Unit {
+  int mt, nt, split, k0, k1;
+};
+
+// unit u: split (u / tiles) of a tile; tiles run in groups of kGroupM tile
+// rows, rows fastest, so that the clusters running at one time share their
+// rows of a and their columns of w in L2
+ICSA_DEV Unit decode_unit(const Fp4GemmParams& p, int u) {
+  const int tiles = p.m_tiles * p.n_tiles;
+  Unit t;
+  t.split = u / tiles;
+  const int i = u - t.split * tiles;
+  const int group = kGroupM * p.n_tiles;
+  const int g = i / group, r = i - g * group;
+  const int m0 = g * kGroupM;
+  const int gm = min(kGroupM, p.m_tiles - m0);
+  t.mt = m0 + r % gm;
+  t.nt = r / gm;
+  t.k0 = int(int64_t(p.k_steps) * t.split / p.splits);
+  t.k1 = int(int64_t(p.k_steps) * (t.split + 1) / p.splits);
+  return t;
+}
+
+template <int ATOMS>
+ICSA_DEV void producer(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm, uint32_t rank, int* issued) {
+  constexpr uint32_t kBytes = 2u * (2 * kOpBytes + 3 * ATOMS * kScaleAtomBytes);
+  volatile int* abort_flag = &sm.abort_flag;
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  int it = 0;
+  for (int u = cluster; u < p.units; u += clusters) {
+    const Unit t = decode_unit(p, u);
+    const int row0 = t.mt * (2 * kRows) + int(rank) * kRows;
+    const int wrow0 = t.nt * kCols + int(rank) * kRows;
+    const int sa0 = (t.mt * 2 + int(rank)) * p.k_steps * ATOMS;
+    const int sw0 = t.nt * 2 * p.k_steps * ATOMS, sw1 = sw0 + p.k_steps * ATOMS;
+    for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+      const int s = it % kStages;
+      if (!pair::wait(&sm.empty[s], (uint32_t(it / kStages) & 1u) ^ 1u, nullptr, kErrEmpty, abort_flag)) {
+        *issued = it;
+        return;
+      }
+      if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], kBytes);
+      const uint32_t full = pair::mapa(&sm.full[s], 0);
+      pair::tma_load_2d(sm.a[s], &maps.a, full, kb * 128, row0);
+      pair::tma_load_2d(sm.w[s], &maps.w, full, kb * 128, wrow0);
+      pair::tma_load_2d(sm.sa[s], &maps.sa, full, 0, sa0 + kb * ATOMS);
+      pair::tma_load_2d(sm.sw[s], &maps.sw, full, 0, sw0 + kb * ATOMS);
+      pair::tma_load_2d(sm.sw[s] + ATOMS * kScaleAtomBytes, &maps.sw, full, 0, sw1 + kb * ATOMS);
+    }
+  }
+  *issued = it;
+}
+
+// Descriptor of scale tiles in shared memory: 16-byte rows without swizzle,
+// 8-row groups 128 bytes apart.
+ICSA_DEV uint64_t scale_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= uint64_t((saddr >> 4) & 0x3FFFu);
+  d |= uint64_t(1) << 16;
+  d |= uint64_t(128 >> 4) << 32;
+  d |= uint64_t(1) << 46;  // descriptor version for sm_100
+  return d;
+}
+
+// Four TMEM columns (32 lanes x 16 bytes, repeated in the four lane
+// quadrants) from one scale tile, in both CTAs of the pair.
+ICSA_DEV void copy_scales_elect(uint32_t taddr, uint64_t desc) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
+      "l"(desc)
+      : "memory");
+}
+
+// Instruction descriptor of the block-scaled kinds with e2m1 operands.
+template <int FMT>
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, uint32_t scale_id) {
+  return (scale_id << 4)                                  // which scale byte pair of w
+         | (1u << 7)                                      // A format: e2m1
+         | (1u << 10)                                     // B format: e2m1
+         | (uint32_t(N >> 3) << 17)                       // N / 8
+         | ((FMT == ICSA_MXFP4 ? 1u : 0u) << 23)          // scale format: e4m3 or e8m0
+         | (uint32_t(M >> 4) << 24)                       // M / 16
+         | (scale_id << 29);                              // which scale byte pair of a
+}
+
+template <int FMT>
+ICSA_DEV void mma_fp4_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                            uint32_t sb, uint32_t accumulate) {
+  if constexpr (FMT == ICSA_NVFP4) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// MMA issuer: all 32 lanes of warp 9 of the leader (waits are warp-uniform,
+// one elected lane issues each instruction).
+template <int FMT>
+ICSA_DEV void issuer(const Fp4GemmParams& p, Smem& sm, uint32_t tmem) {
+  constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
+  volatile int* abort_flag = &sm.abort_flag;
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const uint64_t ad0 = tc::make_sw128_desc(smem_u32(sm.a[0]), 16, 1024);
+  const uint64_t wd0 = tc::make_sw128_desc(smem_u32(sm.w[0]), 16, 1024);
+  const uint64_t sad0 = scale_desc(smem_u32(sm.sa[0]));
+  const uint64_t swd0 = scale_desc(smem_u32(sm.sw[0]));
+  int it = 0, count = 0;
+  for (int u = cluster; u < p.units; u += clusters, ++count) {
+    const Unit t = decode_unit(p, u);
+    // the epilogue has read the previous tile's accumulator
+    if (!pair::warp_wait(&sm.acc_empty, (uint32_t(count) & 1u) ^ 1u, nullptr, kErrAccEmpty, abort_flag)) return;
+    tc::fence_after_sync();
+    for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+      const int s = it % kStages;
+      if (!pair::warp_wait(&sm.full[s], uint32_t(it / kStages) & 1u, nullptr, kErrFull, abort_flag)) return;
+      tc::fence_after_sync();
+      const uint32_t sfa = tmem + kTmScale + uint32_t(it & 1) * kTmScaleStep, sfb = sfa + kTmSfb;
+      const uint64_t sad = sad0 + uint64_t(s) * (4 * kScaleAtomBytes >> 4);
+      const uint64_t swd = swd0 + uint64_t(s) * (8 * kScaleAtomBytes >> 4);
+#pragma unroll
+      for (int at = 0; at < kAtoms; ++at) {
+        // a scale tile holds 128 rows; the weight's second 128 rows follow its first
+        copy_scales_elect(sfa + 4u * at, sad + uint64_t(at) * (kScaleAtomBytes >> 4));
+        copy_scales_elect(sfb + 8u * at, swd + uint64_t(at) * (kScaleAtomBytes >> 4));
+        copy_scales_elect(sfb + 8u * at + 4u, swd + uint64_t(kAtoms + at) * (kScaleAtomBytes >> 4));
+      }
+      const uint64_t ad = ad0 + uint64_t(s) * (kOpBytes >> 4), wd = wd0 + uint64_t(s) * (kOpBytes >> 4);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        // nvfp4: one scale tile a step; mxfp4: two steps share a tile, bytes 0-1 and 2-3
+        const int at = FMT == ICSA_NVFP4 ? ks : ks >> 1;
+        const uint32_t id = FMT == ICSA_NVFP4 ? 0u : uint32_t(ks & 1) * 2u;
+        mma_fp4_elect<FMT>(tmem, ad + uint64_t(ks * 2), wd + uint64_t(ks * 2), make_idesc_fp4<FMT>(256, kCols, id),
+                           sfa + 4u * at, sfb + 8u * at, (kb > t.k0 || ks > 0) ? 1u : 0u);
+      }
+      pair::commit_both_elect(&sm.empty[s]);
+    }
+    pair::commit_both_elect(&sm.acc_full);
+  }
+}
+
+// x / (1 + 2^(-2 u log2 e)), u = sqrt(2/pi) (x + 0.044715 x^3): the tanh form
+// of GELU, 0.5 x (1 + tanh u), without the cancellation at negative x.
+ICSA_DEV float gelu_tanh(float x) {
+  const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
+  const float u = x * fmaf(0.044715f * x, x, 1.0f);
+  return __fdividef(x, 1.0f + attn::ex2(c * u));
+}
+
+ICSA_DEV float finish(const Fp4GemmParams& p, float acc, int c) {
+  float y = acc * p.alpha;
+  if (p.bias != nullptr) y += __bfloat162float(p.bias[c]);
+  if (p.activation == ICSA_ACT_GELU_TANH) y = gelu_tanh(y);
+  return y;
+}
+
+ICSA_DEV void epilogue(const Fp4GemmParams& p, Smem& sm, uint32_t tmem, uint32_t rank) {
+  volatile int* abort_flag = &sm.abort_flag;
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w = warp >> 2;
+  const uint32_t src = tmem + (uint32_t((warp & 3) * 32) << 16) + 128u * uint32_t(w);
+  int count = 0;
+  for (int u = cluster; u < p.units; u += clusters, ++count) {
+    const Unit t = decode_unit(p, u);
+    const bool ok = pair::warp_wait(&sm.acc_full, uint32_t(count) & 1u, nullptr, kErrAccFull, abort_flag);
+    tc::fence_after_sync();
+    float acc[128];
+    attn::tmem_load_row128(src, acc);
+    tc::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) pair::arrive_cluster(pair::mapa(&sm.acc_empty, 0));
+    __syncwarp();
+    const int r = t.mt * (2 * kRows) + int(rank) * kRows + (threadIdx.x & 127);
+    const int c0 = t.nt * kCols + 128 * w;
+    if (!ok || r >= p.M) continue;
+    if (p.splits > 1) {
+      // n_pad is a multiple of 256: whole rows of the tile are stored
+      float4* dst = reinterpret_cast<float4*>(p.partial + (size_t(t.split) * p.M + r) * p.n_pad + c0);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dst[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+      continue;
+    }
+    __nv_bfloat16* dst = p.out + size_t(r) * p.ldo + c0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = c0 + 8 * i;
+      if (c >= p.N) break;
+      if (p.vec_out && c + 8 <= p.N) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = finish(p, acc[8 * i + e], c + e);
+        uint4 o;
+        o.x = pack_bf16x2(y[0], y[1]);
+        o.y = pack_bf16x2(y[2], y[3]);
+        o.z = pack_bf16x2(y[4], y[5]);
+        o.w = pack_bf16x2(y[6], y[7]);
+        *reinterpret_cast<uint4*>(dst + 8 * i) = o;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < p.N) dst[8 * i + e] = __float2bfloat16_rn(finish(p, acc[8 * i + e], c + e));
+      }
+    }
+  }
+}
+
+template <int FMT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    fp4_gemm_kernel(const Fp4GemmParams p, const __grid_constant__ Fp4GemmMaps maps) {
+  extern __shared__ uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair::cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    mbar_init(&sm.acc_full, 1);
+    mbar_init(&sm.acc_empty, 16);  // one arrival per epilogue warp, both CTAs
+    sm.abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == kMmaWarp) {
+    pair::tmem_alloc(&sm.tmem_base, kTmemCols);
+    pair::tmem_relinquish();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.w);
+    prefetch_tensormap(&maps.sa);
+    prefetch_tensormap(&maps.sw);
+  }
+  tc::fence_before_sync();
+  pair::cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = sm.tmem_base;
+  if (warp < 8) {
+    epilogue(p, sm, tmem, rank);
+  } else if (warp == kProducerWarp) {
+    if (lane == 0) {
+      int issued = 0;
+      producer<FMT == ICSA_NVFP4 ? 4 : 2>(p, maps, sm, rank, &issued);
+      if (sm.abort_flag && rank == 0) {
+        // the leader's full barriers count the bytes of both CTAs: let every
+        // copy still in flight land before either CTA releases its memory
+        for (int j = max(0, issued - kStages); j < issued; ++j)
+          attn::drain_wait(&sm.full[j % kStages], uint32_t(j / kStages) & 1u, nullptr);
+      }
+    }
+  } else if (rank == 0) {
+    issuer<FMT>(p, sm, tmem);
+  }
+  __syncwarp();
+  tc::fence_before_sync();
+  pair::cluster_sync();
+  if (warp == kMmaWarp) {
+    tc::fence_after_sync();
+    pair::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// out = bf16(act(alpha * (sum of the splits, in order) + bias))
+__global__ void __launch_bounds__(256) fp4_reduce_kernel(const Fp4GemmParams p) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int r = blockIdx.y;
+  if (c >= p.N) return;
+  float acc = 0.f;
+  for (int s = 0; s < p.splits; ++s) acc += p.partial[(size_t(s) * p.M + r) * p.n_pad + c];
+  p.out[size_t(r) * p.ldo + c] = __float2bfloat16_rn(finish(p, acc, c));
+}
+
+}  // namespace
+
+int fp4_gemm_splits(int M, int N, int K, int num_sms) {
+  const int64_t tiles = int64_t((M + 2 * kRows - 1) / (2 * kRows)) * ((N + kCols - 1) / kCols);
+  const int k_steps = (K + kFp4TileK - 1) / kFp4TileK;
+  const int clusters = std::max(1, num_sms / 2);
+  if (tiles <= 0 || tiles * 2 > clusters || M > 65535) return 1;
+  return int(std::max<int64_t>(1, std::min<int64_t>(clusters / tiles, k_steps)));
+}
+
+cudaError_t launch_fp4_gemm(Fp4GemmParams p, const Fp4GemmMaps& maps, int format, int num_sms, cudaStream_t stream) {
+  p.m_tiles = (p.M + 2 * kRows - 1) / (2 * kRows);
+  p.n_tiles = (p.N + kCols - 1) / kCols;
+  p.k_steps = (p.K + kFp4TileK - 1) / kFp4TileK;
+  p.units = p.m_tiles * p.n_tiles * p.splits;
+  if (p.units == 0) return cudaSuccess;
+  const int clusters = std::max(1, std::min(num_sms / 2, p.units));
+  const size_t smem = sizeof(Smem) + 1024;
+  auto kernel = format == ICSA_NVFP4 ? fp4_gemm_kernel<ICSA_NVFP4> : fp4_gemm_kernel<ICSA_MXFP4>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  kernel<<<2 * clusters, kThreads, smem, stream>>>(p, maps);
+  if ((e = cudaGetLastError()) != cudaSuccess || p.splits == 1) return e;
+  fp4_reduce_kernel<<<dim3((p.N + 255) / 256, p.M), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+ICSA_DEFINE_STICKY_ACCESSOR(sticky_status_fp4)
+
+}  // namespace icsa

@@ -9,6 +9,13 @@ extern "C" void icsa_set_last_error(const char* msg);
 
 namespace icsa {
 
+// TMA descriptors (icsa_capi.cu); on failure the message is set and an
+// icsa_status other than ICSA_OK returned.  rows: bf16 [B, rows, H, D] with
+// 64 x 64 boxes and 128-byte swizzle, rows `row_stride` elements apart.
+int encode_rows_tensor_map(CUtensorMap* m, const void* base, int B, int rows, int H, int D, int64_t row_stride);
+int encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t cols, uint64_t rows,
+                         uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
+
 // ---------------------------------------------------------------- stage 1 --
 struct PoolTensor {
   const void* x;             // [B, S, H, D] input rows (nullptr: skip this tensor)
@@ -105,6 +112,10 @@ struct AttnParams {
   int out_dtype;
   int out_tma;                   // 1: bf16 output written by TMA stores through maps.o
   int* err;
+  // plain attention only (no block table): valid keys per batch element (nullptr: tkv),
+  // and query heads per key/value head (0: one, with kv_lens nullptr)
+  const int* kv_lens;
+  int kv_group;
 };
 
 struct AttnMaps {
@@ -139,5 +150,6 @@ cudaError_t sticky_status_sparse(int** out);
 cudaError_t sticky_status_selftest(int** out);
 cudaError_t sticky_status_gemm(int** out);
 cudaError_t sticky_status_scores(int** out);
+cudaError_t sticky_status_fp4(int** out);
 
 }  // namespace icsa

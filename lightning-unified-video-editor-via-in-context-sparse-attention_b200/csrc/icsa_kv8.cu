@@ -1,0 +1,580 @@
+// Key/value cache in e4m3 with a power-of-two scale for each block of 64
+// tokens and head (storage form in icsa_lowp.h), and the attention of a few
+// query tokens over it.
+//
+// Scales are powers of two, so scaling is exact both ways: a code times its
+// scale is an exact bf16 number, and the only rounding of the cache is the one
+// to e4m3.  Floating-point codes lose nothing by it, as their relative step
+// does not depend on the scale.
+//
+// Attention of few queries (kv8_decode_kernel) is a read of the cache, so it
+// is built around that read: every warp takes whole 64-token blocks by itself
+// and loads their bytes from global memory straight into the registers in
+// which the tensor core wants them, without shared memory or barriers in the
+// loop.  It computes transposed products, S^T = K Q^T and O^T = V^T P^T, so
+// the bytes are the 16-row operand and the queries the 8-column one
+// (mma m16n8k16), and the order of the summed index is free:
+//   * S: the head features are split so that thread t of a quad owns the 16
+//     consecutive bytes 16 t .. 16 t + 15 of each 64-byte half of a key row;
+//   * P.V: V is stored with the tokens of a block innermost, and the keys are
+//     dealt to the rows of S such that thread t needs tokens 16 t .. 16 t + 15,
+//     again 16 consecutive bytes;
+// so a block is read in 16-byte loads of which each covers whole sectors.
+// P^T reaches its operand form with one 8 x 8 transpose (movmatrix) per 8 keys.
+//
+// Both products run in f16 with float32 accumulation: e4m3 codes are exact in
+// f16, a query row is scaled by a power of two to [2^14, 2^15) (bf16 has 8
+// significant bits, f16 11; only elements 2^-28 below the row's largest lose
+// bits), and the probabilities have 11 bits.  The scale of a value block
+// joins the exponent: with s the base-2 scores and v the log2 of the scale,
+//   p = 2^(s + v - m),  m the running maximum of s + v,
+// p enters the product with the codes, and 2^-v p the row sum.
+//
+// Long caches are split over CTAs (and over the warps of a CTA); partial
+// results (unnormalised O, m, sum) are joined in a fixed order.
+#include "icsa_attn_common.cuh"
+#include "icsa_lowp.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+namespace icsa {
+
+namespace {
+
+constexpr int kTokens = 64;
+constexpr int kDWarps = 4;           // warps of a decode CTA
+constexpr float kNegInf = -INFINITY;
+
+ICSA_DEV int valid_tokens(const Kv8Cache& c, int b) {
+  return c.lengths == nullptr ? c.L : min(max(c.lengths[b], 0), c.L);
+}
+
+// two e4m3 bytes (low 16 bits of `pair`) to f16x2
+ICSA_DEV uint32_t e4m3x2_f16x2(uint16_t pair) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(pair));
+  return r;
+}
+ICSA_DEV float2 f16x2_floats(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+
+// two floats to e4m3 bytes (nearest even, saturating), the first in the low byte
+ICSA_DEV uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ---------------------------------------------------------------- filling --
+// One CTA per (block, head, batch) and tensor (grid.y: keys, values).  Thread:
+// 8 consecutive features of tokens 4 i .. 4 i + 3, so that the four tokens'
+// bytes of one feature make a word of the transposed value block.
+template <typename T, int D>
+ICSA_DEV void load8(const T* p, bool vec, float (&v)[8]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(p) + h);
+        v[4 * h] = u.x;
+        v[4 * h + 1] = u.y;
+        v[4 * h + 2] = u.z;
+        v[4 * h + 3] = u.w;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 2) v[i] = __bfloat162float(p[i]);
+    else v[i] = p[i];
+  }
+}
+
+template <int D>
+struct FillShape {
+  static constexpr int kPerRow = D / 8;                   // threads over the features of a token
+  static constexpr int kThreads = 16 * kPerRow;           // 16 groups of 4 tokens
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(FillShape<D>::kThreads) kv8_quantize_kernel(const Kv8Rows x, const Kv8Cache c) {
+  constexpr int kPerRow = FillShape<D>::kPerRow, kThreads = FillShape<D>::kThreads;
+  const int which = blockIdx.y;
+  const int blk = blockIdx.x % c.nb, bh = blockIdx.x / c.nb;
+  const int b = bh / c.H, h = bh % c.H;
+  const int len = valid_tokens(c, b);
+  const int f0 = (threadIdx.x % kPerRow) * 8, g = threadIdx.x / kPerRow;
+  const T* base = static_cast<const T*>(x.x[which]) + b * x.sb[which] + h * x.sh[which] + f0;
+  // 16-byte accesses: every row start and stride aligned
+  const bool vec = (reinterpret_cast<uintptr_t>(x.x[which]) & 15u) == 0 &&
+                   ((x.sb[which] | x.st[which] | x.sh[which]) * int64_t(sizeof(T))) % 16 == 0;
+  float v[4][8];
+  uint32_t top = 0;  // largest magnitude as bits: NaN and infinity stay above every number
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tok = blk * kTokens + 4 * g + i;
+    if (tok < len) {
+      load8<T, D>(base + int64_t(tok) * x.st[which], vec, v[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7FFFFFFFu);
+  }
+  __shared__ uint32_t tops[kThreads / 32];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) top = max(top, tops[i]);
+  // smallest e with amax <= 448 2^e = 1.75 2^(8 + e); a subnormal amax is far
+  // below the clamp at -96
+  int e = int(top >> 23) - 127 - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  e = min(max(e, -96), 96);
+  const bool bad = top >= 0x7F800000u;
+  if (top == 0u || bad) e = 0;
+  const float inv = __uint_as_float(uint32_t(127 - e) << 23);
+  const size_t slot = size_t(bh) * c.nb + blk;
+  if (threadIdx.x == 0)
+    (which ? c.v_scale : c.k_scale)[slot] = bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(uint32_t(127 + e) << 23);
+  uint32_t code[2][4];  // [features 0-3 | 4-7][token], 4 code bytes each
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (bad) {
+      code[0][i] = code[1][i] = 0u;
+      continue;
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      code[q][i] = e4m3x2(v[i][4 * q] * inv, v[i][4 * q + 1] * inv) |
+                   (e4m3x2(v[i][4 * q + 2] * inv, v[i][4 * q + 3] * inv) << 16);
+  }
+  if (which == 0) {
+    uint8_t* dst = c.k + (slot * kTokens + 4 * g) * D + f0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(dst + i * D) = make_uint2(code[0][i], code[1][i]);
+    return;
+  }
+  // values: words of four tokens, [feature][token / 4]
+  __shared__ uint32_t tile[D][17];
+  __syncthreads();
+#pragma unroll
+  for (int e8 = 0; e8 < 8; ++e8) {
+    const uint32_t sel = uint32_t(e8 & 3) | (uint32_t((e8 & 3) + 4) << 4);
+    const uint32_t p01 = __byte_perm(code[e8 >> 2][0], code[e8 >> 2][1], sel);
+    const uint32_t p23 = __byte_perm(code[e8 >> 2][2], code[e8 >> 2][3], sel);
+    tile[f0 + e8][g] = (p01 & 0xFFFFu) | (p23 << 16);
+  }
+  __syncthreads();
+  uint32_t* out = reinterpret_cast<uint32_t*>(c.v + slot * kTokens * D);
+#pragma unroll
+  for (int i = 0; i < D * 16 / kThreads; ++i) {
+    const int wd = i * kThreads + threadIdx.x;
+    out[wd] = tile[wd >> 4][wd & 15];
+  }
+}
+
+// ------------------------------------------------------------- expansion --
+// [B, L, H, D] of T from the cache; rows behind a length are zero whatever
+// the cache holds there.
+template <typename T, int D>
+ICSA_DEV void store8(T* dst, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    uint4 u;
+    u.x = pack_bf16x2(v[0], v[1]);
+    u.y = pack_bf16x2(v[2], v[3]);
+    u.z = pack_bf16x2(v[4], v[5]);
+    u.w = pack_bf16x2(v[6], v[7]);
+    *reinterpret_cast<uint4*>(dst) = u;
+  } else {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(FillShape<D>::kThreads)
+    kv8_dequantize_kernel(const Kv8Cache c, T* k_out, T* v_out) {
+  constexpr int kPerRow = FillShape<D>::kPerRow, kThreads = FillShape<D>::kThreads;
+  const int which = k_out == nullptr ? 1 : int(blockIdx.y);
+  T* out = which ? v_out : k_out;
+  const int blk = blockIdx.x % c.nb, bh = blockIdx.x / c.nb;
+  const int b = bh / c.H, h = bh % c.H;
+  const int len = valid_tokens(c, b);
+  const int f0 = (threadIdx.x % kPerRow) * 8, g = threadIdx.x / kPerRow;
+  const size_t slot = size_t(bh) * c.nb + blk;
+  const bool any = blk * kTokens < len;
+  const float scale = any ? (which ? c.v_scale : c.k_scale)[slot] : 0.f;
+  uint32_t code[2][4] = {};  // [features 0-3 | 4-7][token]
+  __shared__ uint32_t tile[D][17];
+  if (any) {
+    if (which == 0) {
+      const uint8_t* src = c.k + (slot * kTokens + 4 * g) * D + f0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + i * D));
+        code[0][i] = u.x;
+        code[1][i] = u.y;
+      }
+    } else {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(c.v + slot * kTokens * D);
+#pragma unroll
+      for (int i = 0; i < D * 16 / kThreads; ++i) {
+        const int wd = i * kThreads + threadIdx.x;
+        tile[wd >> 4][wd & 15] = __ldg(src + wd);
+      }
+      __syncthreads();
+      // four tokens' bytes of a feature back to one token's bytes of four features
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = tile[f0 + 4 * half + e][g];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t sel = uint32_t(i) | (uint32_t(i + 4) << 4);
+          code[half][i] = (__byte_perm(w[0], w[1], sel) & 0xFFFFu) | (__byte_perm(w[2], w[3], sel) << 16);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tok = blk * kTokens + 4 * g + i;
+    if (tok >= c.L) break;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = f16x2_floats(e4m3x2_f16x2(uint16_t(code[e >> 1][i] >> (16 * (e & 1)))));
+      v[2 * e] = f.x * scale;
+      v[2 * e + 1] = f.y * scale;
+    }
+    if (tok >= len) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    }
+    store8<T, D>(out + ((size_t(b) * c.L + tok) * c.H + h) * D + f0, v);
+  }
+}
+
+// ---------------------------------------------------- attention, few rows --
+ICSA_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+ICSA_DEV uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+ICSA_DEV uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+ICSA_DEV uint4 load_stream16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+ICSA_DEV uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+
+// the bytes of tokens [0, n) of the 16 in `u` (n <= 0: none)
+ICSA_DEV uint4 keep_bytes(uint4 u, int n) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = n - 4 * i;
+    w[i] = k >= 4 ? w[i] : k <= 0 ? 0u : w[i] & (0xFFFFFFFFu >> (8 * (4 - k)));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// exponent of a power of two as a float; NaN stays NaN
+ICSA_DEV float scale_log2(float s) { return s != s ? s : float(int(__float_as_uint(s) >> 23) - 127); }
+
+// Rows of the 8-query tile blockIdx.z of (b, cache head): row r is query
+// token r / group, head h * group + r % group.
+template <int D>
+__global__ void __launch_bounds__(kDWarps * 32) kv8_decode_kernel(const Kv8AttnParams p, const Kv8Cache c) {
+  constexpr int kHalves = D / 64;            // 64-byte halves of a key row
+  constexpr int kSteps = D / 16;             // 16-feature steps of S
+  constexpr int kOTiles = D / 16;            // 16-feature tiles of O^T
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x, bh = blockIdx.y, b = bh / c.H, h = bh % c.H;
+  const int rows = p.Lq * p.group, row0 = blockIdx.z * 8;
+  const int len = valid_tokens(c, b);
+  const int nb = (len + kTokens - 1) / kTokens;
+  const int blk0 = int(int64_t(nb) * split / p.splits), blk1 = int(int64_t(nb) * (split + 1) / p.splits);
+
+  auto q_row = [&](int r) {
+    return p.q + int64_t(b) * p.q_sb + int64_t(r / p.group) * p.q_st + int64_t(h * p.group + r % p.group) * p.q_sh;
+  };
+  // Q^T operand: query row g, features 64 hf + 16 t + 4 j + {0,1 | 2,3} for step 4 hf + j
+  uint32_t qf[kSteps][2];
+  float q_scale;
+  {
+    uint32_t raw[kHalves][8];
+    const bool ok = row0 + g < rows;
+    uint32_t top = 0;
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (ok) u = __ldg(reinterpret_cast<const uint4*>(q_row(row0 + g) + 64 * hf + 16 * t) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) raw[hf][4 * i + k] = word(u, k);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        top = max(top, max(raw[hf][k] & 0x7FFFu, (raw[hf][k] >> 16) & 0x7FFFu));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // scale the row's largest magnitude into [2^14, 2^15); a row with a NaN or
+    // an infinity makes all its scores NaN
+    const int e = min(max(int(top >> 7) - 127 - 14, -126), 126);
+    const float inv = __uint_as_float(uint32_t(127 - e) << 23);
+    q_scale = top >= 0x7F80u ? __uint_as_float(0x7FC00000u) : __uint_as_float(uint32_t(127 + e) << 23);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w = raw[s >> 2][2 * (s & 3) + i];
+        qf[s][i] = pack_f16x2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xFFFF0000u) * inv);
+      }
+  }
+  // columns 2 t, 2 t + 1 of this thread's accumulators
+  float qs[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) qs[i] = __shfl_sync(0xffffffffu, q_scale, (2 * t + i) * 4) * p.scale_log2;
+
+  float o[kOTiles][4];
+#pragma unroll
+  for (int i = 0; i < kOTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+
+  const size_t slot0 = size_t(bh) * c.nb;
+  // key row of S row (tile i, row r): 16 (r' / 2) + 4 i + r' % 2, + 2 for rows r = r' + 8
+  const int key_g = 16 * (g >> 1) + (g & 1);
+  const uint8_t* kbase = c.k + slot0 * kTokens * D + key_g * D + 16 * t;
+  const uint8_t* vbase = c.v + slot0 * kTokens * D + g * kTokens + 16 * t;
+
+  for (int blk = blk0 + warp; blk < blk1; blk += kDWarps) {
+    const uint8_t* kp = kbase + size_t(blk) * kTokens * D;
+    const uint8_t* vp = vbase + size_t(blk) * kTokens * D;
+    uint4 kr[4][2][kHalves];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf) kr[i][r][hf] = load_stream16(kp + (4 * i + 2 * r) * D + 64 * hf);
+    const float ks = c.k_scale[slot0 + blk], lv = scale_log2(c.v_scale[slot0 + blk]);
+    uint4 vr[kOTiles][2];
+#pragma unroll
+    for (int i = 0; i < kOTiles; ++i)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) vr[i][r] = load_stream16(vp + (16 * i + 8 * r) * kTokens);
+
+    float s[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const uint32_t w0 = word(kr[i][0][st >> 2], st & 3), w1 = word(kr[i][1][st >> 2], st & 3);
+        mma_f16(s[i], e4m3x2_f16x2(uint16_t(w0)), e4m3x2_f16x2(uint16_t(w1)), e4m3x2_f16x2(uint16_t(w0 >> 16)),
+                e4m3x2_f16x2(uint16_t(w1 >> 16)), qf[st][0], qf[st][1]);
+      }
+    }
+    const int left = len - blk * kTokens;  // valid tokens of this block
+    float mx[2] = {kNegInf, kNegInf};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // rows g (e < 2) and g + 8, columns 2 t + (e & 1)
+        float x = s[i][e] * (qs[e & 1] * ks) + lv;
+        if (left < kTokens && key_g + 4 * i + 2 * (e >> 1) >= left) x = kNegInf;
+        s[i][e] = x;
+        mx[e & 1] = fmaxf(mx[e & 1], x);
+      }
+    float neg[2], a[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
+      const float mn = fmaxf(m[i], mx[i]);
+      const float ref = mn == kNegInf ? 0.f : mn;
+      a[i] = attn::ex2(m[i] - ref);
+      m[i] = mn;
+      neg[i] = -ref;
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = attn::ex2(s[i][e] + neg[e & 1]);
+        sum[e & 1] += s[i][e];
+      }
+    const float wl = attn::ex2(-lv);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) l[i] = l[i] * a[i] + sum[i] * wl;
+#pragma unroll
+    for (int i = 0; i < kOTiles; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] *= a[e & 1];
+    if (left < kTokens) {
+      // a probability of zero does not hide a NaN code
+#pragma unroll
+      for (int i = 0; i < kOTiles; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) vr[i][r] = keep_bytes(vr[i][r], left - 16 * t);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b0 = transpose8x8(pack_f16x2(s[i][0], s[i][1]));
+      const uint32_t b1 = transpose8x8(pack_f16x2(s[i][2], s[i][3]));
+#pragma unroll
+      for (int d = 0; d < kOTiles; ++d) {
+        const uint32_t w0 = word(vr[d][0], i), w1 = word(vr[d][1], i);
+        mma_f16(o[d], e4m3x2_f16x2(uint16_t(w0)), e4m3x2_f16x2(uint16_t(w1)), e4m3x2_f16x2(uint16_t(w0 >> 16)),
+                e4m3x2_f16x2(uint16_t(w1 >> 16)), b0, b1);
+      }
+    }
+  }
+  // the threads of a column hold different keys: join their sums (m is equal)
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int d = 4; d < 32; d *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+
+  // join the warps: [warp][column][feature]
+  __shared__ float so[kDWarps][8][D + 4];
+  __shared__ float sm[kDWarps][8], sl[kDWarps][8];
+#pragma unroll
+  for (int d = 0; d < kOTiles; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) so[warp][2 * t + (e & 1)][16 * d + g + 8 * (e >> 1)] = o[d][e];
+  if (g == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sm[warp][2 * t + i] = m[i];
+      sl[warp][2 * t + i] = l[i];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 8 * D; i += kDWarps * 32) {
+    const int col = i / D, d = i % D, r = row0 + col;
+    if (r >= rows) break;
+    float mm = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kDWarps; ++w) mm = fmaxf(mm, sm[w][col]);
+    const float ref = mm == kNegInf ? 0.f : mm;
+    float acc = 0.f, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDWarps; ++w) {
+      const float f = attn::ex2(sm[w][col] - ref);
+      acc += so[w][col][d] * f;
+      lt += sl[w][col] * f;
+    }
+    if (p.splits == 1) {
+      const float y = len == 0 ? 0.f : acc / lt;
+      p.out[((size_t(b) * p.Lq + r / p.group) * p.Hq + h * p.group + r % p.group) * D + d] = __float2bfloat16_rn(y);
+    } else {
+      float* dst = p.partial + ((size_t(bh) * rows + r) * p.splits + split) * (D + 2);
+      dst[d] = acc;
+      if (d == 0) {
+        dst[D] = mm;
+        dst[D + 1] = lt;
+      }
+    }
+  }
+}
+
+// joins the splits of one query row; one CTA per (b, cache head, row)
+template <int D>
+__global__ void __launch_bounds__(D) kv8_join_kernel(const Kv8AttnParams p, const Kv8Cache c) {
+  const int rows = p.Lq * p.group;
+  const int r = blockIdx.x, bh = blockIdx.y, b = bh / c.H, h = bh % c.H, d = threadIdx.x;
+  const float* src = p.partial + (size_t(bh) * rows + r) * p.splits * (D + 2);
+  float mm = kNegInf;
+  for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, src[s * (D + 2) + D]);
+  const float ref = mm == kNegInf ? 0.f : mm;
+  float acc = 0.f, lt = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = attn::ex2(src[s * (D + 2) + D] - ref);
+    acc += src[s * (D + 2) + d] * f;
+    lt += src[s * (D + 2) + D + 1] * f;
+  }
+  const float y = valid_tokens(c, b) == 0 ? 0.f : acc / lt;
+  p.out[((size_t(b) * p.Lq + r / p.group) * p.Hq + h * p.group + r % p.group) * D + d] = __float2bfloat16_rn(y);
+}
+
+template <typename T>
+cudaError_t quantize_as(const Kv8Rows& x, const Kv8Cache& c, cudaStream_t stream) {
+  const dim3 grid(unsigned(c.B) * c.H * c.nb, 2);
+  if (c.D == 128) kv8_quantize_kernel<T, 128><<<grid, FillShape<128>::kThreads, 0, stream>>>(x, c);
+  else kv8_quantize_kernel<T, 64><<<grid, FillShape<64>::kThreads, 0, stream>>>(x, c);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t dequantize_as(const Kv8Cache& c, void* const out[2], cudaStream_t stream) {
+  const dim3 grid(unsigned(c.B) * c.H * c.nb, (out[0] != nullptr) + (out[1] != nullptr));
+  T *k = static_cast<T*>(out[0]), *v = static_cast<T*>(out[1]);
+  if (c.D == 128) kv8_dequantize_kernel<T, 128><<<grid, FillShape<128>::kThreads, 0, stream>>>(c, k, v);
+  else kv8_dequantize_kernel<T, 64><<<grid, FillShape<64>::kThreads, 0, stream>>>(c, k, v);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_quantize(const Kv8Rows& x, int dtype, const Kv8Cache& c, cudaStream_t stream) {
+  return dtype == ICSA_BF16 ? quantize_as<__nv_bfloat16>(x, c, stream) : quantize_as<float>(x, c, stream);
+}
+
+cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out_dtype, cudaStream_t stream) {
+  return out_dtype == ICSA_BF16 ? dequantize_as<__nv_bfloat16>(c, out, stream) : dequantize_as<float>(c, out, stream);
+}
+
+int kv8_decode_splits(int B, int H, int rows, int L, int num_sms) {
+  const int64_t ctas = int64_t(B) * H * ((rows + 7) / 8);
+  const int64_t nb = (L + kTokens - 1) / kTokens;
+  // two CTAs per SM; a split keeps at least one block for each warp
+  const int64_t want = 2 * int64_t(num_sms) / std::max<int64_t>(ctas, 1);
+  return int(std::max<int64_t>(1, std::min<int64_t>(want, nb / kDWarps)));
+}
+
+cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream) {
+  const int rows = p.Lq * p.group;
+  const dim3 grid(p.splits, c.B * c.H, (rows + 7) / 8);
+  if (c.D == 128) kv8_decode_kernel<128><<<grid, kDWarps * 32, 0, stream>>>(p, c);
+  else kv8_decode_kernel<64><<<grid, kDWarps * 32, 0, stream>>>(p, c);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || p.splits == 1) return e;
+  const dim3 jgrid(rows, c.B * c.H);
+  if (c.D == 128) kv8_join_kernel<128><<<jgrid, 128, 0, stream>>>(p, c);
+  else kv8_join_kernel<64><<<jgrid, 64, 0, stream>>>(p, c);
+  return cudaGetLastError();
+}
+
+}  // namespace icsa

@@ -22,6 +22,8 @@ import torch.nn.functional as F
 
 from in_context_sparse_attention import _capi
 
+from . import lowp
+
 DIT_EXPORTED = ("icsa_dit_modulated_norm", "icsa_dit_norm_rope", "icsa_dit_norm_rope_pool",
                 "icsa_dit_gated_residual", "icsa_dit_cross_attention", "icsa_dit_linear_residual")
 
@@ -252,6 +254,17 @@ class CudaOps:
             x.stride(0), rows, N, K, rows_per_batch, gp, gbs, _stream()), "icsa_dit_linear_residual")
         return x
 
+    # --- 4-bit linear layers (lowp.py) -------------------------------------
+    @staticmethod
+    def fp4_weight(w, fmt):
+        """An nn.Linear weight [N, K] in 4 bits, with its own global scale for nvfp4."""
+        return lowp.fp4_quantize(w, fmt, lowp.fp4_global_scale(w) if fmt == "nvfp4" else 1.0)
+
+    @staticmethod
+    def fp4_linear(x, w, b=None, activation=None):
+        """bf16 act(x @ w^T + b): x bf16 rows, quantised per call; w from fp4_weight."""
+        return lowp.fp4_linear(x, w, b, activation)
+
     # --- attention ---------------------------------------------------------
     def self_attention(self, q, k, v, alpha, t_seq_len, means=None):
         """In-context sparse attention of the reference's WanSelfAttention
@@ -344,3 +357,13 @@ class CudaOps:
         _capi.check(self.lib.icsa_dit_cross_attention(*args, out.data_ptr(), B, L, Lk, H, D, _stream()),
                     "icsa_dit_cross_attention")
         return out
+
+    @staticmethod
+    def kv8_quantize(k, v, lengths=None):
+        """8-bit cache of the keys and values [B, L, H, D] of a cross-attention (lowp.kv8_quantize)."""
+        return lowp.kv8_quantize(k, v, lengths)
+
+    @staticmethod
+    def kv8_attention(q, cache):
+        """cross_attention over an 8-bit cache (lowp.kv8_attention)."""
+        return lowp.kv8_attention(q, cache)

@@ -1,0 +1,360 @@
+"""Low-precision operators of the DiT: linear layers on microscaled 4-bit
+operands, and a key/value cache held in 8 bits with the attention that reads
+it (include/icsa_lowp.h; the kernels are in libicsa.so, there is no CPU
+fallback).
+
+    w = fp4_quantize(weight, "nvfp4", fp4_global_scale(weight))   # once, [N, K]
+    y = fp4_linear(x, w, bias, activation="gelu_tanh")            # x: bf16 / f32 [M, K]
+
+    cache = kv8_quantize(k, v, lengths)                           # [B, L, H, D]
+    o = kv8_attention(q, cache)                                   # q: bf16 [B, Lq, Hq, D]
+
+Every function takes and returns torch tensors on one CUDA device (which need
+not be the current one) and runs on that device's current stream.  They
+compute values only: no gradient is recorded.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from in_context_sparse_attention import _capi
+
+LOWP_EXPORTED = ("icsa_fp4_data_bytes", "icsa_fp4_scale_bytes", "icsa_fp4_quantize", "icsa_fp4_dequantize",
+                 "icsa_fp4_linear_workspace_size", "icsa_fp4_linear", "icsa_kv8_quantize", "icsa_kv8_dequantize",
+                 "icsa_kv8_attention_workspace_size", "icsa_kv8_attention")
+
+FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
+FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+ACTIVATIONS = {None: 0, "gelu_tanh": 1}
+KV8_TOKENS = 64     # tokens that share a scale
+
+_DT = {torch.bfloat16: _capi.ICSA_BF16, torch.float32: _capi.ICSA_F32}
+
+
+class _Kv8Desc(ctypes.Structure):
+    """Mirror of struct icsa_kv8_cache."""
+    _fields_ = [("B", ctypes.c_int), ("H", ctypes.c_int), ("L", ctypes.c_int), ("D", ctypes.c_int),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("lengths", ctypes.c_void_p)]
+
+
+_lib = None
+
+
+def _load():
+    global _lib
+    if _lib is not None:
+        return _lib
+    lib = _capi.load()
+    for name in LOWP_EXPORTED:
+        if not hasattr(lib, name):
+            raise ImportError(f"{_capi.LIB_PATH} does not export {name}; rebuild it with `python build.py`")
+    vp, i, i64, f, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+    st, desc = ctypes.POINTER(i64), ctypes.POINTER(_Kv8Desc)
+    for name, res, args in (
+            ("icsa_fp4_data_bytes", sz, [i, i]),
+            ("icsa_fp4_scale_bytes", sz, [i, i, i]),
+            ("icsa_fp4_quantize", i, [vp, i, i64, i, i, i, f, vp, vp, vp]),
+            ("icsa_fp4_dequantize", i, [vp, vp, i, i, i, f, vp, i, i64, vp]),
+            ("icsa_fp4_linear_workspace_size", sz, [i, i, i]),
+            ("icsa_fp4_linear", i, [i, vp, vp, f, vp, vp, f, vp, i, vp, i64, i, i, i, vp, sz, vp]),
+            ("icsa_kv8_quantize", i, [desc, vp, vp, i, st, st, vp]),
+            ("icsa_kv8_dequantize", i, [desc, vp, vp, i, vp]),
+            ("icsa_kv8_attention_workspace_size", sz, [desc, i, i]),
+            ("icsa_kv8_attention", i, [desc, vp, st, vp, i, i, vp, sz, vp])):
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, res
+    _lib = lib
+    return lib
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on_cuda(where, *tensors):
+    """The one CUDA device of the tensors (None entries are skipped)."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{where}: expected CUDA tensors")
+        if device is not None and t.device != device:
+            raise ValueError(f"{where}: tensors on {device} and {t.device}")
+        device = t.device
+    return device
+
+
+# ---------------------------------------------------------------------------
+# 4-bit tensors
+# ---------------------------------------------------------------------------
+@dataclass
+class Fp4Tensor:
+    """A [rows, K] tensor in 4-bit storage (layout: include/icsa_lowp.h).
+
+    data:   uint8 [rows, K' / 2], K' = K rounded up to 32, even element in the low half
+    scales: uint8 [ceil(rows / 128), scale tiles along K, 32, 4, 4], row r and
+            scale c of a tile at [r % 32, r // 32, c]
+    """
+    data: torch.Tensor
+    scales: torch.Tensor
+    shape: tuple
+    fmt: str
+    global_scale: float = 1.0
+
+    def __post_init__(self):
+        if self.fmt not in FP4_FORMATS:
+            raise ValueError(f"4-bit format {self.fmt!r}: expected one of {sorted(FP4_FORMATS)}")
+        self.shape = tuple(int(n) for n in self.shape)
+        if len(self.shape) != 2 or self.shape[0] < 0 or self.shape[1] < 1:
+            raise ValueError(f"Fp4Tensor: shape {self.shape} is not [rows, K] with K >= 1")
+        data, scales = fp4_storage(*self.shape, self.fmt)
+        for name, t, want in (("data", self.data, data), ("scales", self.scales, scales)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
+                raise ValueError(f"Fp4Tensor: {name} must be contiguous uint8 {list(want)} for shape {list(self.shape)}")
+        if self.data.device != self.scales.device:
+            raise ValueError("Fp4Tensor: data and scales on different devices")
+        _check_global_scale(self.fmt, self.global_scale)
+
+    @property
+    def device(self):
+        return self.data.device
+
+
+def fp4_storage(rows: int, K: int, fmt: str):
+    """Shapes of `data` and `scales` of a [rows, K] Fp4Tensor."""
+    tiles = 256 // (4 * FP4_BLOCK[fmt])
+    return (rows, -(-K // 32) * 16), (-(-rows // 128), -(-K // 256) * tiles, 32, 4, 4)
+
+
+def _check_global_scale(fmt, g):
+    if not (isinstance(g, (int, float)) and math.isfinite(g) and g > 0):
+        raise ValueError(f"the global scale must be a positive finite number, got {g!r}")
+    if fmt == "mxfp4" and g != 1:
+        raise ValueError("mxfp4 has no global scale (must be 1)")
+
+
+def fp4_global_scale(x: torch.Tensor) -> float:
+    """A global scale for nvfp4: the smallest power of two with which the
+    largest magnitude of x is in range (448 x 6 steps), so that multiplying by
+    it is exact.  Reads x and synchronises: for weights, once."""
+    top = float(x.detach().abs().max()) if x.numel() else 0.0
+    if not math.isfinite(top):
+        raise ValueError("fp4_global_scale: x holds a NaN or an infinity")
+    m, e = math.frexp(top / (6 * 448))
+    return 1.0 if top == 0 else math.ldexp(1.0, max(min(e - (m == 0.5), 100), -100))
+
+
+def _rows2d(where, x):
+    if x.dim() != 2 or x.dtype not in _DT:
+        raise ValueError(f"{where}: expected a 2-D bf16 or f32 tensor, got {x.dtype} {tuple(x.shape)}")
+    if x.shape[1] < 1:
+        raise ValueError(f"{where}: no columns")
+    # rows of contiguous elements, not overlapping
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+
+
+def fp4_quantize(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0) -> Fp4Tensor:
+    """x: bf16 or f32 [rows, K], any strides.  nvfp4: blocks of 16 with e4m3
+    scales e4m3(amax / (6 global_scale)); mxfp4: blocks of 32 with
+    power-of-two scales 2^(floor(log2 amax) - 2)."""
+    if fmt not in FP4_FORMATS:
+        raise ValueError(f"4-bit format {fmt!r}: expected one of {sorted(FP4_FORMATS)}")
+    _check_global_scale(fmt, global_scale)
+    device = _on_cuda("fp4_quantize", x)
+    x, ld = _rows2d("fp4_quantize", x)
+    rows, K = x.shape
+    lib = _load()
+    with torch.cuda.device(device):
+        data, scales = (torch.empty(s, dtype=torch.uint8, device=device) for s in fp4_storage(rows, K, fmt))
+        _capi.check(lib.icsa_fp4_quantize(x.data_ptr(), _DT[x.dtype], ld, rows, K, FP4_FORMATS[fmt],
+                                          float(global_scale), data.data_ptr(), scales.data_ptr(), _stream(device)),
+                    "icsa_fp4_quantize")
+    return Fp4Tensor(data, scales, (rows, K), fmt, float(global_scale))
+
+
+def fp4_dequantize(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """[rows, K] values of a 4-bit tensor, code * (block scale * global scale)."""
+    if dtype not in _DT:
+        raise ValueError(f"fp4_dequantize: dtype {dtype}, expected bf16 or f32")
+    device = _on_cuda("fp4_dequantize", t.data, t.scales)
+    rows, K = t.shape
+    lib = _load()
+    with torch.cuda.device(device):
+        out = torch.empty(rows, K, dtype=dtype, device=device)
+        _capi.check(lib.icsa_fp4_dequantize(t.data.data_ptr(), t.scales.data_ptr(), rows, K, FP4_FORMATS[t.fmt],
+                                            t.global_scale, out.data_ptr(), _DT[dtype], K, _stream(device)),
+                    "icsa_fp4_dequantize")
+    return out
+
+
+def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
+    """bf16 [M, N] = act(x @ w^T + bias) with both operands in 4 bits.
+
+    x: an Fp4Tensor [M, K] of w's format, or bf16 / f32 [M, K], which is
+    quantised to it (global scale 1) first.  w: [N, K].  bias: bf16 [N].
+    activation: None or "gelu_tanh"."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"fp4_linear: activation {activation!r}, expected one of {list(ACTIVATIONS)}")
+    if not isinstance(w, Fp4Tensor):
+        raise ValueError("fp4_linear: w must be an Fp4Tensor (fp4_quantize)")
+    N, K = w.shape
+    if N < 1:
+        raise ValueError("fp4_linear: w has no rows")
+    if tuple(x.shape)[1:] != (K,) or len(x.shape) != 2:
+        raise ValueError(f"fp4_linear: x {tuple(x.shape)} and w {w.shape} differ in K")
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,)):
+        raise ValueError(f"fp4_linear: bias must be bf16 [{N}]")
+    a = x if isinstance(x, Fp4Tensor) else None
+    if a is not None and a.fmt != w.fmt:
+        raise ValueError(f"fp4_linear: x is {a.fmt}, w is {w.fmt}")
+    device = _on_cuda("fp4_linear", *((a.data, a.scales) if a is not None else (x,)), w.data, w.scales, bias)
+    if a is None:
+        a = fp4_quantize(x, w.fmt)
+    if bias is not None:
+        bias = bias.contiguous()
+    M = a.shape[0]
+    lib = _load()
+    with torch.cuda.device(device):
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=device)
+        size = lib.icsa_fp4_linear_workspace_size(M, N, K)
+        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        _capi.check(lib.icsa_fp4_linear(
+            FP4_FORMATS[w.fmt], a.data.data_ptr(), a.scales.data_ptr(), a.global_scale, w.data.data_ptr(),
+            w.scales.data_ptr(), w.global_scale, bias.data_ptr() if bias is not None else None,
+            ACTIVATIONS[activation], out.data_ptr(), N, M, N, K, ws.data_ptr() if size else None, size,
+            _stream(device)), "icsa_fp4_linear")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit key/value cache
+# ---------------------------------------------------------------------------
+@dataclass
+class Kv8Cache:
+    """Keys and values of B sequences in e4m3 (layout: include/icsa_lowp.h).
+
+    k: float8_e4m3fn [B, H, nb, 64, D], v: float8_e4m3fn [B, H, nb, D, 64]
+    (nb blocks of 64 tokens); k_scale, v_scale: f32 [B, H, nb], powers of two;
+    L: tokens the cache has room for; lengths: int32 [B] on the device, the
+    valid tokens of each sequence, or None (all L)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    L: int
+    lengths: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        if self.k.dim() != 5 or self.k.shape[3] != KV8_TOKENS or self.k.shape[4] not in (64, 128):
+            raise ValueError(f"Kv8Cache: k {tuple(self.k.shape)} is not [B, H, nb, 64, D] with D 64 or 128")
+        B, H, nb, T, D = self.k.shape
+        if self.L < 1 or nb != -(-self.L // T):
+            raise ValueError(f"Kv8Cache: {nb} blocks do not hold L={self.L} tokens")
+        for name, t, shape, dt in (("k", self.k, (B, H, nb, T, D), torch.float8_e4m3fn),
+                                   ("v", self.v, (B, H, nb, D, T), torch.float8_e4m3fn),
+                                   ("k_scale", self.k_scale, (B, H, nb), torch.float32),
+                                   ("v_scale", self.v_scale, (B, H, nb), torch.float32)):
+            if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous():
+                raise ValueError(f"Kv8Cache: {name} must be contiguous {dt} {list(shape)}")
+        _check_lengths("Kv8Cache", self.lengths, B)
+        if len({t.device for t in (self.k, self.v, self.k_scale, self.v_scale, self.lengths) if t is not None}) > 1:
+            raise ValueError("Kv8Cache: tensors on different devices")
+
+    @property
+    def device(self):
+        return self.k.device
+
+    def _desc(self):
+        B, H, _, _, D = self.k.shape
+        return _Kv8Desc(B, H, self.L, D, self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                        self.v_scale.data_ptr(), self.lengths.data_ptr() if self.lengths is not None else None)
+
+
+def _check_lengths(where, lengths, B):
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,)
+                                or not lengths.is_contiguous()):
+        raise ValueError(f"{where}: lengths must be contiguous int32 [{B}]")
+
+
+def _strides(t):
+    """Batch, token and head strides; 0 for an axis of one."""
+    return (ctypes.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+
+
+def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> Kv8Cache:
+    """k, v: bf16 or f32 [B, L, H, D] with contiguous features; lengths: int32
+    [B] on the device or None.  One scale for each block of 64 tokens and
+    head, the smallest power of two with which the block's largest magnitude
+    is at most 448.  Tokens behind a length are not read."""
+    device = _on_cuda("kv8_quantize", k, v, lengths)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DT:
+        raise ValueError(f"kv8_quantize: k {tuple(k.shape)} and v {tuple(v.shape)} must be bf16 or f32 [B, L, H, D]")
+    B, L, H, D = k.shape
+    if D not in (64, 128):
+        raise ValueError(f"kv8_quantize: head dim {D} (supported: 64, 128)")
+    if min(B, L, H) < 1:
+        raise ValueError(f"kv8_quantize: empty k, v {tuple(k.shape)}")
+    _check_lengths("kv8_quantize", lengths, B)
+    k, v = (t if t.stride(3) == 1 and min(t.stride()) >= 0 else t.contiguous() for t in (k, v))
+    lib = _load()
+    nb = -(-L // KV8_TOKENS)
+    with torch.cuda.device(device):
+        c = Kv8Cache(torch.empty(B, H, nb, KV8_TOKENS, D, dtype=torch.float8_e4m3fn, device=device),
+                     torch.empty(B, H, nb, D, KV8_TOKENS, dtype=torch.float8_e4m3fn, device=device),
+                     torch.empty(B, H, nb, device=device), torch.empty(B, H, nb, device=device), L, lengths)
+        _capi.check(lib.icsa_kv8_quantize(ctypes.byref(c._desc()), k.data_ptr(), v.data_ptr(), _DT[k.dtype],
+                                          _strides(k), _strides(v), _stream(device)), "icsa_kv8_quantize")
+    return c
+
+
+def kv8_dequantize(cache: Kv8Cache, dtype: torch.dtype = torch.bfloat16):
+    """(k, v) [B, L, H, D], code * scale (exact in bf16); zero behind a length."""
+    if dtype not in _DT:
+        raise ValueError(f"kv8_dequantize: dtype {dtype}, expected bf16 or f32")
+    device = _on_cuda("kv8_dequantize", cache.k, cache.v, cache.k_scale, cache.v_scale, cache.lengths)
+    B, H, _, _, D = cache.k.shape
+    lib = _load()
+    with torch.cuda.device(device):
+        k, v = (torch.empty(B, cache.L, H, D, dtype=dtype, device=device) for _ in range(2))
+        _capi.check(lib.icsa_kv8_dequantize(ctypes.byref(cache._desc()), k.data_ptr(), v.data_ptr(), _DT[dtype],
+                                            _stream(device)), "icsa_kv8_dequantize")
+    return k, v
+
+
+def kv8_attention(q: torch.Tensor, cache: Kv8Cache) -> torch.Tensor:
+    """softmax(q k^T / sqrt(D)) v over the valid tokens of the cache, bf16
+    [B, Lq, Hq, D]; zero for a sequence of length 0.  q: bf16 [B, Lq, Hq, D],
+    Hq a multiple of the cache's heads (query heads h of one group share
+    cache head h // (Hq / H))."""
+    device = _on_cuda("kv8_attention", q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.lengths)
+    B, H, _, _, D = cache.k.shape
+    if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != B or q.shape[3] != D or q.shape[2] % H or not q.shape[2]:
+        raise ValueError(f"kv8_attention: q must be bf16 [{B}, Lq, a multiple of {H}, {D}], got {q.dtype} {tuple(q.shape)}")
+    Lq, Hq = q.shape[1], q.shape[2]
+    lib = _load()
+    with torch.cuda.device(device):
+        out = torch.empty(B, Lq, Hq, D, dtype=torch.bfloat16, device=device)
+        if Lq == 0:
+            return out
+        # rows of a wider GEMM output are taken as they are
+        if (q.stride(3) != 1 or (Hq > 1 and q.stride(2) != D) or (Lq > 1 and q.stride(1) < Hq * D) or q.stride(1) % 8
+                or (B > 1 and q.stride(0) != Lq * q.stride(1)) or q.data_ptr() % 16):
+            q = q.clone(memory_format=torch.contiguous_format)
+        ts = q.stride(1) if Lq > 1 or B > 1 else Hq * D
+        strides = (ctypes.c_int64 * 3)(Lq * ts, ts, D)
+        desc = cache._desc()
+        size = lib.icsa_kv8_attention_workspace_size(ctypes.byref(desc), Lq, Hq)
+        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        _capi.check(lib.icsa_kv8_attention(ctypes.byref(desc), q.data_ptr(), strides, out.data_ptr(), Lq, Hq,
+                                           ws.data_ptr() if size else None, size, _stream(device)),
+                    "icsa_kv8_attention")
+    return out

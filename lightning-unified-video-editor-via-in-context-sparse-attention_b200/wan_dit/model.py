@@ -51,6 +51,9 @@ class WanDiTConfig:
     patch_size: tuple = (1, 2, 2)
     eps: float = 1e-6
     init_std: float = 0.02
+    # operands of the blocks' linear layers: "bf16", or "nvfp4" / "mxfp4"
+    # (weights held in 4 bits, activations quantised per call)
+    linear_format: str = "bf16"
 
     @property
     def head_dim(self) -> int:
@@ -96,8 +99,19 @@ class _Block:
         self.wc_o, self.bc_o = w(C, C), zeros(C)
         self.w1, self.b1 = w(Fd, C), zeros(Fd)
         self.w2, self.b2 = w(C, Fd), zeros(C)
+        self.fp4 = {}      # 4-bit weights by name, in place of the bf16 ones
         # modulation: randn / sqrt(dim) (model.py:246), kept in bf16 like the model's parameters
         self.modulation = (torch.randn(6, C, generator=g, device=device) / C ** 0.5).to(torch.bfloat16)
+
+
+    # the layers that linear_format applies to
+    LINEARS = ("w_qkv", "w_o", "wc_q", "wc_kv", "wc_o", "w1", "w2")
+
+    def quantize_linears(self, ops, fmt: str):
+        """Replaces the bf16 weights of the linear layers by 4-bit ones."""
+        for name in self.LINEARS:
+            self.fp4[name] = ops.fp4_weight(getattr(self, name), fmt)
+            setattr(self, name, None)
 
 
 class WanDiT:
@@ -154,7 +168,14 @@ class WanDiT:
         self.w_time1, self.b_time1 = w(C, cfg.freq_dim), zeros(C)
         self.w_time2, self.b_time2 = w(C, C), zeros(C)
         self.w_tproj, self.b_tproj = w(6 * C, C), zeros(6 * C)
-        self.blocks = [_Block(cfg, g, self.device) for _ in range(cfg.num_layers)]
+        if cfg.linear_format not in ("bf16", "nvfp4", "mxfp4"):
+            raise ValueError(f"linear_format {cfg.linear_format!r}: expected 'bf16', 'nvfp4' or 'mxfp4'")
+        self.blocks = []
+        for _ in range(cfg.num_layers):
+            blk = _Block(cfg, g, self.device)
+            if cfg.linear_format != "bf16":
+                blk.quantize_linears(ops, cfg.linear_format)
+            self.blocks.append(blk)
         self.w_head, self.b_head = w(cfg.out_dim * p, C), zeros(cfg.out_dim * p)
         self.head_modulation = (torch.randn(2, C, generator=g, device=self.device) / C ** 0.5).to(torch.bfloat16)
         self.rope_table = rope_mod.rope_table(D).to(self.device)
@@ -242,13 +263,54 @@ class WanDiT:
         return r.permute(0, 2, 1, 3, 4).reshape(B * s, n * hp * D)
 
     # ------------------------------------------------------------------
+    # linear layers of a block, in the configured format
+    # ------------------------------------------------------------------
+    def _linear(self, blk: _Block, w: str, b: str, x, activation=None):
+        """bf16 act(x @ w^T + b); w, b: names of the block's weight and bias."""
+        if w in blk.fp4:
+            return self.ops.fp4_linear(x, blk.fp4[w], getattr(blk, b), activation)
+        y = self.ops.linear(x, getattr(blk, w), getattr(blk, b))
+        return self.ops.gelu_tanh(y) if activation == "gelu_tanh" else y
+
+    def _linear_residual_(self, blk: _Block, w: str, b: str, x, a, gate, rows_per_batch):
+        """x += (a @ w^T + b) * gate in place (gate None: + ...)."""
+        if w in blk.fp4:
+            self.ops.gated_residual_(x, self.ops.fp4_linear(a, blk.fp4[w], getattr(blk, b)), gate, rows_per_batch)
+        else:
+            self.ops.linear_residual_(x, a, getattr(blk, w), getattr(blk, b), gate, rows_per_batch)
+
+    def _text_kv(self, blk: _Block, ctx):
+        """Normalised keys and the values [B, L, H, D] of the text tokens
+        (WanT2VCrossAttention, model.py:181-186)."""
+        cfg = self.cfg
+        C, H, D = cfg.dim, cfg.num_heads, cfg.head_dim
+        B, L, _ = ctx.shape
+        kv = self._linear(blk, "wc_kv", "bc_kv", ctx.reshape(B * L, C))
+        kn = torch.empty(B, 1, L, H, D, dtype=torch.bfloat16, device=ctx.device)
+        self.ops.norm_rope([(kv[:, :C], blk.cnorm_k, False, kn)], rows_per_batch=L, eps=cfg.eps)
+        return kn.view(B, L, H, D), kv[:, C:].view(B, L, H, D)
+
+    def text_cache(self, context: torch.Tensor, lengths=None):
+        """Keys and values of the prompts for every block, in 8 bits: one
+        Kv8Cache per block, to pass to `forward` / `denoise_step` instead of
+        the context.  The text does not change over the denoising steps, so
+        one cache serves them all.
+
+        context: [B, text_len, text_dim]; lengths: int32 [B] on the device,
+        the valid text tokens of each prompt (the k_lens of the reference's
+        flash_attention, wanx/attention.py:18-85), or None: all of them."""
+        ctx = self.text_embed(context)
+        return [self.ops.kv8_quantize(*self._text_kv(blk, ctx), lengths) for blk in self.blocks]
+
+    # ------------------------------------------------------------------
     # one block
     # ------------------------------------------------------------------
-    def block_forward(self, blk: _Block, x, e0, ctx, t_seq_len: int, first: bool = False):
+    def block_forward(self, blk: _Block, x, e0, ctx, t_seq_len: int, first: bool = False, cache=None):
         """WanAttentionBlock.forward (model.py:248-269) on this rank's tokens.
         x: f32 [B*s, C] (bf16 for the first block, whose LayerNorm output the
         reference rounds to the residual stream's bf16); returns the new f32
-        residual stream."""
+        residual stream.  cache: the block's 8-bit text keys and values
+        (`text_cache`), read instead of ctx."""
         cfg, ops = self.cfg, self.ops
         C, H, D = cfg.dim, cfg.num_heads, cfg.head_dim
         B = e0.shape[0]
@@ -267,32 +329,31 @@ class WanDiT:
         elif n == 1 and self.pooled_exchange and s % 64 == 0:
             self._self_attention_local_pooled(blk, xin, B, s, t_seq_len, x, e["gate0"])
         else:
-            qkv = ops.linear(xin, blk.w_qkv, blk.b_qkv)
+            qkv = self._linear(blk, "w_qkv", "b_qkv", xin)
             q, k, v, gate = self._qkv(blk, qkv, B, s)
             del xin, qkv
             qf, kf, vf, alpha = self._exchange_in(q, k, v, gate)
             del q, k, v
             o = ops.self_attention(qf, kf, vf, alpha, t_seq_len)
             del qf, kf, vf
-            ops.linear_residual_(x, self._exchange_out(o), blk.w_o, blk.b_o, e["gate0"], s)
+            self._linear_residual_(blk, "w_o", "b_o", x, self._exchange_out(o), e["gate0"], s)
             del o
 
         # cross-attention (model.py:262, WanT2VCrossAttention :181-188)
         xn = ops.modulated_norm(x, blk.norm3_w, blk.norm3_b, s, cfg.eps)
-        qc = ops.linear(xn, blk.wc_q, blk.bc_q)
-        L = ctx.shape[1]
-        kv = ops.linear(ctx.reshape(B * L, C), blk.wc_kv, blk.bc_kv)
+        qc = self._linear(blk, "wc_q", "bc_q", xn)
         qn = torch.empty(B, 1, s, H, D, dtype=torch.bfloat16, device=dev)
-        kn = torch.empty(B, 1, L, H, D, dtype=torch.bfloat16, device=dev)
         ops.norm_rope([(qc, blk.cnorm_q, False, qn)], rows_per_batch=s, eps=cfg.eps)
-        ops.norm_rope([(kv[:, :C], blk.cnorm_k, False, kn)], rows_per_batch=L, eps=cfg.eps)
-        oc = ops.cross_attention(qn.view(B, s, H, D), kn.view(B, L, H, D), kv[:, C:].view(B, L, H, D))
-        ops.linear_residual_(x, oc.reshape(B * s, C), blk.wc_o, blk.bc_o, None, s)
+        if cache is not None:
+            oc = ops.kv8_attention(qn.view(B, s, H, D), cache)
+        else:
+            oc = ops.cross_attention(qn.view(B, s, H, D), *self._text_kv(blk, ctx))
+        self._linear_residual_(blk, "wc_o", "bc_o", x, oc.reshape(B * s, C), None, s)
 
         # FFN (model.py:263-265)
         xn = ops.modulated_norm(x, e["scale1"], e["shift1"], s, cfg.eps)
-        h = ops.gelu_tanh(ops.linear(xn, blk.w1, blk.b1))
-        ops.linear_residual_(x, h, blk.w2, blk.b2, e["gate1"], s)
+        h = self._linear(blk, "w1", "b1", xn, "gelu_tanh")
+        self._linear_residual_(blk, "w2", "b2", x, h, e["gate1"], s)
         del h
         return x
 
@@ -347,7 +408,7 @@ class WanDiT:
         ops, cfg = self.ops, self.cfg
         C, H, D = cfg.dim, cfg.num_heads, cfg.head_dim
         for b in range(B):
-            qkv = ops.linear(xin[b * s:(b + 1) * s], blk.w_qkv, blk.b_qkv)
+            qkv = self._linear(blk, "w_qkv", "b_qkv", xin[b * s:(b + 1) * s])
             q, k, v, gate, stats = self._qkv_pooled(blk, qkv, s)
             del qkv
             # [1, 1, H, s/64, D] -> [1, H, s/64, D]
@@ -355,7 +416,7 @@ class WanDiT:
             o = ops.self_attention(q.view(1, s, H, D), k.view(1, s, H, D), v.view(1, s, H, D), gate.view(1, s),
                                    t_seq_len, means=means)
             del q, k, v
-            ops.linear_residual_(x[b * s:(b + 1) * s], o.view(s, C), blk.w_o, blk.b_o, res_gate[b:b + 1], s)
+            self._linear_residual_(blk, "w_o", "b_o", x[b * s:(b + 1) * s], o.view(s, C), res_gate[b:b + 1], s)
 
     def _self_attention_pipelined(self, blk: _Block, xin, B, s, t_seq_len, x, res_gate):
         """Ulysses self-attention with the exchanges of one batch element
@@ -382,7 +443,7 @@ class WanDiT:
         qdt = torch.bfloat16 if pooled else torch.float32
         inbound = []
         for b in range(B):
-            qkv = ops.linear(xin[b * s:(b + 1) * s], blk.w_qkv, blk.b_qkv)
+            qkv = self._linear(blk, "w_qkv", "b_qkv", xin[b * s:(b + 1) * s])
             if pooled:
                 q, k, v, gate, stats = self._qkv_pooled(blk, qkv, s)
             else:
@@ -419,8 +480,8 @@ class WanDiT:
         for b in range(B):
             work, r = outbound[b]
             work.wait()
-            ops.linear_residual_(x[b * s:(b + 1) * s], r.permute(1, 0, 2, 3).reshape(s, C), blk.w_o, blk.b_o,
-                                 res_gate[b:b + 1], s)
+            self._linear_residual_(blk, "w_o", "b_o", x[b * s:(b + 1) * s], r.permute(1, 0, 2, 3).reshape(s, C),
+                                   res_gate[b:b + 1], s)
 
     @staticmethod
     def e_block(blk: _Block, e0):
@@ -433,16 +494,20 @@ class WanDiT:
     # ------------------------------------------------------------------
     # whole model
     # ------------------------------------------------------------------
-    def forward(self, latent, source_latent, t, context, seq_len: int):
+    def forward(self, latent, source_latent, t, context, seq_len: int, text_cache=None):
         """Noise prediction for a batch of CFG branches sharing one latent.
 
         latent, source_latent: f32 [C_in, F, H, W] (replicated on every rank);
         t: timestep (python number or 0-d tensor); context: [B, text_len,
         text_dim] (one text embedding per branch); seq_len: joint tokens,
-        divisible by the world size.  Returns f32 [B, out_dim, F, H, W] on
+        divisible by the world size.  text_cache: the blocks' 8-bit text keys
+        and values (`text_cache`), read instead of the context, which may then
+        be None.  Returns f32 [B, out_dim, F, H, W] on
         every rank (model.py:410-451)."""
         cfg = self.cfg
-        B = context.shape[0]
+        if text_cache is not None and len(text_cache) != len(self.blocks):
+            raise ValueError(f"text_cache holds {len(text_cache)} blocks, the model has {len(self.blocks)}")
+        B = context.shape[0] if text_cache is None else text_cache[0].k.shape[0]
         if seq_len % self.world:
             raise ValueError(f"seq_len={seq_len} does not split over {self.world} ranks")
         x_all, grid, sgrid = self.embed(latent, source_latent, seq_len)
@@ -453,9 +518,10 @@ class WanDiT:
         tt = torch.as_tensor(t, dtype=torch.float64, device=self.device).reshape(1)
         e, e0 = self.time_embed(tt)
         e, e0 = e.expand(B, -1), e0.expand(B, -1, -1)
-        ctx = self.text_embed(context)
+        ctx = self.text_embed(context) if text_cache is None else None
         for i, blk in enumerate(self.blocks):
-            x = self.block_forward(blk, x, e0, ctx, t_seq_len, first=(i == 0))
+            x = self.block_forward(blk, x, e0, ctx, t_seq_len, first=(i == 0),
+                                   cache=text_cache[i] if text_cache is not None else None)
         return self.head(x, e, B, s, grid, seq_len)
 
     def head(self, x, e, B, s, grid, seq_len):
@@ -477,19 +543,19 @@ class WanDiT:
         return u.reshape(B, cfg.out_dim, f * pf, h * ph, w * pw)
 
     def denoise_step(self, latent, source_latent, t, sigma, sigma_next, context, seq_len, guidance_scale=2.5,
-                     check_status=True):
+                     check_status=True, text_cache=None):
         """One denoising step of the reference's loop (inference.py:266-291):
         both CFG branches in one batch (context[0] unconditional, context[1]
         conditional), noise = uncond + g * (cond - uncond), then a
         flow-matching Euler update latent + (sigma_next - sigma) * noise,
         which stands in for the reference's UniPC solver (a few elementwise
-        ops on the latent).
+        ops on the latent).  text_cache: of both branches, as in `forward`.
 
         check_status: after the step, synchronise and raise IcsaError if a
         bounded wait inside any attention kernel of the step gave up (the
         per-device record of icsa_last_status); skipped while the stream is
         being captured into a CUDA graph."""
-        out = self.forward(latent, source_latent, t, context, seq_len)
+        out = self.forward(latent, source_latent, t, context, seq_len, text_cache)
         noise = out[0] + guidance_scale * (out[1] - out[0])
         new = latent + (sigma_next - sigma) * noise
         if check_status and not torch.cuda.is_current_stream_capturing():
