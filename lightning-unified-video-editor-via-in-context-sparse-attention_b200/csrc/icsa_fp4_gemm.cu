@@ -60,6 +60,8 @@ struct __align__(1024) Smem {
   uint8_t w[kStages][kOpBytes];
   uint8_t sa[kStages][4 * kScaleAtomBytes];
   uint8_t sw[kStages][8 * kScaleAtomBytes];
+  uint8_t out[8][32 * 128];   // output box of each epilogue warp
+  float bias[2][128];
   uint64_t full[kStages], empty[kStages];
   uint64_t acc_full, acc_empty;
   uint32_t tmem_base;
@@ -131,16 +133,34 @@ ICSA_DEV uint64_t scale_desc(uint32_t saddr) {
   return d;
 }
 
-// Four TMEM columns (32 lanes x 16 bytes, repeated in the four lane
-// quadrants) from one scale tile, in both CTAs of the pair.
-ICSA_DEV void copy_scales_elect(uint32_t taddr, uint64_t desc) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
-      "l"(desc)
-      : "memory");
+// The scales of one K step to TMEM, in both CTAs of the pair: a scale tile
+// fills four columns (32 lanes x 16 bytes, repeated in the four lane
+// quadrants); a's tiles go to sfa + 4 i, the weight's first and second 128
+// rows to sfa + 16 + 8 i and + 4.  One election for all copies keeps the
+// issuing warp short.
+#define ICSA_CP(T, D, OFF_T, OFF_D)                                      \
+  "add.u32 t, " T ", " #OFF_T ";\n\tadd.s64 d, " D ", " #OFF_D ";\n\t" \
+  "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], d;\n\t"
+template <int ATOMS>
+ICSA_DEV void copy_scales_elect(uint32_t sfa, uint64_t sa_desc, uint64_t sw_desc) {
+  if constexpr (ATOMS == 4) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b32 t;\n\t.reg .b64 d;\n\telect.sync _|e, 0xffffffff;\n\t"
+        ICSA_CP("%0", "%1", 0, 0) ICSA_CP("%0", "%2", 16, 0) ICSA_CP("%0", "%2", 20, 128)
+        ICSA_CP("%0", "%1", 4, 32) ICSA_CP("%0", "%2", 24, 32) ICSA_CP("%0", "%2", 28, 160)
+        ICSA_CP("%0", "%1", 8, 64) ICSA_CP("%0", "%2", 32, 64) ICSA_CP("%0", "%2", 36, 192)
+        ICSA_CP("%0", "%1", 12, 96) ICSA_CP("%0", "%2", 40, 96) ICSA_CP("%0", "%2", 44, 224)
+        "}" ::"r"(sfa), "l"(sa_desc), "l"(sw_desc) : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b32 t;\n\t.reg .b64 d;\n\telect.sync _|e, 0xffffffff;\n\t"
+        ICSA_CP("%0", "%1", 0, 0) ICSA_CP("%0", "%2", 16, 0) ICSA_CP("%0", "%2", 20, 64)
+        ICSA_CP("%0", "%1", 4, 32) ICSA_CP("%0", "%2", 24, 32) ICSA_CP("%0", "%2", 28, 96)
+        "}" ::"r"(sfa), "l"(sa_desc), "l"(sw_desc) : "memory");
+  }
 }
+#undef ICSA_CP
+static_assert(kScaleAtomBytes >> 4 == 32 && kTmSfb == 16, "offsets of copy_scales_elect");
 
 // Instruction descriptor of the block-scaled kinds with e2m1 operands.
 template <int FMT>
@@ -202,13 +222,7 @@ ICSA_DEV void issuer(const Fp4GemmParams& p, Smem& sm, uint32_t tmem) {
       const uint32_t sfa = tmem + kTmScale + uint32_t(it & 1) * kTmScaleStep, sfb = sfa + kTmSfb;
       const uint64_t sad = sad0 + uint64_t(s) * (4 * kScaleAtomBytes >> 4);
       const uint64_t swd = swd0 + uint64_t(s) * (8 * kScaleAtomBytes >> 4);
-#pragma unroll
-      for (int at = 0; at < kAtoms; ++at) {
-        // a scale tile holds 128 rows; the weight's second 128 rows follow its first
-        copy_scales_elect(sfa + 4u * at, sad + uint64_t(at) * (kScaleAtomBytes >> 4));
-        copy_scales_elect(sfb + 8u * at, swd + uint64_t(at) * (kScaleAtomBytes >> 4));
-        copy_scales_elect(sfb + 8u * at + 4u, swd + uint64_t(kAtoms + at) * (kScaleAtomBytes >> 4));
-      }
+      copy_scales_elect<kAtoms>(sfa, sad, swd);
       const uint64_t ad = ad0 + uint64_t(s) * (kOpBytes >> 4), wd = wd0 + uint64_t(s) * (kOpBytes >> 4);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
@@ -224,70 +238,102 @@ ICSA_DEV void issuer(const Fp4GemmParams& p, Smem& sm, uint32_t tmem) {
   }
 }
 
-// x / (1 + 2^(-2 u log2 e)), u = sqrt(2/pi) (x + 0.044715 x^3): the tanh form
-// of GELU, 0.5 x (1 + tanh u), without the cancellation at negative x.
+// The tanh form of GELU, 0.5 x (1 + tanh u), u = sqrt(2/pi) (x + 0.044715 x^3),
+// as x / (1 + 2^(-2 u log2 e)): no cancellation at negative x, two
+// multi-function operations.
 ICSA_DEV float gelu_tanh(float x) {
-  const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
-  const float u = x * fmaf(0.044715f * x, x, 1.0f);
-  return __fdividef(x, 1.0f + attn::ex2(c * u));
+  constexpr float c1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
+  constexpr float c3 = c1 * 0.044715f;
+  return __fdividef(x, 1.0f + attn::ex2(x * fmaf(c3 * x, x, c1)));
 }
 
-ICSA_DEV float finish(const Fp4GemmParams& p, float acc, int c) {
-  float y = acc * p.alpha;
-  if (p.bias != nullptr) y += __bfloat162float(p.bias[c]);
-  if (p.activation == ICSA_ACT_GELU_TANH) y = gelu_tanh(y);
-  return y;
+ICSA_DEV float finish(const Fp4GemmParams& p, float acc, float bias) {
+  const float y = fmaf(acc, p.alpha, bias);
+  return p.activation == ICSA_ACT_GELU_TANH ? gelu_tanh(y) : y;
 }
 
-ICSA_DEV void epilogue(const Fp4GemmParams& p, Smem& sm, uint32_t tmem, uint32_t rank) {
+// Epilogue warps: thread <-> TMEM lane <-> output row, warpgroup w columns
+// [128 w, 128 w + 128) of the tile.  The row goes to registers in one piece,
+// so the accumulator is free again after one TMEM read; the output leaves in
+// 32-row x 64-column boxes staged in shared memory (one 4 KB box a warp,
+// 128-byte swizzle) and written by TMA, which stores whole lines and clips
+// the tile at M and N.  (Storing the rows straight from registers, 16 bytes
+// a lane in 32 different lines, took 8600 clk a tile, more than half of a
+// K = 5120 main loop.)
+ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm, uint32_t tmem, uint32_t rank) {
   volatile int* abort_flag = &sm.abort_flag;
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int w = warp >> 2;
   const uint32_t src = tmem + (uint32_t((warp & 3) * 32) << 16) + 128u * uint32_t(w);
+  uint8_t* box = sm.out[warp];
+  float* bias = sm.bias[w];
+  const uint32_t acc_empty = pair::mapa(&sm.acc_empty, 0);
   int count = 0;
   for (int u = cluster; u < p.units; u += clusters, ++count) {
     const Unit t = decode_unit(p, u);
+    const int row0 = t.mt * (2 * kRows) + int(rank) * kRows + 32 * (warp & 3), r = row0 + lane;
+    const int c0 = t.nt * kCols + 128 * w;
+    {
+      const int c = c0 + int(threadIdx.x & 127);
+      const float bv = p.bias != nullptr && c < p.N ? __bfloat162float(p.bias[c]) : 0.f;
+      pair::named_sync(1u + uint32_t(w), 128);  // the last tile's bias has been read
+      bias[threadIdx.x & 127] = bv;
+      pair::named_sync(1u + uint32_t(w), 128);
+    }
     const bool ok = pair::warp_wait(&sm.acc_full, uint32_t(count) & 1u, nullptr, kErrAccFull, abort_flag);
     tc::fence_after_sync();
     float acc[128];
     attn::tmem_load_row128(src, acc);
     tc::fence_before_sync();
     __syncwarp();
-    if (lane == 0) pair::arrive_cluster(pair::mapa(&sm.acc_empty, 0));
+    if (lane == 0) pair::arrive_cluster_relaxed(acc_empty);
     __syncwarp();
-    const int r = t.mt * (2 * kRows) + int(rank) * kRows + (threadIdx.x & 127);
-    const int c0 = t.nt * kCols + 128 * w;
-    if (!ok || r >= p.M) continue;
+    if (!ok || row0 >= p.M) continue;
     if (p.splits > 1) {
+      if (r >= p.M) continue;
       // n_pad is a multiple of 256: whole rows of the tile are stored
       float4* dst = reinterpret_cast<float4*>(p.partial + (size_t(t.split) * p.M + r) * p.n_pad + c0);
 #pragma unroll
       for (int i = 0; i < 32; ++i) dst[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
       continue;
     }
+    if (p.tma_out) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (c0 + 64 * h >= p.N) break;
+        // the box's previous contents have been read by their store
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 b0 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i);
+          const float4 b1 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i + 4);
+          const float* x = acc + 64 * h + 8 * i;
+          uint4 o;
+          o.x = pack_bf16x2(finish(p, x[0], b0.x), finish(p, x[1], b0.y));
+          o.y = pack_bf16x2(finish(p, x[2], b0.z), finish(p, x[3], b0.w));
+          o.z = pack_bf16x2(finish(p, x[4], b1.x), finish(p, x[5], b1.y));
+          o.w = pack_bf16x2(finish(p, x[6], b1.z), finish(p, x[7], b1.w));
+          *reinterpret_cast<uint4*>(box + lane * 128 + ((uint32_t(i) ^ uint32_t(lane & 7)) << 4)) = o;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&maps.out, box, c0 + 64 * h, row0);
+          bulk_commit();
+        }
+      }
+      continue;
+    }
+    // an output whose rows are not 16-byte aligned
+    if (r >= p.M) continue;
     __nv_bfloat16* dst = p.out + size_t(r) * p.ldo + c0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int c = c0 + 8 * i;
-      if (c >= p.N) break;
-      if (p.vec_out && c + 8 <= p.N) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = finish(p, acc[8 * i + e], c + e);
-        uint4 o;
-        o.x = pack_bf16x2(y[0], y[1]);
-        o.y = pack_bf16x2(y[2], y[3]);
-        o.z = pack_bf16x2(y[4], y[5]);
-        o.w = pack_bf16x2(y[6], y[7]);
-        *reinterpret_cast<uint4*>(dst + 8 * i) = o;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < p.N) dst[8 * i + e] = __float2bfloat16_rn(finish(p, acc[8 * i + e], c + e));
-      }
-    }
+    for (int i = 0; i < 128; ++i)
+      if (c0 + i < p.N) dst[i] = __float2bfloat16_rn(finish(p, acc[i], bias[i]));
   }
+  if (lane == 0) bulk_wait_read();
 }
 
 template <int FMT>
@@ -322,7 +368,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
   if (warp < 8) {
-    epilogue(p, sm, tmem, rank);
+    epilogue(p, maps, sm, tmem, rank);
   } else if (warp == kProducerWarp) {
     if (lane == 0) {
       int issued = 0;
@@ -353,7 +399,7 @@ __global__ void __launch_bounds__(256) fp4_reduce_kernel(const Fp4GemmParams p) 
   if (c >= p.N) return;
   float acc = 0.f;
   for (int s = 0; s < p.splits; ++s) acc += p.partial[(size_t(s) * p.M + r) * p.n_pad + c];
-  p.out[size_t(r) * p.ldo + c] = __float2bfloat16_rn(finish(p, acc, c));
+  p.out[size_t(r) * p.ldo + c] = __float2bfloat16_rn(finish(p, acc, p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.f));
 }
 
 }  // namespace

@@ -52,6 +52,7 @@ cudaError_t launch_fp4_dequantize(const Fp4DequantParams& p, int out_dtype, int 
 struct Fp4GemmMaps {
   CUtensorMap a, w;      // uint8 [rows, row bytes], box {128 bytes, 128 rows}, 128-byte swizzle
   CUtensorMap sa, sw;    // uint32 [scale tiles, 128], box {128, scale tiles of one K tile}
+  CUtensorMap out;       // bf16 [M, ldo], box {64, 32}, 128-byte swizzle (when tma_out)
 };
 struct Fp4GemmParams {
   int M, N, K;
@@ -64,7 +65,7 @@ struct Fp4GemmParams {
   int n_pad;
   int splits;
   int m_tiles, n_tiles, units, k_steps;
-  int vec_out;                 // 16-byte stores of the output are aligned
+  int tma_out;                 // the output's rows are 16-byte aligned: written by TMA
 };
 // Splits of K for an M x N x K product on `num_sms` SMs (1: none).
 int fp4_gemm_splits(int M, int N, int K, int num_sms);

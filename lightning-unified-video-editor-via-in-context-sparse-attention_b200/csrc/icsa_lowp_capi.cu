@@ -223,7 +223,7 @@ int icsa_fp4_linear(int format, const void* a_data, const void* a_scales, float 
   p.activation = activation;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ldo = ldo;
-  p.vec_out = aligned(out, 16) && ldo % 8 == 0;
+  p.tma_out = aligned(out, 16) && ldo % 8 == 0;
   p.splits = icsa::fp4_gemm_splits(M, N, K, sms);
   p.n_pad = fp4_n_pad(N);
   if (p.splits > 1) {
@@ -237,6 +237,11 @@ int icsa_fp4_linear(int format, const void* a_data, const void* a_scales, float 
   icsa::Fp4GemmMaps maps;
   if ((rc = encode_fp4_maps(&maps.a, &maps.sa, a_data, a_scales, format, M, K)) != ICSA_OK) return rc;
   if ((rc = encode_fp4_maps(&maps.w, &maps.sw, w_data, w_scales, format, N, K)) != ICSA_OK) return rc;
+  std::memset(&maps.out, 0, sizeof(maps.out));
+  if (p.tma_out && (rc = icsa::encode_tensor_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, uint64_t(N),
+                                                    uint64_t(M), uint64_t(ldo) * 2, 64, 32,
+                                                    CU_TENSOR_MAP_SWIZZLE_128B)) != ICSA_OK)
+    return rc;
   cudaError_t e = icsa::launch_fp4_gemm(p, maps, format, sms, stream);
   return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_linear");
 }
