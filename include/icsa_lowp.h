@@ -76,6 +76,16 @@ ICSA_API int icsa_fp4_linear(int format, const void* a_data, const void* a_scale
                              size_t workspace_bytes, cudaStream_t stream);
 
 /*
+ * The same for x of ICSA_BF16 or ICSA_F32 (rows ldx elements apart), which is
+ * quantised to the weight's format (global scale 1) in the workspace first.
+ */
+ICSA_API size_t icsa_fp4_linear_rows_workspace_size(int format, int M, int N, int K);
+ICSA_API int icsa_fp4_linear_rows(int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
+                                  const void* w_scales, float w_global_scale, const void* bias, int activation,
+                                  void* out, int64_t ldo, int M, int N, int K, void* workspace,
+                                  size_t workspace_bytes, cudaStream_t stream);
+
+/*
  * Key/value cache in e4m3 with one power-of-two scale for each block of 64
  * tokens and head.  nb = ceil(L / 64).
  *   k: [B, H, nb, 64, D] bytes;  v: [B, H, nb, D, 64] bytes (a block's tokens

@@ -59,30 +59,101 @@ template <>
 ICSA_DEV float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
   return __bfloat162float(v);
 }
+template <typename T>
+ICSA_DEV T from_float(float v);
+template <>
+ICSA_DEV float from_float<float>(float v) {
+  return v;
+}
+template <>
+ICSA_DEV __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
 
-// 16 consecutive elements of a row from column k0; zeros from column K on
-template <typename T, bool VEC>
-ICSA_DEV void load16(const T* row, int k0, int K, float (&v)[16]) {
-  if (VEC && k0 + 16 <= K) {
-    if constexpr (sizeof(T) == 2) {
-      const Words8 r = load32(row + k0);
+// Bytes by which every row start is aligned: 32 (one access per 8 words), 16,
+// or 0 (any alignment: the warp moves its 512 elements through shared memory,
+// so that global accesses stay contiguous).
+constexpr int kStage = kQChunk / 16 * 17;  // floats of one warp's stage, a pad word behind each lane's 16
+
+ICSA_DEV Words8 load16x2(const void* p) {
+  const uint4 a = __ldg(static_cast<const uint4*>(p)), b = __ldg(static_cast<const uint4*>(p) + 1);
+  return Words8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+ICSA_DEV void store16x2(void* p, const Words8& r) {
+  static_cast<uint4*>(p)[0] = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  static_cast<uint4*>(p)[1] = make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]);
+}
+
+// Elements [c0 + 16 lane, + 16) of a row of K (zeros from column K on); called
+// by whole warps.
+template <typename T, int ALIGN>
+ICSA_DEV void load16(const T* row, int c0, int lane, int K, float* stage, float (&v)[16]) {
+  const int k0 = c0 + 16 * lane;
+  if constexpr (ALIGN > 0) {
+    if (k0 + 16 <= K) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[2 * i] = __uint_as_float(r.w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+      for (int h = 0; h < int(sizeof(T)) / 2; ++h) {
+        const T* src = row + k0 + 8 * h;
+        const Words8 r = ALIGN == 32 ? load32(src) : load16x2(src);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (sizeof(T) == 2) {
+            v[2 * i] = __uint_as_float(r.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+          } else {
+            v[8 * h + i] = __uint_as_float(r.w[i]);
+          }
+        }
       }
     } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Words8 r = load32(row + k0 + 8 * h);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(r.w[i]);
-      }
+      for (int i = 0; i < 16; ++i) v[i] = k0 + i < K ? to_float<T>(row[k0 + i]) : 0.f;
     }
-    return;
-  }
+  } else {
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = k0 + i < K ? to_float<T>(row[k0 + i]) : 0.f;
+    for (int i = 0; i < 16; ++i) {
+      const int k = 32 * i + lane;
+      stage[k + (k >> 4)] = c0 + k < K ? to_float<T>(row[c0 + k]) : 0.f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = stage[17 * lane + i];
+  }
+}
+
+template <typename T, int ALIGN>
+ICSA_DEV void store16(T* row, int c0, int lane, int K, float* stage, const float (&v)[16]) {
+  const int k0 = c0 + 16 * lane;
+  if constexpr (ALIGN > 0) {
+    if (k0 + 16 <= K) {
+#pragma unroll
+      for (int h = 0; h < int(sizeof(T)) / 2; ++h) {
+        Words8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (sizeof(T) == 2) o.w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+          else o.w[i] = __float_as_uint(v[8 * h + i]);
+        }
+        if constexpr (ALIGN == 32) store32(row + k0 + 8 * h, o);
+        else store16x2(row + k0 + 8 * h, o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + i < K) row[k0 + i] = from_float<T>(v[i]);
+    }
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) stage[17 * lane + i] = v[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int k = 32 * i + lane;
+      if (c0 + k < K) row[c0 + k] = from_float<T>(stage[k + (k >> 4)]);
+    }
+  }
 }
 
 // eight floats to e2m1 (nearest even, saturating), the first in the low half of byte 0
@@ -133,16 +204,46 @@ ICSA_DEV int tile_row(int cta, int warp) {
   return (cta >> 4) * kFp4TileRows + (cta & 15) * 2 + (warp & 1) + 32 * (warp >> 1);
 }
 
-// The 16 codes of x / d: nearest to the float32 quotient.
-ICSA_DEV void quotient_codes(const float (&v)[16], float d, uint32_t (&code)[2]) {
+// The 16 codes of x / d, those of the correctly rounded float32 quotient:
+// with 1 / d as the sum of two floats, rh + rl, the product
+// fma(x, rh, x rl) has the quotient's relative error below 2^-46 before its
+// one rounding, so it equals the quotient's float32 rounding, and exact ties
+// stay exact.  Two operations an element instead of a division.
+// (Blocks beyond the largest scale, whose quotients might overflow, divide.)
+ICSA_DEV void quotient_codes(const float (&v)[16], float amax, float d, uint32_t (&code)[2]) {
   float q[16];
+  if (d > 0x1p-100f && d < 0x1p100f && amax <= 8.f * d) {
+    float rh;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(rh) : "f"(d));  // any value near 1 / d: rl is what it lacks
+    const float rl = fmaf(-d, rh, 1.0f) * rh;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) q[i] = __fdiv_rn(v[i], d);
+    for (int i = 0; i < 16; ++i) q[i] = fmaf(v[i], rh, v[i] * rl);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = __fdiv_rn(v[i], d);
+  }
   code[0] = e2m1x8(q);
   code[1] = e2m1x8(q + 8);
 }
 
-template <typename T, int FMT, bool VEC>
+// Largest magnitude of 16 elements as float32 bits: NaN and infinity stay
+// above every number.  Elements of 16 bits are compared in pairs.
+template <typename T>
+ICSA_DEV uint32_t top_bits(const float (&v)[16]) {
+  uint32_t top = 0;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      top = __vmaxu2(top, __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632) & 0x7FFF7FFFu);
+    return max(top << 16, top & 0xFFFF0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return top;
+  }
+}
+
+template <typename T, int FMT, int ALIGN>
 __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantParams p, int chunks_per_cta) {
   constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -154,28 +255,31 @@ __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantP
   const T* xrow = static_cast<const T*>(p.x) + int64_t(r) * p.ldx;
   uint8_t* drow = p.data + int64_t(r) * row_bytes;
   const bool row_ok = r < p.rows;
+  __shared__ float stages[ALIGN > 0 ? 1 : kQThreads / 32 * kStage];
+  float* stage = stages + (ALIGN > 0 ? 0 : warp * kStage);
   const int c0 = blockIdx.y * chunks_per_cta;
   for (int c = c0; c < c0 + chunks_per_cta; ++c) {
     const int k0 = c * kQChunk + lane * 16;
     if (c * kQChunk >= k_end) break;
     float v[16];
-    if (row_ok && k0 < p.K) {
-      load16<T, VEC>(xrow, k0, p.K, v);
+    if (row_ok) {
+      load16<T, ALIGN>(xrow, c * kQChunk, lane, p.K, stage, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.f;
     }
-    // largest magnitude as bits: NaN and infinity stay above every number
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    uint32_t top = top_bits<T>(v);
     uint32_t code[2] = {0u, 0u};
     uint32_t sbyte;
     if (FMT == ICSA_NVFP4) {
-      const float t = __fdiv_rn(__uint_as_float(top), 6.0f * p.global_scale);
+      const float amax = __uint_as_float(top);
+      // (beyond 597 x 6 g the scale is 448 in any case: no product overflows)
+      const float capped = fminf(amax, 3584.f * p.global_scale);
+      const float t = p.inv_hi != 0.f ? fmaf(capped, p.inv_hi, capped * p.inv_lo)
+                                      : __fdiv_rn(amax, 6.0f * p.global_scale);
       sbyte = top >= 0x7F800000u ? 0x7Fu : uint32_t(__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3));
       const float d = e4m3_float(sbyte) * p.global_scale;
-      if (d > 0.f && top < 0x7F800000u) quotient_codes(v, d, code);
+      if (d > 0.f && top < 0x7F800000u) quotient_codes(v, amax, d, code);
     } else {
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       // floor(log2 amax): the exponent field; subnormal magnitudes clamp to 2^-127
@@ -206,7 +310,7 @@ __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantP
   }
 }
 
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT, int ALIGN>
 __global__ void __launch_bounds__(kQThreads) fp4_dequantize_kernel(const Fp4DequantParams p, int chunks_per_cta) {
   constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -217,16 +321,18 @@ __global__ void __launch_bounds__(kQThreads) fp4_dequantize_kernel(const Fp4Dequ
   const uint8_t* srow = p.scales + scale_row(r, k_tiles, kAtoms);
   const uint8_t* drow = p.data + int64_t(r) * row_bytes;
   T* orow = static_cast<T*>(p.out) + int64_t(r) * p.ldo;
+  __shared__ float stages[ALIGN > 0 ? 1 : kQThreads / 32 * kStage];
+  float* stage = stages + (ALIGN > 0 ? 0 : warp * kStage);
   const int c0 = blockIdx.y * chunks_per_cta;
   for (int c = c0; c < c0 + chunks_per_cta; ++c) {
-    const int k0 = c * kQChunk + lane * 16;
-    if (k0 >= p.K) break;
+    if (c * kQChunk >= p.K) break;
+    const int k0 = min(c * kQChunk + lane * 16, (p.K - 1) & ~15);  // lanes behind the row repeat its last block
     const uint2 code = __ldg(reinterpret_cast<const uint2*>(drow + k0 / 2));
     float d;
     if (FMT == ICSA_NVFP4) {
-      d = e4m3_float(srow[size_t(k0 / 64) * kScaleAtomBytes + (k0 / 16) % 4]) * p.global_scale;
+      d = e4m3_float(__ldg(srow + size_t(k0 / 64) * kScaleAtomBytes + (k0 / 16) % 4)) * p.global_scale;
     } else {
-      const uint32_t e = srow[size_t(k0 / 128) * kScaleAtomBytes + (k0 / 32) % 4];
+      const uint32_t e = __ldg(srow + size_t(k0 / 128) * kScaleAtomBytes + (k0 / 32) % 4);
       // 2^(e - 127): the subnormal 2^-127 for 0, NaN for 255
       d = __uint_as_float(e == 255u ? 0x7FC00000u : e == 0u ? 0x00400000u : e << 23);
     }
@@ -238,34 +344,14 @@ __global__ void __launch_bounds__(kQThreads) fp4_dequantize_kernel(const Fp4Dequ
     e2m1x8_floats(code.y, h);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[8 + i] = h[i] * d;
-    if (VEC && k0 + 16 <= p.K) {
-      if constexpr (sizeof(T) == 2) {
-        Words8 o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o.w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-        store32(orow + k0, o);
-      } else {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          Words8 o;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o.w[i] = __float_as_uint(v[8 * half + i]);
-          store32(orow + k0 + 8 * half, o);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (k0 + i < p.K) {
-          if constexpr (sizeof(T) == 2) orow[k0 + i] = __float2bfloat16_rn(v[i]);
-          else orow[k0 + i] = v[i];
-        }
-    }
+    store16<T, ALIGN>(orow, c * kQChunk, lane, p.K, stage, v);
   }
 }
 
-bool rows_aligned32(const void* base, int64_t ld, int elem) {
-  return (reinterpret_cast<uintptr_t>(base) & 31u) == 0 && (ld * elem) % 32 == 0;
+// alignment of every row start: 32, 16 or 0
+int row_alignment(const void* base, int64_t ld, int elem) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(base) | uint64_t(ld * elem);
+  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 0;
 }
 
 // CTAs cover `chunks` row chunks in grid.y; four chunks per CTA once the rows
@@ -278,12 +364,21 @@ void quant_grid(int rows, int k_elems, dim3* grid, int* chunks_per_cta) {
 }
 
 template <typename T, int FMT>
-cudaError_t quantize_as(const Fp4QuantParams& p, cudaStream_t stream) {
+cudaError_t quantize_as(Fp4QuantParams p, cudaStream_t stream) {
+  const float c = 6.0f * p.global_scale;
+  p.inv_hi = p.inv_lo = 0.f;
+  if (c > 0x1p-100f && c < 0x1p100f) {
+    p.inv_hi = float(1.0 / double(c));
+    p.inv_lo = float(1.0 / double(c) - double(p.inv_hi));
+  }
   dim3 grid;
   int per;
   quant_grid(p.rows, (p.K + kFp4TileK - 1) / kFp4TileK * kFp4TileK, &grid, &per);
-  if (rows_aligned32(p.x, p.ldx, sizeof(T))) fp4_quantize_kernel<T, FMT, true><<<grid, kQThreads, 0, stream>>>(p, per);
-  else fp4_quantize_kernel<T, FMT, false><<<grid, kQThreads, 0, stream>>>(p, per);
+  const int al = row_alignment(p.x, p.ldx, sizeof(T));
+  const auto kernel = al == 32   ? fp4_quantize_kernel<T, FMT, 32>
+                      : al == 16 ? fp4_quantize_kernel<T, FMT, 16>
+                                 : fp4_quantize_kernel<T, FMT, 0>;
+  kernel<<<grid, kQThreads, 0, stream>>>(p, per);
   return cudaGetLastError();
 }
 
@@ -292,8 +387,11 @@ cudaError_t dequantize_as(const Fp4DequantParams& p, cudaStream_t stream) {
   dim3 grid;
   int per;
   quant_grid(p.rows, p.K, &grid, &per);
-  if (rows_aligned32(p.out, p.ldo, sizeof(T))) fp4_dequantize_kernel<T, FMT, true><<<grid, kQThreads, 0, stream>>>(p, per);
-  else fp4_dequantize_kernel<T, FMT, false><<<grid, kQThreads, 0, stream>>>(p, per);
+  const int al = row_alignment(p.out, p.ldo, sizeof(T));
+  const auto kernel = al == 32   ? fp4_dequantize_kernel<T, FMT, 32>
+                      : al == 16 ? fp4_dequantize_kernel<T, FMT, 16>
+                                 : fp4_dequantize_kernel<T, FMT, 0>;
+  kernel<<<grid, kQThreads, 0, stream>>>(p, per);
   return cudaGetLastError();
 }
 

@@ -35,6 +35,7 @@ struct Fp4QuantParams {
   float global_scale;
   uint8_t* data;
   uint8_t* scales;
+  float inv_hi, inv_lo;  // 1 / (6 global_scale) as a sum of two floats (0: out of their range); set by the launcher
 };
 cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, int x_dtype, int format, cudaStream_t stream);
 

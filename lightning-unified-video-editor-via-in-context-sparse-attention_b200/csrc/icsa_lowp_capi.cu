@@ -80,6 +80,69 @@ int encode_fp4_maps(CUtensorMap* data_map, CUtensorMap* scale_map, const void* d
 
 int fp4_n_pad(int N) { return (N + 255) / 256 * 256; }
 
+struct Fp4Call {
+  icsa::Fp4GemmMaps maps;
+  icsa::Fp4GemmParams p;
+  int sms;
+};
+
+// Checks of a linear layer, and its launch parameters (M = 0: nothing to launch).
+int prepare_linear(Fp4Call* call, int format, const void* a_data, const void* a_scales, float a_global_scale,
+                   const void* w_data, const void* w_scales, float w_global_scale, const void* bias, int activation,
+                   void* out, int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes) {
+  int rc;
+  std::memset(call, 0, sizeof(*call));
+  icsa::Fp4GemmParams& p = call->p;
+  icsa::Fp4GemmMaps& maps = call->maps;
+  int& sms = call->sms;
+  if ((rc = check_fp4("fp4_linear", format, M, K)) != ICSA_OK) return rc;
+  if ((rc = check_fp4("fp4_linear", format, N, K)) != ICSA_OK) return rc;
+  if ((rc = check_global_scale("fp4_linear", format, a_global_scale)) != ICSA_OK) return rc;
+  if ((rc = check_global_scale("fp4_linear", format, w_global_scale)) != ICSA_OK) return rc;
+  if (N < 1) return fail(ICSA_ERR_INVALID, "fp4_linear: N=%d must be positive", N);
+  if (activation != ICSA_ACT_NONE && activation != ICSA_ACT_GELU_TANH)
+    return fail(ICSA_ERR_INVALID, "fp4_linear: unknown activation %d", activation);
+  if (ldo < N) return fail(ICSA_ERR_INVALID, "fp4_linear: ldo=%lld is smaller than N=%d", (long long)ldo, N);
+  const int64_t tiles = ((int64_t(M) + 255) / 256) * ((int64_t(N) + 255) / 256);
+  if (tiles > 0x3FFFFFFFll) return fail(ICSA_ERR_UNSUPPORTED, "fp4_linear: M=%d x N=%d exceeds this build's limits", M, N);
+  if (M == 0) return ICSA_OK;
+  if ((rc = check_fp4_buffers("fp4_linear", a_data, a_scales)) != ICSA_OK) return rc;
+  if ((rc = check_fp4_buffers("fp4_linear", w_data, w_scales)) != ICSA_OK) return rc;
+  if (out == nullptr || !aligned(out, 2) || !aligned(bias, 2))
+    return fail(ICSA_ERR_INVALID, "fp4_linear: out must be non-NULL, out and bias aligned to their elements");
+  if (!sm_count(&sms)) return ICSA_ERR_CUDA;
+  p.M = M; p.N = N; p.K = K;
+  p.alpha = a_global_scale * w_global_scale;
+  p.bias = static_cast<const __nv_bfloat16*>(bias);
+  p.activation = activation;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ldo = ldo;
+  p.tma_out = aligned(out, 16) && ldo % 8 == 0;
+  p.splits = icsa::fp4_gemm_splits(M, N, K, sms);
+  p.n_pad = fp4_n_pad(N);
+  if (p.splits > 1) {
+    const size_t need = align256(size_t(p.splits) * M * p.n_pad * sizeof(float));
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(ICSA_ERR_WORKSPACE, "fp4_linear: workspace of %zu bytes is smaller than the %zu bytes required",
+                  workspace == nullptr ? size_t(0) : workspace_bytes, need);
+    if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "fp4_linear: the workspace must be 256-byte aligned");
+    p.partial = static_cast<float*>(workspace);
+  }
+  if ((rc = encode_fp4_maps(&maps.a, &maps.sa, a_data, a_scales, format, M, K)) != ICSA_OK) return rc;
+  if ((rc = encode_fp4_maps(&maps.w, &maps.sw, w_data, w_scales, format, N, K)) != ICSA_OK) return rc;
+  if (p.tma_out && (rc = icsa::encode_tensor_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, uint64_t(N),
+                                                    uint64_t(M), uint64_t(ldo) * 2, 64, 32,
+                                                    CU_TENSOR_MAP_SWIZZLE_128B)) != ICSA_OK)
+    return rc;
+  return ICSA_OK;
+}
+
+int launch_linear(const Fp4Call& call, int format, cudaStream_t stream) {
+  if (call.p.M == 0) return ICSA_OK;
+  cudaError_t e = icsa::launch_fp4_gemm(call.p, call.maps, format, call.sms, stream);
+  return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_linear");
+}
+
 // ------------------------------------------------------------------ 8 bits --
 int check_cache(const char* who, const icsa_kv8_cache* c, icsa::Kv8Cache* out) {
   if (c == nullptr) return fail(ICSA_ERR_INVALID, "%s: the cache is NULL", who);
@@ -165,7 +228,8 @@ int icsa_fp4_quantize(const void* x, int x_dtype, int64_t ldx, int rows, int K, 
   if ((rc = check_fp4_buffers("fp4_quantize", data, scales)) != ICSA_OK) return rc;
   if (x == nullptr || !aligned(x, x_dtype == ICSA_F32 ? 4 : 2))
     return fail(ICSA_ERR_INVALID, "fp4_quantize: x must be non-NULL and aligned to its elements");
-  icsa::Fp4QuantParams p = {x, ldx, rows, K, global_scale, static_cast<uint8_t*>(data), static_cast<uint8_t*>(scales)};
+  icsa::Fp4QuantParams p = {x, ldx, rows, K, global_scale, static_cast<uint8_t*>(data), static_cast<uint8_t*>(scales),
+                            0.f, 0.f};
   cudaError_t e = icsa::launch_fp4_quantize(p, x_dtype, format, stream);
   return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_quantize");
 }
@@ -197,53 +261,40 @@ size_t icsa_fp4_linear_workspace_size(int M, int N, int K) {
 int icsa_fp4_linear(int format, const void* a_data, const void* a_scales, float a_global_scale, const void* w_data,
                     const void* w_scales, float w_global_scale, const void* bias, int activation, void* out,
                     int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  Fp4Call call;
+  const int rc = prepare_linear(&call, format, a_data, a_scales, a_global_scale, w_data, w_scales, w_global_scale, bias,
+                                activation, out, ldo, M, N, K, workspace, workspace_bytes);
+  return rc != ICSA_OK ? rc : launch_linear(call, format, stream);
+}
+
+size_t icsa_fp4_linear_rows_workspace_size(int format, int M, int N, int K) {
+  if (check_fp4("fp4_linear_rows_workspace_size", format, M, K) != ICSA_OK || M < 1 || N < 1) return 0;
+  return align256(icsa_fp4_data_bytes(M, K)) + align256(icsa_fp4_scale_bytes(format, M, K)) +
+         icsa_fp4_linear_workspace_size(M, N, K);
+}
+
+int icsa_fp4_linear_rows(int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
+                         const void* w_scales, float w_global_scale, const void* bias, int activation, void* out,
+                         int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes,
+                         cudaStream_t stream) {
   int rc;
-  if ((rc = check_fp4("fp4_linear", format, M, K)) != ICSA_OK) return rc;
-  if ((rc = check_fp4("fp4_linear", format, N, K)) != ICSA_OK) return rc;
-  if ((rc = check_global_scale("fp4_linear", format, a_global_scale)) != ICSA_OK) return rc;
-  if ((rc = check_global_scale("fp4_linear", format, w_global_scale)) != ICSA_OK) return rc;
-  if (N < 1) return fail(ICSA_ERR_INVALID, "fp4_linear: N=%d must be positive", N);
-  if (activation != ICSA_ACT_NONE && activation != ICSA_ACT_GELU_TANH)
-    return fail(ICSA_ERR_INVALID, "fp4_linear: unknown activation %d", activation);
-  if (ldo < N) return fail(ICSA_ERR_INVALID, "fp4_linear: ldo=%lld is smaller than N=%d", (long long)ldo, N);
-  const int64_t tiles = ((int64_t(M) + 255) / 256) * ((int64_t(N) + 255) / 256);
-  if (tiles > 0x3FFFFFFFll) return fail(ICSA_ERR_UNSUPPORTED, "fp4_linear: M=%d x N=%d exceeds this build's limits", M, N);
-  if (M == 0) return ICSA_OK;
-  if ((rc = check_fp4_buffers("fp4_linear", a_data, a_scales)) != ICSA_OK) return rc;
-  if ((rc = check_fp4_buffers("fp4_linear", w_data, w_scales)) != ICSA_OK) return rc;
-  if (out == nullptr || !aligned(out, 2) || !aligned(bias, 2))
-    return fail(ICSA_ERR_INVALID, "fp4_linear: out must be non-NULL, out and bias aligned to their elements");
-  int sms = 0;
-  if (!sm_count(&sms)) return ICSA_ERR_CUDA;
-  icsa::Fp4GemmParams p;
-  std::memset(&p, 0, sizeof(p));
-  p.M = M; p.N = N; p.K = K;
-  p.alpha = a_global_scale * w_global_scale;
-  p.bias = static_cast<const __nv_bfloat16*>(bias);
-  p.activation = activation;
-  p.out = static_cast<__nv_bfloat16*>(out);
-  p.ldo = ldo;
-  p.tma_out = aligned(out, 16) && ldo % 8 == 0;
-  p.splits = icsa::fp4_gemm_splits(M, N, K, sms);
-  p.n_pad = fp4_n_pad(N);
-  if (p.splits > 1) {
-    const size_t need = align256(size_t(p.splits) * M * p.n_pad * sizeof(float));
-    if (workspace == nullptr || workspace_bytes < need)
-      return fail(ICSA_ERR_WORKSPACE, "fp4_linear: workspace of %zu bytes is smaller than the %zu bytes required",
-                  workspace == nullptr ? size_t(0) : workspace_bytes, need);
-    if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "fp4_linear: the workspace must be 256-byte aligned");
-    p.partial = static_cast<float*>(workspace);
+  if ((rc = check_fp4("fp4_linear_rows", format, M, K)) != ICSA_OK) return rc;
+  const size_t data = align256(icsa_fp4_data_bytes(M, K)), scales = align256(icsa_fp4_scale_bytes(format, M, K));
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (M > 0) {
+    if (workspace == nullptr || workspace_bytes < data + scales)
+      return fail(ICSA_ERR_WORKSPACE, "fp4_linear_rows: workspace of %zu bytes is smaller than the %zu bytes that the "
+                  "quantised rows take", workspace == nullptr ? size_t(0) : workspace_bytes, data + scales);
+    if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "fp4_linear_rows: the workspace must be 256-byte aligned");
   }
-  icsa::Fp4GemmMaps maps;
-  if ((rc = encode_fp4_maps(&maps.a, &maps.sa, a_data, a_scales, format, M, K)) != ICSA_OK) return rc;
-  if ((rc = encode_fp4_maps(&maps.w, &maps.sw, w_data, w_scales, format, N, K)) != ICSA_OK) return rc;
-  std::memset(&maps.out, 0, sizeof(maps.out));
-  if (p.tma_out && (rc = icsa::encode_tensor_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, uint64_t(N),
-                                                    uint64_t(M), uint64_t(ldo) * 2, 64, 32,
-                                                    CU_TENSOR_MAP_SWIZZLE_128B)) != ICSA_OK)
+  // the linear layer's own checks come before anything is launched
+  Fp4Call call;
+  if ((rc = prepare_linear(&call, format, ws, ws + data, 1.f, w_data, w_scales, w_global_scale, bias, activation, out,
+                           ldo, M, N, K, M > 0 ? ws + data + scales : nullptr,
+                           M > 0 ? workspace_bytes - data - scales : 0)) != ICSA_OK)
     return rc;
-  cudaError_t e = icsa::launch_fp4_gemm(p, maps, format, sms, stream);
-  return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_linear");
+  if ((rc = icsa_fp4_quantize(x, x_dtype, ldx, M, K, format, 1.f, ws, ws + data, stream)) != ICSA_OK) return rc;
+  return launch_linear(call, format, stream);
 }
 
 int icsa_kv8_quantize(const icsa_kv8_cache* cache, const void* k, const void* v, int dtype, const int64_t k_strides[3],

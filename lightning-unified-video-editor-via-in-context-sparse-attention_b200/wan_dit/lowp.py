@@ -16,6 +16,7 @@ compute values only: no gradient is recorded.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -25,7 +26,8 @@ import torch
 from in_context_sparse_attention import _capi
 
 LOWP_EXPORTED = ("icsa_fp4_data_bytes", "icsa_fp4_scale_bytes", "icsa_fp4_quantize", "icsa_fp4_dequantize",
-                 "icsa_fp4_linear_workspace_size", "icsa_fp4_linear", "icsa_kv8_quantize", "icsa_kv8_dequantize",
+                 "icsa_fp4_linear_workspace_size", "icsa_fp4_linear", "icsa_fp4_linear_rows_workspace_size",
+                 "icsa_fp4_linear_rows", "icsa_kv8_quantize", "icsa_kv8_dequantize",
                  "icsa_kv8_attention_workspace_size", "icsa_kv8_attention")
 
 FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
@@ -63,6 +65,8 @@ def _load():
             ("icsa_fp4_dequantize", i, [vp, vp, i, i, i, f, vp, i, i64, vp]),
             ("icsa_fp4_linear_workspace_size", sz, [i, i, i]),
             ("icsa_fp4_linear", i, [i, vp, vp, f, vp, vp, f, vp, i, vp, i64, i, i, i, vp, sz, vp]),
+            ("icsa_fp4_linear_rows_workspace_size", sz, [i, i, i, i]),
+            ("icsa_fp4_linear_rows", i, [i, vp, i, i64, vp, vp, f, vp, i, vp, i64, i, i, i, vp, sz, vp]),
             ("icsa_kv8_quantize", i, [desc, vp, vp, i, st, st, vp]),
             ("icsa_kv8_dequantize", i, [desc, vp, vp, i, vp]),
             ("icsa_kv8_attention_workspace_size", sz, [desc, i, i]),
@@ -73,28 +77,43 @@ def _load():
     return lib
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _on_cuda(where, *tensors):
-    """The one CUDA device of the tensors (None entries are skipped)."""
-    device = None
+def _device(where, *tensors):
+    """Index of the one CUDA device of the tensors (None entries are skipped)."""
+    index = None
     for t in tensors:
         if t is None:
             continue
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"{where}: expected CUDA tensors")
-        if device is not None and t.device != device:
-            raise ValueError(f"{where}: tensors on {device} and {t.device}")
-        device = t.device
-    return device
+        i = t.get_device()
+        if index is None:
+            index = i
+        elif i != index:
+            raise ValueError(f"{where}: tensors on cuda:{index} and cuda:{i}")
+    return index
+
+
+def _on(index, fn, *args):
+    """fn(library, raw handle of the device's current stream, *args) with the device current."""
+    lib = _lib or _load()
+    if index == torch.cuda.current_device():
+        return fn(lib, torch._C._cuda_getCurrentRawStream(index), *args)
+    with torch.cuda.device(index):
+        return fn(lib, torch._C._cuda_getCurrentRawStream(index), *args)
+
+
+def _bytes(like, n):
+    """n bytes of workspace on the device of `like` (None for 0) and their address."""
+    if not n:
+        return None, None
+    ws = like.new_empty(n, dtype=torch.uint8)
+    return ws, ws.data_ptr()
 
 
 # ---------------------------------------------------------------------------
 # 4-bit tensors
 # ---------------------------------------------------------------------------
-@dataclass
+@dataclass(frozen=True)
 class Fp4Tensor:
     """A [rows, K] tensor in 4-bit storage (layout: include/icsa_lowp.h).
 
@@ -111,14 +130,14 @@ class Fp4Tensor:
     def __post_init__(self):
         if self.fmt not in FP4_FORMATS:
             raise ValueError(f"4-bit format {self.fmt!r}: expected one of {sorted(FP4_FORMATS)}")
-        self.shape = tuple(int(n) for n in self.shape)
+        object.__setattr__(self, "shape", tuple(int(n) for n in self.shape))
         if len(self.shape) != 2 or self.shape[0] < 0 or self.shape[1] < 1:
             raise ValueError(f"Fp4Tensor: shape {self.shape} is not [rows, K] with K >= 1")
         data, scales = fp4_storage(*self.shape, self.fmt)
         for name, t, want in (("data", self.data, data), ("scales", self.scales, scales)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
+            if t.dtype != torch.uint8 or t.shape != want or not t.is_contiguous():
                 raise ValueError(f"Fp4Tensor: {name} must be contiguous uint8 {list(want)} for shape {list(self.shape)}")
-        if self.data.device != self.scales.device:
+        if self.data.get_device() != self.scales.get_device():
             raise ValueError("Fp4Tensor: data and scales on different devices")
         _check_global_scale(self.fmt, self.global_scale)
 
@@ -169,30 +188,38 @@ def fp4_quantize(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0)
     if fmt not in FP4_FORMATS:
         raise ValueError(f"4-bit format {fmt!r}: expected one of {sorted(FP4_FORMATS)}")
     _check_global_scale(fmt, global_scale)
-    device = _on_cuda("fp4_quantize", x)
+    index = _device("fp4_quantize", x)
     x, ld = _rows2d("fp4_quantize", x)
+    return _on(index, _quantize, x, ld, fmt, float(global_scale))
+
+
+def _quantize(lib, stream, x, ld, fmt, g):
     rows, K = x.shape
-    lib = _load()
-    with torch.cuda.device(device):
-        data, scales = (torch.empty(s, dtype=torch.uint8, device=device) for s in fp4_storage(rows, K, fmt))
-        _capi.check(lib.icsa_fp4_quantize(x.data_ptr(), _DT[x.dtype], ld, rows, K, FP4_FORMATS[fmt],
-                                          float(global_scale), data.data_ptr(), scales.data_ptr(), _stream(device)),
-                    "icsa_fp4_quantize")
-    return Fp4Tensor(data, scales, (rows, K), fmt, float(global_scale))
+    data, scales = fp4_storage(rows, K, fmt)
+    data, scales = x.new_empty(data, dtype=torch.uint8), x.new_empty(scales, dtype=torch.uint8)
+    code = lib.icsa_fp4_quantize(x.data_ptr(), _DT[x.dtype], ld, rows, K, FP4_FORMATS[fmt], g, data.data_ptr(),
+                                 scales.data_ptr(), stream)
+    if code:
+        _capi.check(code, "icsa_fp4_quantize")
+    t = object.__new__(Fp4Tensor)       # its tensors are as the constructor wants them
+    t.__dict__.update(data=data, scales=scales, shape=(rows, K), fmt=fmt, global_scale=g)
+    return t
 
 
 def fp4_dequantize(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """[rows, K] values of a 4-bit tensor, code * (block scale * global scale)."""
     if dtype not in _DT:
         raise ValueError(f"fp4_dequantize: dtype {dtype}, expected bf16 or f32")
-    device = _on_cuda("fp4_dequantize", t.data, t.scales)
+    return _on(_device("fp4_dequantize", t.data, t.scales), _dequantize, t, dtype)
+
+
+def _dequantize(lib, stream, t, dtype):
     rows, K = t.shape
-    lib = _load()
-    with torch.cuda.device(device):
-        out = torch.empty(rows, K, dtype=dtype, device=device)
-        _capi.check(lib.icsa_fp4_dequantize(t.data.data_ptr(), t.scales.data_ptr(), rows, K, FP4_FORMATS[t.fmt],
-                                            t.global_scale, out.data_ptr(), _DT[dtype], K, _stream(device)),
-                    "icsa_fp4_dequantize")
+    out = t.data.new_empty((rows, K), dtype=dtype)
+    code = lib.icsa_fp4_dequantize(t.data.data_ptr(), t.scales.data_ptr(), rows, K, FP4_FORMATS[t.fmt],
+                                   t.global_scale, out.data_ptr(), _DT[dtype], K, stream)
+    if code:
+        _capi.check(code, "icsa_fp4_dequantize")
     return out
 
 
@@ -209,36 +236,61 @@ def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation:
     N, K = w.shape
     if N < 1:
         raise ValueError("fp4_linear: w has no rows")
-    if tuple(x.shape)[1:] != (K,) or len(x.shape) != 2:
+    if len(x.shape) != 2 or x.shape[1] != K:
         raise ValueError(f"fp4_linear: x {tuple(x.shape)} and w {w.shape} differ in K")
-    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,)):
-        raise ValueError(f"fp4_linear: bias must be bf16 [{N}]")
-    a = x if isinstance(x, Fp4Tensor) else None
-    if a is not None and a.fmt != w.fmt:
-        raise ValueError(f"fp4_linear: x is {a.fmt}, w is {w.fmt}")
-    device = _on_cuda("fp4_linear", *((a.data, a.scales) if a is not None else (x,)), w.data, w.scales, bias)
-    if a is None:
-        a = fp4_quantize(x, w.fmt)
     if bias is not None:
+        if bias.dtype != torch.bfloat16 or bias.shape != (N,):
+            raise ValueError(f"fp4_linear: bias must be bf16 [{N}]")
         bias = bias.contiguous()
-    M = a.shape[0]
-    lib = _load()
-    with torch.cuda.device(device):
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=device)
-        size = lib.icsa_fp4_linear_workspace_size(M, N, K)
-        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _capi.check(lib.icsa_fp4_linear(
-            FP4_FORMATS[w.fmt], a.data.data_ptr(), a.scales.data_ptr(), a.global_scale, w.data.data_ptr(),
-            w.scales.data_ptr(), w.global_scale, bias.data_ptr() if bias is not None else None,
-            ACTIVATIONS[activation], out.data_ptr(), N, M, N, K, ws.data_ptr() if size else None, size,
-            _stream(device)), "icsa_fp4_linear")
+    if isinstance(x, Fp4Tensor):
+        if x.fmt != w.fmt:
+            raise ValueError(f"fp4_linear: x is {x.fmt}, w is {w.fmt}")
+        return _on(_device("fp4_linear", x.data, x.scales, w.data, w.scales, bias), _linear, x, w, bias, activation)
+    index = _device("fp4_linear", x, w.data, w.scales, bias)
+    x, ld = _rows2d("fp4_linear", x)
+    return _on(index, _linear_rows, x, ld, w, bias, activation)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(index, fmt, M, N, K):
+    """Workspace bytes of icsa_fp4_linear (fmt None) or icsa_fp4_linear_rows; the device is current."""
+    if fmt is None:
+        return _lib.icsa_fp4_linear_workspace_size(M, N, K)
+    return _lib.icsa_fp4_linear_rows_workspace_size(FP4_FORMATS[fmt], M, N, K)
+
+
+def _linear(lib, stream, a, w, bias, activation):
+    (M, K), N = a.shape, w.shape[0]
+    out = a.data.new_empty((M, N), dtype=torch.bfloat16)
+    size = _linear_workspace(a.data.get_device(), None, M, N, K)
+    ws, ptr = _bytes(out, size)
+    code = lib.icsa_fp4_linear(FP4_FORMATS[w.fmt], a.data.data_ptr(), a.scales.data_ptr(), a.global_scale,
+                               w.data.data_ptr(), w.scales.data_ptr(), w.global_scale,
+                               bias.data_ptr() if bias is not None else None, ACTIVATIONS[activation], out.data_ptr(),
+                               N, M, N, K, ptr, size, stream)
+    if code:
+        _capi.check(code, "icsa_fp4_linear")
+    return out
+
+
+def _linear_rows(lib, stream, x, ld, w, bias, activation):
+    (M, K), N = x.shape, w.shape[0]
+    out = x.new_empty((M, N), dtype=torch.bfloat16)
+    size = _linear_workspace(x.get_device(), w.fmt, M, N, K)
+    ws, ptr = _bytes(out, size)
+    code = lib.icsa_fp4_linear_rows(FP4_FORMATS[w.fmt], x.data_ptr(), _DT[x.dtype], ld, w.data.data_ptr(),
+                                    w.scales.data_ptr(), w.global_scale,
+                                    bias.data_ptr() if bias is not None else None, ACTIVATIONS[activation],
+                                    out.data_ptr(), N, M, N, K, ptr, size, stream)
+    if code:
+        _capi.check(code, "icsa_fp4_linear_rows")
     return out
 
 
 # ---------------------------------------------------------------------------
 # 8-bit key/value cache
 # ---------------------------------------------------------------------------
-@dataclass
+@dataclass(frozen=True)
 class Kv8Cache:
     """Keys and values of B sequences in e4m3 (layout: include/icsa_lowp.h).
 
@@ -263,10 +315,12 @@ class Kv8Cache:
                                    ("v", self.v, (B, H, nb, D, T), torch.float8_e4m3fn),
                                    ("k_scale", self.k_scale, (B, H, nb), torch.float32),
                                    ("v_scale", self.v_scale, (B, H, nb), torch.float32)):
-            if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous():
+            if t.shape != shape or t.dtype != dt or not t.is_contiguous():
                 raise ValueError(f"Kv8Cache: {name} must be contiguous {dt} {list(shape)}")
         _check_lengths("Kv8Cache", self.lengths, B)
-        if len({t.device for t in (self.k, self.v, self.k_scale, self.v_scale, self.lengths) if t is not None}) > 1:
+        index = self.k.get_device()
+        if any(t.get_device() != index for t in (self.v, self.k_scale, self.v_scale)) or (
+                self.lengths is not None and self.lengths.get_device() != index):
             raise ValueError("Kv8Cache: tensors on different devices")
 
     @property
@@ -280,14 +334,18 @@ class Kv8Cache:
 
 
 def _check_lengths(where, lengths, B):
-    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,)
-                                or not lengths.is_contiguous()):
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous()):
         raise ValueError(f"{where}: lengths must be contiguous int32 [{B}]")
+
+
+@functools.lru_cache(maxsize=1024)
+def _int64x3(a, b, c):
+    return (ctypes.c_int64 * 3)(a, b, c)
 
 
 def _strides(t):
     """Batch, token and head strides; 0 for an axis of one."""
-    return (ctypes.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+    return _int64x3(*(st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride())))
 
 
 def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> Kv8Cache:
@@ -295,7 +353,7 @@ def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tenso
     [B] on the device or None.  One scale for each block of 64 tokens and
     head, the smallest power of two with which the block's largest magnitude
     is at most 448.  Tokens behind a length are not read."""
-    device = _on_cuda("kv8_quantize", k, v, lengths)
+    index = _device("kv8_quantize", k, v, lengths)
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DT:
         raise ValueError(f"kv8_quantize: k {tuple(k.shape)} and v {tuple(v.shape)} must be bf16 or f32 [B, L, H, D]")
     B, L, H, D = k.shape
@@ -304,15 +362,22 @@ def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tenso
     if min(B, L, H) < 1:
         raise ValueError(f"kv8_quantize: empty k, v {tuple(k.shape)}")
     _check_lengths("kv8_quantize", lengths, B)
-    k, v = (t if t.stride(3) == 1 and min(t.stride()) >= 0 else t.contiguous() for t in (k, v))
-    lib = _load()
+    k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (k, v))
+    return _on(index, _quantize_kv, k, v, lengths)
+
+
+def _quantize_kv(lib, stream, k, v, lengths):
+    B, L, H, D = k.shape
     nb = -(-L // KV8_TOKENS)
-    with torch.cuda.device(device):
-        c = Kv8Cache(torch.empty(B, H, nb, KV8_TOKENS, D, dtype=torch.float8_e4m3fn, device=device),
-                     torch.empty(B, H, nb, D, KV8_TOKENS, dtype=torch.float8_e4m3fn, device=device),
-                     torch.empty(B, H, nb, device=device), torch.empty(B, H, nb, device=device), L, lengths)
-        _capi.check(lib.icsa_kv8_quantize(ctypes.byref(c._desc()), k.data_ptr(), v.data_ptr(), _DT[k.dtype],
-                                          _strides(k), _strides(v), _stream(device)), "icsa_kv8_quantize")
+    c = object.__new__(Kv8Cache)        # its tensors are as the constructor wants them
+    c.__dict__.update(k=k.new_empty((B, H, nb, KV8_TOKENS, D), dtype=torch.float8_e4m3fn),
+                      v=k.new_empty((B, H, nb, D, KV8_TOKENS), dtype=torch.float8_e4m3fn),
+                      k_scale=k.new_empty((B, H, nb), dtype=torch.float32),
+                      v_scale=k.new_empty((B, H, nb), dtype=torch.float32), L=L, lengths=lengths)
+    code = lib.icsa_kv8_quantize(ctypes.byref(c._desc()), k.data_ptr(), v.data_ptr(), _DT[k.dtype], _strides(k),
+                                 _strides(v), stream)
+    if code:
+        _capi.check(code, "icsa_kv8_quantize")
     return c
 
 
@@ -320,13 +385,15 @@ def kv8_dequantize(cache: Kv8Cache, dtype: torch.dtype = torch.bfloat16):
     """(k, v) [B, L, H, D], code * scale (exact in bf16); zero behind a length."""
     if dtype not in _DT:
         raise ValueError(f"kv8_dequantize: dtype {dtype}, expected bf16 or f32")
-    device = _on_cuda("kv8_dequantize", cache.k, cache.v, cache.k_scale, cache.v_scale, cache.lengths)
+    return _on(_device("kv8_dequantize", cache.k), _dequantize_kv, cache, dtype)
+
+
+def _dequantize_kv(lib, stream, cache, dtype):
     B, H, _, _, D = cache.k.shape
-    lib = _load()
-    with torch.cuda.device(device):
-        k, v = (torch.empty(B, cache.L, H, D, dtype=dtype, device=device) for _ in range(2))
-        _capi.check(lib.icsa_kv8_dequantize(ctypes.byref(cache._desc()), k.data_ptr(), v.data_ptr(), _DT[dtype],
-                                            _stream(device)), "icsa_kv8_dequantize")
+    k, v = (cache.k.new_empty((B, cache.L, H, D), dtype=dtype) for _ in range(2))
+    code = lib.icsa_kv8_dequantize(ctypes.byref(cache._desc()), k.data_ptr(), v.data_ptr(), _DT[dtype], stream)
+    if code:
+        _capi.check(code, "icsa_kv8_dequantize")
     return k, v
 
 
@@ -335,26 +402,36 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache) -> torch.Tensor:
     [B, Lq, Hq, D]; zero for a sequence of length 0.  q: bf16 [B, Lq, Hq, D],
     Hq a multiple of the cache's heads (query heads h of one group share
     cache head h // (Hq / H))."""
-    device = _on_cuda("kv8_attention", q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.lengths)
+    index = _device("kv8_attention", q, cache.k)
     B, H, _, _, D = cache.k.shape
     if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != B or q.shape[3] != D or q.shape[2] % H or not q.shape[2]:
         raise ValueError(f"kv8_attention: q must be bf16 [{B}, Lq, a multiple of {H}, {D}], got {q.dtype} {tuple(q.shape)}")
-    Lq, Hq = q.shape[1], q.shape[2]
-    lib = _load()
-    with torch.cuda.device(device):
-        out = torch.empty(B, Lq, Hq, D, dtype=torch.bfloat16, device=device)
-        if Lq == 0:
-            return out
-        # rows of a wider GEMM output are taken as they are
-        if (q.stride(3) != 1 or (Hq > 1 and q.stride(2) != D) or (Lq > 1 and q.stride(1) < Hq * D) or q.stride(1) % 8
-                or (B > 1 and q.stride(0) != Lq * q.stride(1)) or q.data_ptr() % 16):
-            q = q.clone(memory_format=torch.contiguous_format)
-        ts = q.stride(1) if Lq > 1 or B > 1 else Hq * D
-        strides = (ctypes.c_int64 * 3)(Lq * ts, ts, D)
-        desc = cache._desc()
-        size = lib.icsa_kv8_attention_workspace_size(ctypes.byref(desc), Lq, Hq)
-        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _capi.check(lib.icsa_kv8_attention(ctypes.byref(desc), q.data_ptr(), strides, out.data_ptr(), Lq, Hq,
-                                           ws.data_ptr() if size else None, size, _stream(device)),
-                    "icsa_kv8_attention")
+    return _on(index, _attention, q, cache)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(index, B, H, L, D, Lq, Hq):
+    return _lib.icsa_kv8_attention_workspace_size(ctypes.byref(_Kv8Desc(B, H, L, D)), Lq, Hq)
+
+
+def _attention(lib, stream, q, cache):
+    B, Lq, Hq, D = q.shape
+    H = cache.k.shape[1]
+    out = q.new_empty((B, Lq, Hq, D))
+    if Lq == 0:
+        return out
+    sb, st, sh, sd = q.stride()
+    # rows of a wider GEMM output are taken as they are
+    if (sd != 1 or (Hq > 1 and sh != D) or (Lq > 1 and st < Hq * D) or st % 8 or (B > 1 and sb != Lq * st)
+            or q.data_ptr() % 16):
+        q = q.clone(memory_format=torch.contiguous_format)
+        st = Hq * D
+    if Lq == 1 and B == 1:
+        st = Hq * D
+    size = _attention_workspace(q.get_device(), B, H, cache.L, D, Lq, Hq)
+    ws, ptr = _bytes(out, size)
+    code = lib.icsa_kv8_attention(ctypes.byref(cache._desc()), q.data_ptr(), _int64x3(Lq * st, st, D), out.data_ptr(),
+                                  Lq, Hq, ptr, size, stream)
+    if code:
+        _capi.check(code, "icsa_kv8_attention")
     return out

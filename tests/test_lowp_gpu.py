@@ -73,12 +73,12 @@ def test_quantisation_of_zeros_ties_extremes_and_non_finite_blocks(fmt):
     x[5, 40] = math.nan
     x[6, 40] = math.inf
     x[7, 40] = -math.inf
-    x[8, 95] = 3.3e38
+    x[8, 95], x[8, 94] = 3.3e38, -3.3e38
     x[9, 0] = 2.0 ** -126
     x[10, :] = -0.0
     x[11, 33], x[11, 34] = 1.0, 2.0 ** -149
     x[12:] = torch.randn(8, 96, generator=torch.Generator().manual_seed(5)) * 1e-9
-    for g in ((1.0, 2.0 ** -30, 2.0 ** 60, 1e-37) if fmt == "nvfp4" else (1.0,)):
+    for g in ((1.0, 2.0 ** -30, 2.0 ** -60, 2.0 ** 60, 1e-37) if fmt == "nvfp4" else (1.0,)):
         assert_fp4_equal(lowp.fp4_quantize(x.cuda(), fmt, g), x, fmt, g)
 
 

@@ -119,6 +119,15 @@ def test_c_abi_refuses_before_any_launch():
     assert linear(M=1 << 28) == UNSUPPORTED
     assert linear(M=0, a=None, out=None) == 0
 
+    def rows(fmt=0, x=16, dt=0, ldx=32, w=16, sw=128, gw=1.0, bias=None, act=0, out=16, ldo=8, M=4, N=8, K=32, ws=256,
+             size=1 << 20):
+        return lib.icsa_fp4_linear_rows(fmt, x, dt, ldx, w, sw, gw, bias, act, out, ldo, M, N, K, ws, size, None)
+    for bad in (dict(fmt=7), dict(w=8), dict(sw=None), dict(gw=-1.0), dict(bias=3), dict(act=2), dict(out=None),
+                dict(ldo=7), dict(M=-1), dict(N=0), dict(K=0), dict(ws=128)):
+        assert rows(**bad) == INVALID, bad
+    assert rows(ws=None) == WORKSPACE and rows(size=100) == WORKSPACE
+    assert rows(M=0, x=None, out=None, ws=None, size=0) == 0
+
     strides = (ctypes.c_int64 * 3)(0, 256, 128)
     odd = (ctypes.c_int64 * 3)(0, 257, 128)
     neg = (ctypes.c_int64 * 3)(0, -256, 128)
