@@ -186,6 +186,21 @@ int encode_rows_tensor_map(CUtensorMap* m, const void* base, int B, int rows, in
   return encode_rows_map(m, base, B, rows, H, D, row_stride);
 }
 
+int encode_heads_tensor_map(CUtensorMap* m, const void* base, int B, int L, int H, int D, uint64_t batch_bytes,
+                            uint64_t token_bytes, uint64_t head_bytes, int box_heads, int box_tokens) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return fail(ICSA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(H), cuuint64_t(L), cuuint64_t(B)};
+  const cuuint64_t strides[3] = {head_bytes, token_bytes, batch_bytes};
+  const cuuint32_t box[4] = {64, cuuint32_t(box_heads), cuuint32_t(box_tokens), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ICSA_ERR_CUDA, "cuTensorMapEncodeTiled (heads map) failed with %d", int(r));
+  return ICSA_OK;
+}
+
 int encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t cols, uint64_t rows,
                          uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn enc = get_encode_fn();
@@ -703,7 +718,7 @@ int icsa_dit_linear_residual(const void* a, int64_t lda, const void* w, int64_t 
 }
 
 int icsa_last_status(cudaStream_t stream, int clear) {
-  constexpr int kUnits = 7;
+  constexpr int kUnits = 8;
   static std::mutex mu;
   static int* addr[kMaxDevices][kUnits] = {};
   cudaError_t e = cudaStreamSynchronize(stream);
@@ -716,7 +731,7 @@ int icsa_last_status(cudaStream_t stream, int clear) {
     cudaError_t (*const get[kUnits])(int**) = {icsa::sticky_status_dense_pair, icsa::sticky_status_flat,
                                                icsa::sticky_status_sparse, icsa::sticky_status_selftest,
                                                icsa::sticky_status_gemm, icsa::sticky_status_scores,
-                                               icsa::sticky_status_fp4};
+                                               icsa::sticky_status_fp4, icsa::sticky_status_kv8_tc};
     int* a[kUnits] = {};
     for (int i = 0; i < kUnits; ++i)
       if ((e = get[i](&a[i])) != cudaSuccess) return cuda_fail(e, "sticky status address");

@@ -106,7 +106,7 @@ ICSA_DEV void producer(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
     const int sw0 = t.nt * 2 * p.k_steps * ATOMS, sw1 = sw0 + p.k_steps * ATOMS;
     for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
       const int s = it % kStages;
-      if (!pair::wait(&sm.empty[s], (uint32_t(it / kStages) & 1u) ^ 1u, nullptr, kErrEmpty, abort_flag)) {
+      if (!mbar_wait(&sm.empty[s], (uint32_t(it / kStages) & 1u) ^ 1u, nullptr, kErrEmpty, abort_flag)) {
         *issued = it;
         return;
       }
@@ -213,11 +213,11 @@ ICSA_DEV void issuer(const Fp4GemmParams& p, Smem& sm, uint32_t tmem) {
   for (int u = cluster; u < p.units; u += clusters, ++count) {
     const Unit t = decode_unit(p, u);
     // the epilogue has read the previous tile's accumulator
-    if (!pair::warp_wait(&sm.acc_empty, (uint32_t(count) & 1u) ^ 1u, nullptr, kErrAccEmpty, abort_flag)) return;
+    if (!attn::warp_mbar_wait(&sm.acc_empty, (uint32_t(count) & 1u) ^ 1u, nullptr, kErrAccEmpty, abort_flag)) return;
     tc::fence_after_sync();
     for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
       const int s = it % kStages;
-      if (!pair::warp_wait(&sm.full[s], uint32_t(it / kStages) & 1u, nullptr, kErrFull, abort_flag)) return;
+      if (!attn::warp_mbar_wait(&sm.full[s], uint32_t(it / kStages) & 1u, nullptr, kErrFull, abort_flag)) return;
       tc::fence_after_sync();
       const uint32_t sfa = tmem + kTmScale + uint32_t(it & 1) * kTmScaleStep, sfb = sfa + kTmSfb;
       const uint64_t sad = sad0 + uint64_t(s) * (4 * kScaleAtomBytes >> 4);
@@ -281,7 +281,7 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
       bias[threadIdx.x & 127] = bv;
       pair::named_sync(1u + uint32_t(w), 128);
     }
-    const bool ok = pair::warp_wait(&sm.acc_full, uint32_t(count) & 1u, nullptr, kErrAccFull, abort_flag);
+    const bool ok = attn::warp_mbar_wait(&sm.acc_full, uint32_t(count) & 1u, nullptr, kErrAccFull, abort_flag);
     tc::fence_after_sync();
     float acc[128];
     attn::tmem_load_row128(src, acc);

@@ -13,6 +13,8 @@ namespace icsa {
 // icsa_status other than ICSA_OK returned.  rows: bf16 [B, rows, H, D] with
 // 64 x 64 boxes and 128-byte swizzle, rows `row_stride` elements apart.
 int encode_rows_tensor_map(CUtensorMap* m, const void* base, int B, int rows, int H, int D, int64_t row_stride);
+int encode_heads_tensor_map(CUtensorMap* m, const void* base, int B, int L, int H, int D, uint64_t batch_bytes,
+                            uint64_t token_bytes, uint64_t head_bytes, int box_heads, int box_tokens);
 int encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t cols, uint64_t rows,
                          uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
@@ -151,5 +153,6 @@ cudaError_t sticky_status_selftest(int** out);
 cudaError_t sticky_status_gemm(int** out);
 cudaError_t sticky_status_scores(int** out);
 cudaError_t sticky_status_fp4(int** out);
+cudaError_t sticky_status_kv8_tc(int** out);
 
 }  // namespace icsa

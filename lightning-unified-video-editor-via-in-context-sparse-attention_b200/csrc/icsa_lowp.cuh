@@ -102,4 +102,33 @@ struct Kv8AttnParams {
 int kv8_decode_splits(int B, int H, int rows, int L, int num_sms);
 cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream);
 
+// The same for many query rows, on the tensor cores of SM pairs, for at most
+// kKv8TcMaxBatch sequences.
+constexpr int kKv8TcMaxBatch = 128;
+struct Kv8TcParams {
+  const __nv_bfloat16* q;  // [B, Lq, Hq, D]
+  int64_t q_sb, q_st, q_sh;
+  __nv_bfloat16* out;      // [B, Lq, Hq, D] contiguous
+  int Lq, Hq, group;
+  int rows;                // Lq * group query rows per cache head
+  float scale_log2;
+  float* partial;          // plan.bytes
+  int tiles, rounds, whole;  // from the plan
+  int q_tma, o_tma;          // queries loaded / output stored by TMA through the maps
+};
+struct Kv8TcMaps {
+  CUtensorMap q;  // bf16 [B, Lq, Hq, D], box {64, group, 128 / group, 1}, 128-byte swizzle
+  CUtensorMap o;  // the same of the output, box {64, group, 32 / group, 1}
+};
+struct Kv8TcPlan {
+  int tiles, rounds;       // 256-row tiles and pairs of them per cache head
+  bool whole;              // all key steps fit the ring of stages: rounds are not cut
+  int clusters;
+  size_t bytes;            // partial results
+};
+Kv8TcPlan kv8_tc_plan(const Kv8Cache& c, int rows, int num_sms);
+cudaError_t launch_kv8_tc(Kv8TcParams p, const Kv8TcMaps& maps, const Kv8TcPlan& plan, const Kv8Cache& c,
+                          cudaStream_t stream);
+cudaError_t sticky_status_kv8_tc(int** out);
+
 }  // namespace icsa

@@ -170,28 +170,65 @@ int check_cache_buffers(const char* who, const icsa_kv8_cache* c, bool k, bool v
   return ICSA_OK;
 }
 
-// Few query rows per cache head read the cache as it is; more run the tensor
-// core kernels on a bf16 copy of it.
-constexpr int kDecodeRows = 32;
+// Few query rows per cache head: the register-fed kernel, which takes 8 rows a
+// CTA.  Measured against the pair kernel, us: 2 x 40 heads, D = 128, 32760
+// keys, 32 rows 542 / 566, 64 rows 818 / 566; 300 keys, 48 rows 24 / 28, 64
+// rows 35 / 28; 1 x 8 heads, 32760 keys, 48 rows 60 / 97; 2 x 40, D = 64,
+// 32760 keys, 48 rows 349 / 417.
+constexpr int kDecodeRows = 48;
+
+enum AttnPath { kDecode, kPairs, kDense };
 
 struct AttnPlan {
-  bool decode;
-  int splits;
-  size_t bytes;    // workspace
-  size_t v_offset; // bf16 copy of the values
+  AttnPath path;
+  int splits;            // kDecode
+  icsa::Kv8TcPlan tc;    // kPairs
+  size_t v_offset;       // kDense: bf16 copy of the values, behind that of the keys
+  size_t bytes;          // workspace
 };
+
+// Estimated times of the two ways to attend over a cache whose steps do not
+// fit the pair kernel's ring.  The dense kernels run a 256-row tile per SM
+// pair (D = 128) or SM (D = 64) at a time, 0.86 / 1.87 us a step of 128 keys,
+// in waves of about 7 us beside the steps, on a bf16 copy that is written and
+// read (6 bytes an element).  The pair kernel takes 2.6 us (D = 64: 2.0) for
+// a step of two tiles and 2.2 us (1.6) for one, deals the steps evenly to all
+// pairs and has about 40 us of its own (the join among them).
+// Measured, us, dense / pairs, D = 128: 1 x 40 heads, 1560 rows, 32760 keys
+// 1036 / 1228; 4096 rows 2091 / 2453; 2 x 40, 512 rows 973 / 640; 256 rows
+// 762 / 585; 1 x 8, 2000 rows, 4096 keys 47 / 77.  D = 64: 2 x 40, 2048 rows,
+// 8192 keys 651 / 583; 2 x 8, 512 rows 143 / 64.
+double dense_us(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
+  const bool wide = c.D == 128;
+  const int64_t tiles = int64_t(c.B) * Hq * ((Lq + 255) / 256), units = std::max(1, wide ? sms / 2 : sms);
+  const int64_t steps = (int64_t(c.L) + 127) / 128, waves = (tiles + units - 1) / units;
+  return waves * (steps * (wide ? 0.86 : 1.87) + 7.0) + 6.0 * c.B * c.H * double(c.L) * c.D / 5.5e6 + 8.0;
+}
+double pairs_us(const icsa::Kv8Cache& c, const icsa::Kv8TcPlan& t, int sms) {
+  const bool wide = c.D == 128;
+  const double steps = (double(c.L) + 127) / 128;
+  const double head = (t.tiles / 2) * (wide ? 2.6 : 2.0) + (t.tiles & 1) * (wide ? 2.2 : 1.6);
+  return double(c.B) * c.H * steps * head / std::max(1, sms / 2) + 40.0;
+}
 
 AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   AttnPlan a = {};
   const int64_t rows = int64_t(Lq) * (Hq / c.H);
-  a.decode = rows <= kDecodeRows;
-  if (a.decode) {
+  if (rows <= kDecodeRows) {
+    a.path = kDecode;
     a.splits = icsa::kv8_decode_splits(c.B, c.H, int(rows), c.L, sms);
     a.bytes = a.splits == 1 ? 0 : align256(size_t(c.B) * c.H * rows * a.splits * (c.D + 2) * sizeof(float));
-  } else {
+    return a;
+  }
+  a.tc = icsa::kv8_tc_plan(c, int(rows), sms);
+  if (!a.tc.whole && c.nb <= 16384 && dense_us(c, Lq, Hq, sms) < pairs_us(c, a.tc, sms)) {
+    a.path = kDense;
     a.v_offset = align256(size_t(c.B) * c.L * c.H * c.D * 2);
     a.bytes = 2 * a.v_offset;
+    return a;
   }
+  a.path = kPairs;
+  a.bytes = align256(a.tc.bytes);
   return a;
 }
 
@@ -201,6 +238,39 @@ int check_queries(const char* who, const icsa::Kv8Cache& c, int Lq, int Hq) {
   if (Lq > (1 << 28) || int64_t(Lq) * Hq > 0x7FFFFFFFll)
     return fail(ICSA_ERR_UNSUPPORTED, "%s: Lq=%d, Hq=%d exceed this build's limits", who, Lq, Hq);
   return ICSA_OK;
+}
+
+// The dense tensor core kernels on a bf16 copy of the cache.
+int dense_attention(const icsa::Kv8Cache& c, const AttnPlan& plan, const void* q, const int64_t q_strides[3], void* out,
+                    int Lq, int Hq, float scale_log2, void* workspace, cudaStream_t stream) {
+  if (q_strides[2] != c.D || q_strides[1] < int64_t(Hq) * c.D || (c.B > 1 && q_strides[0] != Lq * q_strides[1]))
+    return fail(ICSA_ERR_UNSUPPORTED, "kv8_attention: %d query tokens over a long cache need contiguous heads, token "
+                "strides of at least Hq * D and a batch stride of Lq tokens", Lq);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  void* const copy[2] = {ws, ws + plan.v_offset};
+  cudaError_t e = icsa::launch_kv8_dequantize(c, copy, ICSA_BF16, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "kv8_attention: bf16 copy of the cache");
+  const int nbq = (Lq + icsa::kBlock - 1) / icsa::kBlock;
+  icsa::AttnMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  int rc;
+  if ((rc = icsa::encode_rows_tensor_map(&maps.q, q, c.B, Lq, Hq, c.D, q_strides[1])) != ICSA_OK) return rc;
+  if ((rc = icsa::encode_rows_tensor_map(&maps.k, copy[0], c.B, c.L, c.H, c.D, 0)) != ICSA_OK) return rc;
+  if ((rc = icsa::encode_rows_tensor_map(&maps.v, copy[1], c.B, c.L, c.H, c.D, 0)) != ICSA_OK) return rc;
+  if ((rc = icsa::encode_rows_tensor_map(&maps.o, out, c.B, Lq, Hq, c.D, 0)) != ICSA_OK) return rc;
+  icsa::AttnParams a;
+  std::memset(&a, 0, sizeof(a));
+  a.B = c.B; a.S = Lq; a.H = Hq; a.NB = nbq;
+  a.num_flat = nbq;
+  a.flat_tiles = (nbq + 1) / 2;
+  a.nkv = c.nb; a.nkv_pad = (c.nb + 127) / 128 * 128; a.tkv = c.L;
+  a.scale_log2 = scale_log2;
+  a.alpha_mode = ICSA_ALPHA_SCALAR;
+  a.out = out; a.out_dtype = ICSA_BF16; a.out_tma = 1;
+  a.kv_lens = c.lengths;
+  a.kv_group = Hq / c.H;
+  e = icsa::launch_flat_attention(a, maps, c.D, stream);
+  return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "kv8_attention");
 }
 
 }  // namespace
@@ -360,7 +430,7 @@ int icsa_kv8_attention(const icsa_kv8_cache* cache, const void* q, const int64_t
     if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "kv8_attention: the workspace must be 256-byte aligned");
   }
   const float scale_log2 = float(std::sqrt(1.0 / c.D) * 1.44269504);
-  if (plan.decode) {
+  if (plan.path == kDecode) {
     icsa::Kv8AttnParams p;
     p.q = static_cast<const __nv_bfloat16*>(q);
     p.q_sb = q_strides[0]; p.q_st = q_strides[1]; p.q_sh = q_strides[2];
@@ -372,36 +442,46 @@ int icsa_kv8_attention(const icsa_kv8_cache* cache, const void* q, const int64_t
     cudaError_t e = icsa::launch_kv8_decode(p, c, stream);
     return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "kv8_attention");
   }
-  // the tensor core kernels take q as rows of Hq * D features, batches Lq rows apart
-  if (q_strides[2] != c.D || q_strides[1] < int64_t(Hq) * c.D || (c.B > 1 && q_strides[0] != Lq * q_strides[1]))
-    return fail(ICSA_ERR_UNSUPPORTED, "kv8_attention: %d query rows need contiguous heads, token strides of at least "
-                "Hq * D and a batch stride of Lq tokens", Lq);
-  if (c.nb > 16384 || (int64_t(c.B) * Hq) * ((Lq + 255) / 256) > 0x3FFFFFFFll)
-    return fail(ICSA_ERR_UNSUPPORTED, "kv8_attention: L=%d / Lq=%d exceed this build's limits", c.L, Lq);
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  void* const copy[2] = {ws, ws + plan.v_offset};
-  cudaError_t e = icsa::launch_kv8_dequantize(c, copy, ICSA_BF16, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "kv8_attention: bf16 copy of the cache");
-  const int nbq = (Lq + icsa::kBlock - 1) / icsa::kBlock;
-  icsa::AttnMaps maps;
-  std::memset(&maps, 0, sizeof(maps));
-  if ((rc = icsa::encode_rows_tensor_map(&maps.q, q, c.B, Lq, Hq, c.D, q_strides[1])) != ICSA_OK) return rc;
-  if ((rc = icsa::encode_rows_tensor_map(&maps.k, copy[0], c.B, c.L, c.H, c.D, 0)) != ICSA_OK) return rc;
-  if ((rc = icsa::encode_rows_tensor_map(&maps.v, copy[1], c.B, c.L, c.H, c.D, 0)) != ICSA_OK) return rc;
-  if ((rc = icsa::encode_rows_tensor_map(&maps.o, out, c.B, Lq, Hq, c.D, 0)) != ICSA_OK) return rc;
-  icsa::AttnParams a;
-  std::memset(&a, 0, sizeof(a));
-  a.B = c.B; a.S = Lq; a.H = Hq; a.NB = nbq;
-  a.num_flat = nbq;
-  a.flat_tiles = (nbq + 1) / 2;
-  a.nkv = c.nb; a.nkv_pad = (c.nb + 127) / 128 * 128; a.tkv = c.L;
-  a.scale_log2 = scale_log2;
-  a.alpha_mode = ICSA_ALPHA_SCALAR;
-  a.out = out; a.out_dtype = ICSA_BF16; a.out_tma = 1;
-  a.kv_lens = c.lengths;
-  a.kv_group = Hq / c.H;
-  e = icsa::launch_flat_attention(a, maps, c.D, stream);
-  return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "kv8_attention");
+  if (plan.path == kDense) return dense_attention(c, plan, q, q_strides, out, Lq, Hq, scale_log2, workspace, stream);
+  icsa::Kv8TcParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = q_strides[0]; p.q_st = q_strides[1]; p.q_sh = q_strides[2];
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.Lq = Lq; p.Hq = Hq; p.group = Hq / c.H;
+  p.rows = Lq * p.group;
+  p.scale_log2 = scale_log2;
+  p.partial = static_cast<float*>(workspace);
+  // boxes of whole tokens of a group; strides of 0 are left to the copies
+  p.q_tma = 128 % p.group == 0 && (c.B == 1 || q_strides[0] > 0) && (Lq == 1 || q_strides[1] > 0) &&
+            (Hq == 1 || q_strides[2] > 0);
+  p.o_tma = 32 % p.group == 0;
+  const auto st = [&](int i, int n) { return uint64_t(n == 1 ? 8 : q_strides[i]) * 2; };  // an axis of one has any stride
+  const uint64_t row = uint64_t(Hq) * c.D * 2;
+  const size_t blocks = size_t(c.H) * c.nb;  // of one sequence
+  for (int b0 = 0; b0 < c.B; b0 += icsa::kKv8TcMaxBatch) {
+    icsa::Kv8Cache part = c;
+    part.B = std::min(c.B - b0, icsa::kKv8TcMaxBatch);
+    part.k += size_t(b0) * blocks * 64 * c.D;
+    part.v += size_t(b0) * blocks * 64 * c.D;
+    part.k_scale += size_t(b0) * blocks;
+    part.v_scale += size_t(b0) * blocks;
+    if (c.lengths != nullptr) part.lengths += b0;
+    icsa::Kv8TcParams pp = p;
+    pp.q += int64_t(b0) * p.q_sb;
+    pp.out += int64_t(b0) * Lq * Hq * c.D;
+    icsa::Kv8TcMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    if (p.q_tma && (rc = icsa::encode_heads_tensor_map(&maps.q, pp.q, part.B, Lq, Hq, c.D, st(0, c.B), st(1, Lq),
+                                                       st(2, Hq), p.group, 128 / p.group)) != ICSA_OK)
+      return rc;
+    if (p.o_tma && (rc = icsa::encode_heads_tensor_map(&maps.o, pp.out, part.B, Lq, Hq, c.D, Lq * row, row,
+                                                       uint64_t(c.D) * 2, p.group, 32 / p.group)) != ICSA_OK)
+      return rc;
+    cudaError_t e = icsa::launch_kv8_tc(pp, maps, icsa::kv8_tc_plan(part, p.rows, sms), part, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "kv8_attention");
+  }
+  return ICSA_OK;
 }
 
 }  // extern "C"
