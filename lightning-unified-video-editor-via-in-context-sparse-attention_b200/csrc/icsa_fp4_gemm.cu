@@ -257,7 +257,7 @@ ICSA_DEV float finish(const Fp4GemmParams& p, float acc, float bias) {
 // so the accumulator is free again after one TMEM read; the output leaves in
 // 32-row x 64-column boxes staged in shared memory (one 4 KB box a warp,
 // 128-byte swizzle) and written by TMA, which stores whole lines and clips
-// the tile at M and N.  (Storing the rows straight from registers, 16 bytes
+// the tile at M and N, or row by row where the output's rows are not aligned.  (Storing the rows straight from registers, 16 bytes
 // a lane in 32 different lines, took 8600 clk a tile, more than half of a
 // K = 5120 main loop.)
 ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm, uint32_t tmem, uint32_t rank) {
@@ -298,40 +298,48 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
       for (int i = 0; i < 32; ++i) dst[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
       continue;
     }
-    if (p.tma_out) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (c0 + 64 * h >= p.N) break;
-        // the box's previous contents have been read by their store
-        if (lane == 0) bulk_wait_read();
-        __syncwarp();
+    for (int h = 0; h < 2; ++h) {
+      const int cols = p.N - (c0 + 64 * h);
+      if (cols <= 0) break;
+      // the box's previous contents have been read by their store
+      if (p.tma_out && lane == 0) bulk_wait_read();
+      __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 b0 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i);
-          const float4 b1 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i + 4);
-          const float* x = acc + 64 * h + 8 * i;
-          uint4 o;
-          o.x = pack_bf16x2(finish(p, x[0], b0.x), finish(p, x[1], b0.y));
-          o.y = pack_bf16x2(finish(p, x[2], b0.z), finish(p, x[3], b0.w));
-          o.z = pack_bf16x2(finish(p, x[4], b1.x), finish(p, x[5], b1.y));
-          o.w = pack_bf16x2(finish(p, x[6], b1.z), finish(p, x[7], b1.w));
-          *reinterpret_cast<uint4*>(box + lane * 128 + ((uint32_t(i) ^ uint32_t(lane & 7)) << 4)) = o;
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float4 b0 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i);
+        const float4 b1 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i + 4);
+        const float* x = acc + 64 * h + 8 * i;
+        uint4 o;
+        o.x = pack_bf16x2(finish(p, x[0], b0.x), finish(p, x[1], b0.y));
+        o.y = pack_bf16x2(finish(p, x[2], b0.z), finish(p, x[3], b0.w));
+        o.z = pack_bf16x2(finish(p, x[4], b1.x), finish(p, x[5], b1.y));
+        o.w = pack_bf16x2(finish(p, x[6], b1.z), finish(p, x[7], b1.w));
+        *reinterpret_cast<uint4*>(box + lane * 128 + ((uint32_t(i) ^ uint32_t(lane & 7)) << 4)) = o;
+      }
+      if (p.tma_out) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           tma_store_2d(&maps.out, box, c0 + 64 * h, row0);
           bulk_commit();
         }
+        continue;
       }
-      continue;
+      // an output whose rows are not 16-byte aligned: row by row, so that a
+      // warp's stores still fill lines
+      __syncwarp();
+      const int rows = min(32, p.M - row0);
+      __nv_bfloat16* dst = p.out + size_t(row0) * p.ldo + c0 + 64 * h;
+#pragma unroll 4
+      for (int q = 0; q < rows; ++q, dst += p.ldo) {
+        const uint32_t w2 = *reinterpret_cast<const uint32_t*>(
+            box + q * 128 + ((uint32_t(lane >> 2) ^ uint32_t(q & 7)) << 4) + (lane & 3) * 4);
+        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w2);
+        if (2 * lane < cols) dst[2 * lane] = v.x;
+        if (2 * lane + 1 < cols) dst[2 * lane + 1] = v.y;
+      }
     }
-    // an output whose rows are not 16-byte aligned
-    if (r >= p.M) continue;
-    __nv_bfloat16* dst = p.out + size_t(r) * p.ldo + c0;
-#pragma unroll
-    for (int i = 0; i < 128; ++i)
-      if (c0 + i < p.N) dst[i] = __float2bfloat16_rn(finish(p, acc[i], bias[i]));
   }
   if (lane == 0) bulk_wait_read();
 }
@@ -367,6 +375,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   pair::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
+  wait_prior_grid();  // the operands are the previous kernels' outputs
   if (warp < 8) {
     epilogue(p, maps, sm, tmem, rank);
   } else if (warp == kProducerWarp) {
@@ -396,6 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 __global__ void __launch_bounds__(256) fp4_reduce_kernel(const Fp4GemmParams p) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   const int r = blockIdx.y;
+  wait_prior_grid();
   if (c >= p.N) return;
   float acc = 0.f;
   for (int s = 0; s < p.splits; ++s) acc += p.partial[(size_t(s) * p.M + r) * p.n_pad + c];
@@ -409,7 +419,19 @@ int fp4_gemm_splits(int M, int N, int K, int num_sms) {
   const int k_steps = (K + kFp4TileK - 1) / kFp4TileK;
   const int clusters = std::max(1, num_sms / 2);
   if (tiles <= 0 || tiles * 2 > clusters || M > 65535) return 1;
-  return int(std::max<int64_t>(1, std::min<int64_t>(clusters / tiles, k_steps)));
+  // a step takes about 0.37 us; splitting costs the second kernel (3 us) and
+  // the partial sums, written and read at about 4 TB/s
+  const int most = int(std::min<int64_t>(clusters / tiles, k_steps));
+  int best = 1;
+  double best_us = k_steps * 0.37;
+  for (int s = 2; s <= most; ++s) {
+    const double us = (k_steps + s - 1) / s * 0.37 + 3.0 + 8.0 * s * M * double(N) / 4e6;
+    if (us < best_us) {
+      best_us = us;
+      best = s;
+    }
+  }
+  return best;
 }
 
 cudaError_t launch_fp4_gemm(Fp4GemmParams p, const Fp4GemmMaps& maps, int format, int num_sms, cudaStream_t stream) {
@@ -423,10 +445,9 @@ cudaError_t launch_fp4_gemm(Fp4GemmParams p, const Fp4GemmMaps& maps, int format
   auto kernel = format == ICSA_NVFP4 ? fp4_gemm_kernel<ICSA_NVFP4> : fp4_gemm_kernel<ICSA_MXFP4>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
-  kernel<<<2 * clusters, kThreads, smem, stream>>>(p, maps);
-  if ((e = cudaGetLastError()) != cudaSuccess || p.splits == 1) return e;
-  fp4_reduce_kernel<<<dim3((p.N + 255) / 256, p.M), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  e = launch_chained(kernel, dim3(2 * clusters), dim3(kThreads), smem, stream, p, maps);
+  if (e != cudaSuccess || p.splits == 1) return e;
+  return launch_chained(fp4_reduce_kernel, dim3((p.N + 255) / 256, p.M), dim3(256), 0, stream, p);
 }
 
 ICSA_DEFINE_STICKY_ACCESSOR(sticky_status_fp4)

@@ -111,8 +111,9 @@ template <typename T, int D>
 __global__ void __launch_bounds__(FillShape<D>::kThreads) kv8_quantize_kernel(const Kv8Rows x, const Kv8Cache c) {
   constexpr int kPerRow = FillShape<D>::kPerRow, kThreads = FillShape<D>::kThreads;
   const int which = blockIdx.y;
-  const int blk = blockIdx.x % c.nb, bh = blockIdx.x / c.nb;
-  const int b = bh / c.H, h = bh % c.H;
+  // heads run fastest: the CTAs of one time read whole rows of x
+  const int h = blockIdx.x % c.H, bk = blockIdx.x / c.H;
+  const int blk = bk % c.nb, b = bk / c.nb, bh = b * c.H + h;
   const int len = valid_tokens(c, b);
   const int f0 = (threadIdx.x % kPerRow) * 8, g = threadIdx.x / kPerRow;
   const T* base = static_cast<const T*>(x.x[which]) + b * x.sb[which] + h * x.sh[which] + f0;
@@ -167,22 +168,23 @@ __global__ void __launch_bounds__(FillShape<D>::kThreads) kv8_quantize_kernel(co
     for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(dst + i * D) = make_uint2(code[0][i], code[1][i]);
     return;
   }
-  // values: words of four tokens, [feature][token / 4]
-  __shared__ uint32_t tile[D][17];
-  __syncthreads();
+  // values: words of four tokens, [feature][token / 4], the words of two
+  // features in an order that keeps stores and loads off each other's banks
+  __shared__ uint32_t tile[D * 16];
+  auto word = [](int f, int q) { return (f >> 1) * 32 + ((f ^ q) & 1) * 16 + (q ^ ((f >> 3) & 15)); };
 #pragma unroll
   for (int e8 = 0; e8 < 8; ++e8) {
     const uint32_t sel = uint32_t(e8 & 3) | (uint32_t((e8 & 3) + 4) << 4);
     const uint32_t p01 = __byte_perm(code[e8 >> 2][0], code[e8 >> 2][1], sel);
     const uint32_t p23 = __byte_perm(code[e8 >> 2][2], code[e8 >> 2][3], sel);
-    tile[f0 + e8][g] = (p01 & 0xFFFFu) | (p23 << 16);
+    tile[word(f0 + e8, g)] = (p01 & 0xFFFFu) | (p23 << 16);
   }
   __syncthreads();
   uint32_t* out = reinterpret_cast<uint32_t*>(c.v + slot * kTokens * D);
 #pragma unroll
   for (int i = 0; i < D * 16 / kThreads; ++i) {
     const int wd = i * kThreads + threadIdx.x;
-    out[wd] = tile[wd >> 4][wd & 15];
+    out[wd] = tile[word(wd >> 4, wd & 15)];
   }
 }
 
@@ -515,6 +517,7 @@ template <int D>
 __global__ void __launch_bounds__(D) kv8_join_kernel(const Kv8AttnParams p, const Kv8Cache c) {
   const int rows = p.Lq * p.group;
   const int r = blockIdx.x, bh = blockIdx.y, b = bh / c.H, h = bh % c.H, d = threadIdx.x;
+  wait_prior_grid();
   const float* src = p.partial + (size_t(bh) * rows + r) * p.splits * (D + 2);
   float mm = kNegInf;
   for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, src[s * (D + 2) + D]);
@@ -572,9 +575,8 @@ cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStr
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;
   const dim3 jgrid(rows, c.B * c.H);
-  if (c.D == 128) kv8_join_kernel<128><<<jgrid, 128, 0, stream>>>(p, c);
-  else kv8_join_kernel<64><<<jgrid, 64, 0, stream>>>(p, c);
-  return cudaGetLastError();
+  return c.D == 128 ? launch_chained(kv8_join_kernel<128>, jgrid, dim3(128), 0, stream, p, c)
+                    : launch_chained(kv8_join_kernel<64>, jgrid, dim3(64), 0, stream, p, c);
 }
 
 }  // namespace icsa

@@ -937,6 +937,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   pair::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
+  wait_prior_grid();
   // Register split: 512 threads launch with 128 registers each;
   // 256 x 176 + 128 x 104 + 128 x 56 = 512 x 128.
   if (warp < 8) {
@@ -984,6 +985,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 template <int D>
 __global__ void __launch_bounds__(256) kv8_tc_join_kernel(const Kv8TcParams p, const Kv8Cache c, int clusters) {
   const int k = int(blockIdx.x) + 1;
+  wait_prior_grid();
   int64_t total = 0;
   for (int i = 0; i < c.B; ++i) total += extent(p, cache_length(c, i)).head * c.H;
   // cluster k covers [total k / clusters, total (k + 1) / clusters)
@@ -1048,8 +1050,8 @@ cudaError_t launch_as(const Kv8TcParams& p, const Kv8TcMaps& maps, const Kv8Cach
   kv8_tc_kernel<D><<<2 * clusters, kThreads, smem, stream>>>(p, c, maps);
   if ((e = cudaGetLastError()) != cudaSuccess || p.whole || clusters == 1) return e;
   const int rows = std::min(p.rows, 2 * kPairRows);
-  kv8_tc_join_kernel<D><<<dim3(clusters - 1, (rows + 31) / 32), 256, 0, stream>>>(p, c, clusters);
-  return cudaGetLastError();
+  return launch_chained(kv8_tc_join_kernel<D>, dim3(clusters - 1, (rows + 31) / 32), dim3(256), 0, stream, p, c,
+                        clusters);
 }
 
 }  // namespace

@@ -183,23 +183,25 @@ def test_linear_layer_refuses_mixed_formats_and_devices():
     assert lowp.fp4_linear(x[:0], w, b).shape == (0, 32)
 
 
-def test_linear_layer_checks_its_workspace_and_leaves_what_is_behind_its_rows():
+@pytest.mark.parametrize("M,K", [(3, 2048), (9, 4096)])
+def test_linear_layer_checks_its_workspace_and_leaves_what_is_behind_its_rows(M, K):
     lib = lowp._load()
-    x, w, b, want, tol = linear_case(3, 40, 2048, "nvfp4", True, None)
+    x, w, b, want, tol = linear_case(M, 40, K, "nvfp4", True, None)
     a = lowp.fp4_quantize(x, "nvfp4")
-    size = lib.icsa_fp4_linear_workspace_size(3, 40, 2048)
-    assert size > 0                                              # few tiles: K is split
-    out = torch.full((5, 48), 7.0, dtype=torch.bfloat16, device="cuda")
+    size = lib.icsa_fp4_linear_workspace_size(M, 40, K)
+    assert (size > 0) == (M > 4)                                 # few tiles of several rows: K is split
+    out = torch.full((M + 2, 48), 7.0, dtype=torch.bfloat16, device="cuda")
     ws = torch.full((size + 256,), 0xFF, dtype=torch.uint8, device="cuda")
 
     def call(ws_ptr, nbytes):
         return lib.icsa_fp4_linear(0, a.data.data_ptr(), a.scales.data_ptr(), 1.0, w.data.data_ptr(),
-                                   w.scales.data_ptr(), w.global_scale, b.data_ptr(), 0, out.data_ptr(), 48, 3, 40,
-                                   2048, ws_ptr, nbytes, torch.cuda.current_stream().cuda_stream)
-    assert call(None, size) == 4 and call(ws.data_ptr(), size - 1) == 4 and call(ws.data_ptr() + 16, size) == 1
+                                   w.scales.data_ptr(), w.global_scale, b.data_ptr(), 0, out.data_ptr(), 48, M, 40,
+                                   K, ws_ptr, nbytes, torch.cuda.current_stream().cuda_stream)
+    if size:
+        assert call(None, size) == 4 and call(ws.data_ptr(), size - 1) == 4 and call(ws.data_ptr() + 16, size) == 1
     assert call(ws.data_ptr(), size) == 0
-    assert bool(((out[:3, :40].double() - want).abs() <= tol).all())
-    assert bool((out[3:] == 7).all()) and bool((out[:, 40:] == 7).all()) and bool((ws[size:] == 0xFF).all())
+    assert bool(((out[:M, :40].double() - want).abs() <= tol).all())
+    assert bool((out[M:] == 7).all()) and bool((out[:, 40:] == 7).all()) and bool((ws[size:] == 0xFF).all())
 
 
 # --------------------------------------------------------------------------- cache
