@@ -68,37 +68,61 @@ ICSA_DEV uint32_t e4m3x2(float lo, float hi) {
 }
 
 // ---------------------------------------------------------------- filling --
-// One CTA per (block, head, batch) and tensor (grid.y: keys, values).  Thread:
-// 8 consecutive features of tokens 4 i .. 4 i + 3, so that the four tokens'
-// bytes of one feature make a word of the transposed value block.
-template <typename T, int D>
-ICSA_DEV void load8(const T* p, bool vec, float (&v)[8]) {
+// One CTA per (block, head, batch): keys and values together in bfloat16, so
+// that 32 KB are on their way before the first is needed, one tensor a CTA in
+// float32 (as many bytes).  Thread: 8 consecutive features of tokens
+// 4 i .. 4 i + 3, so that the four tokens' bytes of one feature make a word
+// of the transposed value block.
+template <typename T>
+constexpr int fill_tensors() { return sizeof(T) == 2 ? 2 : 1; }
+
+template <typename T>
+struct Raw8 {  // 8 elements as loaded
+  uint32_t w[2 * sizeof(T)];
+};
+
+template <typename T>
+ICSA_DEV void load_raw(const T* p, bool vec, Raw8<T>& x) {
   if (vec) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float4 u = __ldg(reinterpret_cast<const float4*>(p) + h);
-        v[4 * h] = u.x;
-        v[4 * h + 1] = u.y;
-        v[4 * h + 2] = u.z;
-        v[4 * h + 3] = u.w;
-      }
+    for (int h = 0; h < int(sizeof(T)) / 2; ++h) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + h);
+      x.w[4 * h] = u.x;
+      x.w[4 * h + 1] = u.y;
+      x.w[4 * h + 2] = u.z;
+      x.w[4 * h + 3] = u.w;
     }
     return;
   }
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (sizeof(T) == 2) v[i] = __bfloat162float(p[i]);
-    else v[i] = p[i];
+    for (int i = 0; i < 4; ++i) x.w[i] = uint32_t(q[2 * i]) | (uint32_t(q[2 * i + 1]) << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.w[i] = __float_as_uint(p[i]);
   }
+}
+
+template <typename T>
+ICSA_DEV float raw_float(const Raw8<T>& x, int i) {
+  if constexpr (sizeof(T) == 2) return __uint_as_float(i & 1 ? x.w[i >> 1] & 0xFFFF0000u : x.w[i >> 1] << 16);
+  else return __uint_as_float(x.w[i]);
+}
+
+// largest magnitude of four rows as float bits: NaN and infinity stay above every number
+template <typename T>
+ICSA_DEV uint32_t raw_top(const Raw8<T> (&x)[4]) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < int(2 * sizeof(T)); ++j) {
+      if constexpr (sizeof(T) == 2) top = __vmaxu2(top, x[i].w[j] & 0x7FFF7FFFu);
+      else top = max(top, x[i].w[j] & 0x7FFFFFFFu);
+    }
+  if constexpr (sizeof(T) == 2) top = max(top & 0xFFFF0000u, top << 16);
+  return top;
 }
 
 template <int D>
@@ -110,81 +134,89 @@ struct FillShape {
 template <typename T, int D>
 __global__ void __launch_bounds__(FillShape<D>::kThreads) kv8_quantize_kernel(const Kv8Rows x, const Kv8Cache c) {
   constexpr int kPerRow = FillShape<D>::kPerRow, kThreads = FillShape<D>::kThreads;
-  const int which = blockIdx.y;
+  constexpr int kTensors = fill_tensors<T>();
   // heads run fastest: the CTAs of one time read whole rows of x
   const int h = blockIdx.x % c.H, bk = blockIdx.x / c.H;
   const int blk = bk % c.nb, b = bk / c.nb, bh = b * c.H + h;
   const int len = valid_tokens(c, b);
   const int f0 = (threadIdx.x % kPerRow) * 8, g = threadIdx.x / kPerRow;
-  const T* base = static_cast<const T*>(x.x[which]) + b * x.sb[which] + h * x.sh[which] + f0;
-  // 16-byte accesses: every row start and stride aligned
-  const bool vec = (reinterpret_cast<uintptr_t>(x.x[which]) & 15u) == 0 &&
-                   ((x.sb[which] | x.st[which] | x.sh[which]) * int64_t(sizeof(T))) % 16 == 0;
-  float v[4][8];
-  uint32_t top = 0;  // largest magnitude as bits: NaN and infinity stay above every number
+  Raw8<T> raw[kTensors][4];
+  __shared__ uint32_t tops[kTensors][kThreads / 32];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int tok = blk * kTokens + 4 * g + i;
-    if (tok < len) {
-      load8<T, D>(base + int64_t(tok) * x.st[which], vec, v[i]);
-    } else {
+  for (int t = 0; t < kTensors; ++t) {
+    const bool values = kTensors == 2 ? t == 1 : blockIdx.y == 1;
+    const void* from = values ? x.x[1] : x.x[0];
+    const int64_t sb = values ? x.sb[1] : x.sb[0], st = values ? x.st[1] : x.st[0], sh = values ? x.sh[1] : x.sh[0];
+    // 16-byte accesses: every row start and stride aligned
+    const bool vec = (reinterpret_cast<uintptr_t>(from) & 15u) == 0 && ((sb | st | sh) * int64_t(sizeof(T))) % 16 == 0;
+    const T* src = static_cast<const T*>(from) + b * sb + h * sh + int64_t(blk * kTokens + 4 * g) * st + f0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    for (int i = 0; i < 4; ++i, src += st) {
+      if (blk * kTokens + 4 * g + i < len) {
+        load_raw<T>(src, vec, raw[t][i]);
+      } else {
+#pragma unroll
+        for (uint32_t& w : raw[t][i].w) w = 0u;
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7FFFFFFFu);
   }
-  __shared__ uint32_t tops[kThreads / 32];
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+#pragma unroll
+  for (int t = 0; t < kTensors; ++t) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, raw_top(raw[t]));
+    if ((threadIdx.x & 31) == 0) tops[t][threadIdx.x >> 5] = top;
+  }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) top = max(top, tops[i]);
-  // smallest e with amax <= 448 2^e = 1.75 2^(8 + e); a subnormal amax is far
-  // below the clamp at -96
-  int e = int(top >> 23) - 127 - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  e = min(max(e, -96), 96);
-  const bool bad = top >= 0x7F800000u;
-  if (top == 0u || bad) e = 0;
-  const float inv = __uint_as_float(uint32_t(127 - e) << 23);
   const size_t slot = size_t(bh) * c.nb + blk;
-  if (threadIdx.x == 0)
-    (which ? c.v_scale : c.k_scale)[slot] = bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(uint32_t(127 + e) << 23);
-  uint32_t code[2][4];  // [features 0-3 | 4-7][token], 4 code bytes each
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (bad) {
-      code[0][i] = code[1][i] = 0u;
+  for (int t = 0; t < kTensors; ++t) {
+    const bool values = kTensors == 2 ? t == 1 : blockIdx.y == 1;
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) top = max(top, tops[t][i]);
+    // smallest e with amax <= 448 2^e = 1.75 2^(8 + e); a subnormal amax is far
+    // below the clamp at -96
+    int e = int(top >> 23) - 127 - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    e = min(max(e, -96), 96);
+    const bool bad = top >= 0x7F800000u;
+    if (top == 0u || bad) e = 0;
+    const float inv = __uint_as_float(uint32_t(127 - e) << 23);
+    if (threadIdx.x == 0)
+      (values ? c.v_scale : c.k_scale)[slot] =
+          bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(uint32_t(127 + e) << 23);
+    uint32_t code[2][4] = {};  // [features 0-3 | 4-7][token], 4 code bytes each
+    if (!bad) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          code[q][i] = e4m3x2(raw_float(raw[t][i], 4 * q) * inv, raw_float(raw[t][i], 4 * q + 1) * inv) |
+                       (e4m3x2(raw_float(raw[t][i], 4 * q + 2) * inv, raw_float(raw[t][i], 4 * q + 3) * inv) << 16);
+    }
+    if (!values) {
+      uint8_t* dst = c.k + (slot * kTokens + 4 * g) * D + f0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(dst + i * D) = make_uint2(code[0][i], code[1][i]);
       continue;
     }
+    // values: words of four tokens, [feature][token / 4], the words of two
+    // features in an order that keeps stores and loads off each other's banks
+    __shared__ uint32_t tile[D * 16];
+    auto word = [](int f, int q) { return (f >> 1) * 32 + ((f ^ q) & 1) * 16 + (q ^ ((f >> 3) & 15)); };
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
-      code[q][i] = e4m3x2(v[i][4 * q] * inv, v[i][4 * q + 1] * inv) |
-                   (e4m3x2(v[i][4 * q + 2] * inv, v[i][4 * q + 3] * inv) << 16);
-  }
-  if (which == 0) {
-    uint8_t* dst = c.k + (slot * kTokens + 4 * g) * D + f0;
+    for (int e8 = 0; e8 < 8; ++e8) {
+      const uint32_t sel = uint32_t(e8 & 3) | (uint32_t((e8 & 3) + 4) << 4);
+      const uint32_t p01 = __byte_perm(code[e8 >> 2][0], code[e8 >> 2][1], sel);
+      const uint32_t p23 = __byte_perm(code[e8 >> 2][2], code[e8 >> 2][3], sel);
+      tile[word(f0 + e8, g)] = __byte_perm(p01, p23, 0x5410);
+    }
+    __syncthreads();
+    // four words of one feature a thread: 16-byte stores
+    uint4* out = reinterpret_cast<uint4*>(c.v + slot * kTokens * D);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(dst + i * D) = make_uint2(code[0][i], code[1][i]);
-    return;
-  }
-  // values: words of four tokens, [feature][token / 4], the words of two
-  // features in an order that keeps stores and loads off each other's banks
-  __shared__ uint32_t tile[D * 16];
-  auto word = [](int f, int q) { return (f >> 1) * 32 + ((f ^ q) & 1) * 16 + (q ^ ((f >> 3) & 15)); };
-#pragma unroll
-  for (int e8 = 0; e8 < 8; ++e8) {
-    const uint32_t sel = uint32_t(e8 & 3) | (uint32_t((e8 & 3) + 4) << 4);
-    const uint32_t p01 = __byte_perm(code[e8 >> 2][0], code[e8 >> 2][1], sel);
-    const uint32_t p23 = __byte_perm(code[e8 >> 2][2], code[e8 >> 2][3], sel);
-    tile[word(f0 + e8, g)] = (p01 & 0xFFFFu) | (p23 << 16);
-  }
-  __syncthreads();
-  uint32_t* out = reinterpret_cast<uint32_t*>(c.v + slot * kTokens * D);
-#pragma unroll
-  for (int i = 0; i < D * 16 / kThreads; ++i) {
-    const int wd = i * kThreads + threadIdx.x;
-    out[wd] = tile[word(wd >> 4, wd & 15)];
+    for (int i = 0; i < D * 4 / kThreads; ++i) {
+      const int wd = i * kThreads + threadIdx.x, f = wd >> 2, q = (wd & 3) * 4;
+      out[wd] = make_uint4(tile[word(f, q)], tile[word(f, q + 1)], tile[word(f, q + 2)], tile[word(f, q + 3)]);
+    }
   }
 }
 
@@ -534,7 +566,7 @@ __global__ void __launch_bounds__(D) kv8_join_kernel(const Kv8AttnParams p, cons
 
 template <typename T>
 cudaError_t quantize_as(const Kv8Rows& x, const Kv8Cache& c, cudaStream_t stream) {
-  const dim3 grid(unsigned(c.B) * c.H * c.nb, 2);
+  const dim3 grid(unsigned(c.B) * c.H * c.nb, 2 / fill_tensors<T>());
   if (c.D == 128) kv8_quantize_kernel<T, 128><<<grid, FillShape<128>::kThreads, 0, stream>>>(x, c);
   else kv8_quantize_kernel<T, 64><<<grid, FillShape<64>::kThreads, 0, stream>>>(x, c);
   return cudaGetLastError();
