@@ -46,6 +46,7 @@ namespace {
 
 constexpr int kTokens = 64;
 constexpr int kDWarps = 4;           // warps of a decode CTA
+constexpr int decode_ctas(int D) { return D == 128 ? 2 : 3; }  // that fit an SM, by their registers
 constexpr float kNegInf = -INFINITY;
 
 ICSA_DEV int valid_tokens(const Kv8Cache& c, int b) {
@@ -344,7 +345,7 @@ ICSA_DEV float scale_log2(float s) { return s != s ? s : float(int(__float_as_ui
 // Rows of the 8-query tile blockIdx.z of (b, cache head): row r is query
 // token r / group, head h * group + r % group.
 template <int D>
-__global__ void __launch_bounds__(kDWarps * 32) kv8_decode_kernel(const Kv8AttnParams p, const Kv8Cache c) {
+__global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kernel(const Kv8AttnParams p, const Kv8Cache c) {
   constexpr int kHalves = D / 64;            // 64-byte halves of a key row
   constexpr int kSteps = D / 16;             // 16-feature steps of S
   constexpr int kOTiles = D / 16;            // 16-feature tiles of O^T
@@ -591,12 +592,25 @@ cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out
   return out_dtype == ICSA_BF16 ? dequantize_as<__nv_bfloat16>(c, out, stream) : dequantize_as<float>(c, out, stream);
 }
 
-int kv8_decode_splits(int B, int H, int rows, int L, int num_sms) {
-  const int64_t ctas = int64_t(B) * H * ((rows + 7) / 8);
+int kv8_decode_splits(int B, int H, int rows, int L, int D, int num_sms) {
+  const int64_t ctas = int64_t(B) * H * ((rows + 7) / 8), slots = int64_t(num_sms) * decode_ctas(D);
   const int64_t nb = (L + kTokens - 1) / kTokens;
-  // two CTAs per SM; a split keeps at least one block for each warp
-  const int64_t want = 2 * int64_t(num_sms) / std::max<int64_t>(ctas, 1);
-  return int(std::max<int64_t>(1, std::min<int64_t>(want, nb / kDWarps)));
+  // Waves of CTAs times the steps of a warp, two steps' time for a CTA's start
+  // and its part of the join; a split keeps at least one block for each warp.
+  // 2 x 40 heads x 32760 tokens, D = 128, 16 query rows: one split (160 CTAs
+  // on 296 places) 284 us, seven 232 us; D = 64, one row: three (two to an
+  // SM) 83 us, eleven 69 us.
+  const int64_t most = std::min<int64_t>(nb / kDWarps, 32);
+  int64_t best = 1;
+  double best_cost = 0;
+  for (int64_t s = 1; s <= std::max<int64_t>(most, 1); ++s) {
+    const double cost = double((ctas * s + slots - 1) / slots) * (double(nb) / double(s * kDWarps) + 2.0);
+    if (s == 1 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return int(best);
 }
 
 cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream) {

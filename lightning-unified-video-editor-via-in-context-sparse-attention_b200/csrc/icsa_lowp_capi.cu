@@ -216,7 +216,7 @@ AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   const int64_t rows = int64_t(Lq) * (Hq / c.H);
   if (rows <= kDecodeRows) {
     a.path = kDecode;
-    a.splits = icsa::kv8_decode_splits(c.B, c.H, int(rows), c.L, sms);
+    a.splits = icsa::kv8_decode_splits(c.B, c.H, int(rows), c.L, c.D, sms);
     a.bytes = a.splits == 1 ? 0 : align256(size_t(c.B) * c.H * rows * a.splits * (c.D + 2) * sizeof(float));
     return a;
   }
