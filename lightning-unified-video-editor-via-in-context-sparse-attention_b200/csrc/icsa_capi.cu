@@ -718,7 +718,7 @@ int icsa_dit_linear_residual(const void* a, int64_t lda, const void* w, int64_t 
 }
 
 int icsa_last_status(cudaStream_t stream, int clear) {
-  constexpr int kUnits = 8;
+  constexpr int kUnits = 9;
   static std::mutex mu;
   static int* addr[kMaxDevices][kUnits] = {};
   cudaError_t e = cudaStreamSynchronize(stream);
@@ -731,7 +731,8 @@ int icsa_last_status(cudaStream_t stream, int clear) {
     cudaError_t (*const get[kUnits])(int**) = {icsa::sticky_status_dense_pair, icsa::sticky_status_flat,
                                                icsa::sticky_status_sparse, icsa::sticky_status_selftest,
                                                icsa::sticky_status_gemm, icsa::sticky_status_scores,
-                                               icsa::sticky_status_fp4, icsa::sticky_status_kv8_tc};
+                                               icsa::sticky_status_fp4, icsa::sticky_status_kv8_tc,
+                                               icsa::sticky_status_fp4_rows};
     int* a[kUnits] = {};
     for (int i = 0; i < kUnits; ++i)
       if ((e = get[i](&a[i])) != cudaSuccess) return cuda_fail(e, "sticky status address");

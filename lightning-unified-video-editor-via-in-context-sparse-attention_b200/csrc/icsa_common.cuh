@@ -202,6 +202,14 @@ ICSA_DEV bool mbar_spin_wait(uint64_t* bar, uint32_t parity, int* err, int code,
 // ---------------------------------------------------------------------------
 // TMA (tensor) loads.  Single-CTA form only: each load lands in the issuing CTA.
 // ---------------------------------------------------------------------------
+ICSA_DEV void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
 ICSA_DEV void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"

@@ -153,6 +153,7 @@ cudaError_t sticky_status_selftest(int** out);
 cudaError_t sticky_status_gemm(int** out);
 cudaError_t sticky_status_scores(int** out);
 cudaError_t sticky_status_fp4(int** out);
+cudaError_t sticky_status_fp4_rows(int** out);
 cudaError_t sticky_status_kv8_tc(int** out);
 
 }  // namespace icsa

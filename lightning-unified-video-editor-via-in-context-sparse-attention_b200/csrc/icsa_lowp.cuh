@@ -73,6 +73,20 @@ int fp4_gemm_splits(int M, int N, int K, int num_sms);
 cudaError_t launch_fp4_gemm(Fp4GemmParams p, const Fp4GemmMaps& maps, int format, int num_sms, cudaStream_t stream);
 cudaError_t sticky_status_fp4(int** out);
 
+// At most kFp4MaxRows rows: see icsa_fp4_rows.cu.  maps.a has boxes of
+// fp4_rows_box(M) rows; partial: plan.bytes of workspace.
+constexpr int kFp4MaxRows = 64;
+struct Fp4RowsPlan {
+  int ctas;
+  bool join;     // tiles are cut between CTAs
+  size_t bytes;
+};
+Fp4RowsPlan fp4_rows_plan(int M, int N, int K, int num_sms);
+int fp4_rows_box(int M);
+cudaError_t launch_fp4_rows(Fp4GemmParams p, const Fp4GemmMaps& maps, int format, const Fp4RowsPlan& plan,
+                            cudaStream_t stream);
+cudaError_t sticky_status_fp4_rows(int** out);
+
 // ------------------------------------------------------------- 8-bit cache --
 struct Kv8Cache {
   uint8_t* k;      // e4m3 [B, H, nb, 64, D]

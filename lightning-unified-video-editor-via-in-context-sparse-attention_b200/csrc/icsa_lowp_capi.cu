@@ -67,10 +67,10 @@ int check_fp4_buffers(const char* who, const void* data, const void* scales) {
 }
 
 int encode_fp4_maps(CUtensorMap* data_map, CUtensorMap* scale_map, const void* data, const void* scales, int format,
-                    int rows, int K) {
+                    int rows, int K, int box_rows) {
   const uint64_t row_bytes = uint64_t(icsa::fp4_row_bytes(K));
   int rc = icsa::encode_tensor_map_2d(data_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, data, row_bytes, uint64_t(rows),
-                                      row_bytes, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+                                      row_bytes, 128, uint32_t(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != ICSA_OK) return rc;
   const uint64_t atoms = uint64_t(icsa::fp4_scale_bytes(format, rows, K)) / icsa::kScaleAtomBytes;
   return icsa::encode_tensor_map_2d(scale_map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, 128, atoms,
@@ -80,9 +80,31 @@ int encode_fp4_maps(CUtensorMap* data_map, CUtensorMap* scale_map, const void* d
 
 int fp4_n_pad(int N) { return (N + 255) / 256 * 256; }
 
+// How an M x N x K product runs, and its workspace.
+struct LinearPlan {
+  bool rows;              // launch_fp4_rows, else launch_fp4_gemm
+  icsa::Fp4RowsPlan few;
+  int splits;
+  size_t bytes;
+};
+LinearPlan plan_linear(int M, int N, int K, int sms) {
+  LinearPlan l = {};
+  l.rows = M <= icsa::kFp4MaxRows;
+  l.splits = 1;
+  if (l.rows) {
+    l.few = icsa::fp4_rows_plan(M, N, K, sms);
+    l.bytes = align256(l.few.bytes);
+  } else {
+    l.splits = icsa::fp4_gemm_splits(M, N, K, sms);
+    l.bytes = l.splits == 1 ? 0 : align256(size_t(l.splits) * M * fp4_n_pad(N) * sizeof(float));
+  }
+  return l;
+}
+
 struct Fp4Call {
   icsa::Fp4GemmMaps maps;
   icsa::Fp4GemmParams p;
+  LinearPlan plan;
   int sms;
 };
 
@@ -118,19 +140,21 @@ int prepare_linear(Fp4Call* call, int format, const void* a_data, const void* a_
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ldo = ldo;
   p.tma_out = aligned(out, 16) && ldo % 8 == 0;
-  p.splits = icsa::fp4_gemm_splits(M, N, K, sms);
+  const LinearPlan& plan = call->plan = plan_linear(M, N, K, sms);
+  p.splits = plan.splits;
   p.n_pad = fp4_n_pad(N);
-  if (p.splits > 1) {
-    const size_t need = align256(size_t(p.splits) * M * p.n_pad * sizeof(float));
+  if (plan.bytes > 0) {
+    const size_t need = plan.bytes;
     if (workspace == nullptr || workspace_bytes < need)
       return fail(ICSA_ERR_WORKSPACE, "fp4_linear: workspace of %zu bytes is smaller than the %zu bytes required",
                   workspace == nullptr ? size_t(0) : workspace_bytes, need);
     if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "fp4_linear: the workspace must be 256-byte aligned");
     p.partial = static_cast<float*>(workspace);
   }
-  if ((rc = encode_fp4_maps(&maps.a, &maps.sa, a_data, a_scales, format, M, K)) != ICSA_OK) return rc;
-  if ((rc = encode_fp4_maps(&maps.w, &maps.sw, w_data, w_scales, format, N, K)) != ICSA_OK) return rc;
-  if (p.tma_out && (rc = icsa::encode_tensor_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, uint64_t(N),
+  if ((rc = encode_fp4_maps(&maps.a, &maps.sa, a_data, a_scales, format, M, K,
+                            plan.rows ? icsa::fp4_rows_box(M) : 128)) != ICSA_OK) return rc;
+  if ((rc = encode_fp4_maps(&maps.w, &maps.sw, w_data, w_scales, format, N, K, 128)) != ICSA_OK) return rc;
+  if (p.tma_out && !plan.rows && (rc = icsa::encode_tensor_map_2d(&maps.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, uint64_t(N),
                                                     uint64_t(M), uint64_t(ldo) * 2, 64, 32,
                                                     CU_TENSOR_MAP_SWIZZLE_128B)) != ICSA_OK)
     return rc;
@@ -139,7 +163,9 @@ int prepare_linear(Fp4Call* call, int format, const void* a_data, const void* a_
 
 int launch_linear(const Fp4Call& call, int format, cudaStream_t stream) {
   if (call.p.M == 0) return ICSA_OK;
-  cudaError_t e = icsa::launch_fp4_gemm(call.p, call.maps, format, call.sms, stream);
+  const cudaError_t e = call.plan.rows
+                            ? icsa::launch_fp4_rows(call.p, call.maps, format, call.plan.few, stream)
+                            : icsa::launch_fp4_gemm(call.p, call.maps, format, call.sms, stream);
   return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_linear");
 }
 
@@ -324,8 +350,7 @@ int icsa_fp4_dequantize(const void* data, const void* scales, int rows, int K, i
 size_t icsa_fp4_linear_workspace_size(int M, int N, int K) {
   int sms = 0;
   if (M < 1 || N < 1 || K < 1 || !sm_count(&sms)) return 0;
-  const int splits = icsa::fp4_gemm_splits(M, N, K, sms);
-  return splits == 1 ? 0 : align256(size_t(splits) * M * fp4_n_pad(N) * sizeof(float));
+  return plan_linear(M, N, K, sms).bytes;
 }
 
 int icsa_fp4_linear(int format, const void* a_data, const void* a_scales, float a_global_scale, const void* w_data,

@@ -145,6 +145,16 @@ def test_linear_layer(fmt, M, N, K, bias, act):
     assert bool((d <= tol).all()), float((d / tol).max())
 
 
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("M,N,K,bias,act", [
+    (1, 30001, 1030, True, None), (1, 128, 65536, False, None), (16, 19001, 520, True, "gelu_tanh"),
+    (17, 129, 8192, True, None), (32, 3000, 256, False, None), (33, 40000, 300, True, None),
+    (64, 2560, 5120, True, "gelu_tanh"), (65, 2560, 5120, True, "gelu_tanh")])
+def test_linear_layer_of_few_rows(fmt, M, N, K, bias, act):
+    """Tiles cut between CTAs at every kind of boundary: many tiles, one tile, whole tiles."""
+    test_linear_layer(fmt, M, N, K, bias, act)
+
+
 def test_linear_layer_of_a_quantised_input_and_of_float32_rows():
     x, w, b, want, tol = linear_case(70, 300, 900, "nvfp4", True, None, g_x=2.0 ** -3)
     t = lowp.fp4_quantize(x, "nvfp4", 2.0 ** -3)
@@ -183,13 +193,13 @@ def test_linear_layer_refuses_mixed_formats_and_devices():
     assert lowp.fp4_linear(x[:0], w, b).shape == (0, 32)
 
 
-@pytest.mark.parametrize("M,K", [(3, 2048), (9, 4096)])
+@pytest.mark.parametrize("M,K", [(3, 2048), (70, 4096)])
 def test_linear_layer_checks_its_workspace_and_leaves_what_is_behind_its_rows(M, K):
     lib = lowp._load()
     x, w, b, want, tol = linear_case(M, 40, K, "nvfp4", True, None)
     a = lowp.fp4_quantize(x, "nvfp4")
     size = lib.icsa_fp4_linear_workspace_size(M, 40, K)
-    assert (size > 0) == (M > 4)                                 # few tiles of several rows: K is split
+    assert size > 0                                              # few tiles: K is split
     out = torch.full((M + 2, 48), 7.0, dtype=torch.bfloat16, device="cuda")
     ws = torch.full((size + 256,), 0xFF, dtype=torch.uint8, device="cuda")
 
@@ -197,8 +207,7 @@ def test_linear_layer_checks_its_workspace_and_leaves_what_is_behind_its_rows(M,
         return lib.icsa_fp4_linear(0, a.data.data_ptr(), a.scales.data_ptr(), 1.0, w.data.data_ptr(),
                                    w.scales.data_ptr(), w.global_scale, b.data_ptr(), 0, out.data_ptr(), 48, M, 40,
                                    K, ws_ptr, nbytes, torch.cuda.current_stream().cuda_stream)
-    if size:
-        assert call(None, size) == 4 and call(ws.data_ptr(), size - 1) == 4 and call(ws.data_ptr() + 16, size) == 1
+    assert call(None, size) == 4 and call(ws.data_ptr(), size - 1) == 4 and call(ws.data_ptr() + 16, size) == 1
     assert call(ws.data_ptr(), size) == 0
     assert bool(((out[:M, :40].double() - want).abs() <= tol).all())
     assert bool((out[M:] == 7).all()) and bool((out[:, 40:] == 7).all()) and bool((ws[size:] == 0xFF).all())
