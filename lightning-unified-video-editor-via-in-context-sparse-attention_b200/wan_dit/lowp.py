@@ -102,11 +102,15 @@ def _on(index, fn, *args):
         return fn(lib, torch._C._cuda_getCurrentRawStream(index), *args)
 
 
+# outputs are allocated with their strides given, the cheapest call
+_empty = torch.empty_strided
+
+
 def _bytes(like, n):
     """n bytes of workspace on the device of `like` (None for 0) and their address."""
     if not n:
         return None, None
-    ws = like.new_empty(n, dtype=torch.uint8)
+    ws = _empty((n,), (1,), dtype=torch.uint8, device=like.device)
     return ws, ws.data_ptr()
 
 
@@ -195,8 +199,10 @@ def fp4_quantize(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0)
 
 def _quantize(lib, stream, x, ld, fmt, g):
     rows, K = x.shape
-    data, scales = fp4_storage(rows, K, fmt)
-    data, scales = x.new_empty(data, dtype=torch.uint8), x.new_empty(scales, dtype=torch.uint8)
+    (_, row), scales = fp4_storage(rows, K, fmt)
+    device = x.device
+    data = _empty((rows, row), (row, 1), dtype=torch.uint8, device=device)
+    scales = _empty(scales, (scales[1] * 512, 512, 16, 4, 1), dtype=torch.uint8, device=device)
     code = lib.icsa_fp4_quantize(x.data_ptr(), _DT[x.dtype], ld, rows, K, FP4_FORMATS[fmt], g, data.data_ptr(),
                                  scales.data_ptr(), stream)
     if code:
@@ -215,7 +221,7 @@ def fp4_dequantize(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
 
 def _dequantize(lib, stream, t, dtype):
     rows, K = t.shape
-    out = t.data.new_empty((rows, K), dtype=dtype)
+    out = _empty((rows, K), (K, 1), dtype=dtype, device=t.data.device)
     code = lib.icsa_fp4_dequantize(t.data.data_ptr(), t.scales.data_ptr(), rows, K, FP4_FORMATS[t.fmt],
                                    t.global_scale, out.data_ptr(), _DT[dtype], K, stream)
     if code:
@@ -261,7 +267,7 @@ def _linear_workspace(index, fmt, M, N, K):
 
 def _linear(lib, stream, a, w, bias, activation):
     (M, K), N = a.shape, w.shape[0]
-    out = a.data.new_empty((M, N), dtype=torch.bfloat16)
+    out = _empty((M, N), (N, 1), dtype=torch.bfloat16, device=a.data.device)
     size = _linear_workspace(a.data.get_device(), None, M, N, K)
     ws, ptr = _bytes(out, size)
     code = lib.icsa_fp4_linear(FP4_FORMATS[w.fmt], a.data.data_ptr(), a.scales.data_ptr(), a.global_scale,
@@ -275,7 +281,7 @@ def _linear(lib, stream, a, w, bias, activation):
 
 def _linear_rows(lib, stream, x, ld, w, bias, activation):
     (M, K), N = x.shape, w.shape[0]
-    out = x.new_empty((M, N), dtype=torch.bfloat16)
+    out = _empty((M, N), (N, 1), dtype=torch.bfloat16, device=x.device)
     size = _linear_workspace(x.get_device(), w.fmt, M, N, K)
     ws, ptr = _bytes(out, size)
     code = lib.icsa_fp4_linear_rows(FP4_FORMATS[w.fmt], x.data_ptr(), _DT[x.dtype], ld, w.data.data_ptr(),
@@ -345,7 +351,8 @@ def _int64x3(a, b, c):
 
 def _strides(t):
     """Batch, token and head strides; 0 for an axis of one."""
-    return _int64x3(*(st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride())))
+    (B, L, H, _), (sb, st, sh, _) = t.shape, t.stride()
+    return _int64x3(sb if B > 1 else 0, st if L > 1 else 0, sh if H > 1 else 0)
 
 
 def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> Kv8Cache:
@@ -362,18 +369,23 @@ def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tenso
     if min(B, L, H) < 1:
         raise ValueError(f"kv8_quantize: empty k, v {tuple(k.shape)}")
     _check_lengths("kv8_quantize", lengths, B)
-    k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (k, v))
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if v.stride(3) != 1:
+        v = v.contiguous()
     return _on(index, _quantize_kv, k, v, lengths)
 
 
 def _quantize_kv(lib, stream, k, v, lengths):
     B, L, H, D = k.shape
     nb = -(-L // KV8_TOKENS)
+    device, T, n = k.device, KV8_TOKENS, nb * KV8_TOKENS * D
     c = object.__new__(Kv8Cache)        # its tensors are as the constructor wants them
-    c.__dict__.update(k=k.new_empty((B, H, nb, KV8_TOKENS, D), dtype=torch.float8_e4m3fn),
-                      v=k.new_empty((B, H, nb, D, KV8_TOKENS), dtype=torch.float8_e4m3fn),
-                      k_scale=k.new_empty((B, H, nb), dtype=torch.float32),
-                      v_scale=k.new_empty((B, H, nb), dtype=torch.float32), L=L, lengths=lengths)
+    c.__dict__.update(
+        k=_empty((B, H, nb, T, D), (H * n, n, T * D, D, 1), dtype=torch.float8_e4m3fn, device=device),
+        v=_empty((B, H, nb, D, T), (H * n, n, T * D, T, 1), dtype=torch.float8_e4m3fn, device=device),
+        k_scale=_empty((B, H, nb), (H * nb, nb, 1), dtype=torch.float32, device=device),
+        v_scale=_empty((B, H, nb), (H * nb, nb, 1), dtype=torch.float32, device=device), L=L, lengths=lengths)
     code = lib.icsa_kv8_quantize(ctypes.byref(c._desc()), k.data_ptr(), v.data_ptr(), _DT[k.dtype], _strides(k),
                                  _strides(v), stream)
     if code:
@@ -389,8 +401,10 @@ def kv8_dequantize(cache: Kv8Cache, dtype: torch.dtype = torch.bfloat16):
 
 
 def _dequantize_kv(lib, stream, cache, dtype):
-    B, H, _, _, D = cache.k.shape
-    k, v = (cache.k.new_empty((B, cache.L, H, D), dtype=dtype) for _ in range(2))
+    (B, H, _, _, D), L, device = cache.k.shape, cache.L, cache.k.device
+    shape, strides = (B, L, H, D), (L * H * D, H * D, D, 1)
+    k = _empty(shape, strides, dtype=dtype, device=device)
+    v = _empty(shape, strides, dtype=dtype, device=device)
     code = lib.icsa_kv8_dequantize(ctypes.byref(cache._desc()), k.data_ptr(), v.data_ptr(), _DT[dtype], stream)
     if code:
         _capi.check(code, "icsa_kv8_dequantize")
@@ -417,7 +431,7 @@ def _attention_workspace(index, B, H, L, D, Lq, Hq):
 def _attention(lib, stream, q, cache):
     B, Lq, Hq, D = q.shape
     H = cache.k.shape[1]
-    out = q.new_empty((B, Lq, Hq, D))
+    out = _empty((B, Lq, Hq, D), (Lq * Hq * D, Hq * D, D, 1), dtype=torch.bfloat16, device=q.device)
     if Lq == 0:
         return out
     sb, st, sh, sd = q.stride()
