@@ -111,7 +111,7 @@ ICSA_DEV int cache_length(const Kv8Cache& c, int b) {
 ICSA_DEV int steps_of(int len) { return (len + kStepKeys - 1) / kStepKeys; }
 
 // Work space: the rounds of batch element 0, 1, .. one behind the other, heads
-// outermost, a step of a round of two tiles weighing 12 and of one tile 5
+// outermost, a step of a round of two tiles weighing 12 and of one tile 10
 // (measured: 2.6 us for the two tiles of a step, 2.2 us for one, which the
 // filling of its stage bounds).  A round without keys, and in whole
 // rounds its epilogue, count as a step.
