@@ -937,7 +937,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   pair::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
-  wait_prior_grid();
   // Register split: 512 threads launch with 128 registers each;
   // 256 x 176 + 128 x 104 + 128 x 56 = 512 x 128.
   if (warp < 8) {

@@ -349,7 +349,7 @@ int icsa_fp4_dequantize(const void* data, const void* scales, int rows, int K, i
 
 size_t icsa_fp4_linear_workspace_size(int M, int N, int K) {
   int sms = 0;
-  if (M < 1 || N < 1 || K < 1 || !sm_count(&sms)) return 0;
+  if (M < 1 || N < 1 || K < 1 || M > kMaxRows || N > kMaxRows || K > kMaxK || !sm_count(&sms)) return 0;
   return plan_linear(M, N, K, sms).bytes;
 }
 

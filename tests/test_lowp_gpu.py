@@ -296,7 +296,12 @@ def check_attention(q, cache, lengths=None, k=None, v=None):
     (2, 8, 200, 2, 1, [131, 200]), (4, 9, 331, 4, 4, [331, 280, 10, 0]), (1, 3, 4000, 1, 3, None),
     (2, 1, 9000, 2, 1, [8000, 77]), (1, 32, 500, 1, 1, None),
     (1, 33, 100, 2, 1, None), (2, 16, 70, 1, 4, [0, 70]), (3, 77, 331, 2, 2, [331, 0, 130]), (1, 64, 64, 3, 1, None),
-    (2, 65, 1, 1, 2, None), (2, 300, 1000, 2, 1, [1000, 63]), (1, 257, 128, 2, 1, [127])])
+    (2, 65, 1, 1, 2, None), (2, 300, 1000, 2, 1, [1000, 63]), (1, 257, 128, 2, 1, [127]),
+    # bf16 copies with shared heads and an empty sequence; rounds cut between clusters, groups that
+    # no box of queries holds; more sequences than a launch takes; many splits
+    (3, 700, 900, 2, 3, [0, 900, 65]), (1, 60, 9000, 2, 1, [8777]), (2, 20, 5000, 3, 5, [4999, 129]),
+    (1, 130, 6000, 1, 3, None), (130, 49, 70, 1, 1, list(range(-30, 100))), (129, 51, 1100, 1, 1, None),
+    (1, 1, 32000, 1, 2, None)])
 def test_attention_over_the_cache(D, B, Lq, Lk, H, group, lengths):
     k, v = kv_rows(B, Lk, H, D, torch.bfloat16)
     q = torch.randn(B, Lq, H * group, D, generator=torch.Generator().manual_seed(Lq + Lk)).to(torch.bfloat16)
@@ -304,7 +309,7 @@ def test_attention_over_the_cache(D, B, Lq, Lk, H, group, lengths):
     cache = lowp.kv8_quantize(k.cuda(), v.cuda(), n)
     got = check_attention(q, cache, lengths)
     for b, m in enumerate(lengths or []):
-        if m == 0:
+        if m <= 0:
             assert not bool(got[b].any())
 
 
@@ -474,6 +479,41 @@ def test_a_run_of_the_operators_is_captured_replayed_and_repeatable():
             assert all(torch.equal(a, b) for a, b in zip(out, want[s]))
 
 
+def test_second_kernels_in_two_graphs_and_on_two_streams():
+    """Products split along K, tiles and rounds cut between CTAs: every call launches a kernel that
+    joins partial results from its workspace."""
+    g = torch.Generator().manual_seed(4)
+    w = lowp.fp4_quantize((torch.randn(300, 4096, generator=g) / 64).cuda(), "nvfp4", 2.0 ** -9)
+    k, v = kv_rows(1, 9000, 2, 128, torch.bfloat16)
+    cache = lowp.kv8_quantize(k.cuda(), v.cuda())
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return [torch.randn(n, 4096, generator=g).to(torch.bfloat16).cuda() for n in (9, 70)] + [
+            torch.randn(1, n, 2, 128, generator=g).to(torch.bfloat16).cuda() for n in (1, 60)]
+
+    def run(x9, x70, q1, q60):
+        return lowp.fp4_linear(x9, w), lowp.fp4_linear(x70, w), lowp.kv8_attention(q1, cache), lowp.kv8_attention(q60, cache)
+    want = [run(*inputs(s)) for s in (0, 1, 2)]
+    static = inputs(0)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for gr in graphs:
+        with torch.cuda.graph(gr):
+            outs.append(run(*static))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in (1, 2):
+        for dst, src in zip(static, inputs(s)):
+            dst.copy_(src)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for gr, st in zip(graphs, streams):                  # both at once
+                with torch.cuda.stream(st):
+                    gr.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[s]))
+
+
 def test_calls_on_two_streams_at_once():
     w1, b1, w2 = together_weights()
     inputs = [together_inputs(s, 200) for s in range(2)]
@@ -501,6 +541,52 @@ def test_tensors_on_another_device_than_the_current_one():
     move = lambda t: lowp.Fp4Tensor(t.data.to(dev), t.scales.to(dev), t.shape, t.fmt, t.global_scale)  # noqa: E731
     got = together(x, move(w1), b1.to(dev), move(w2), k, v, n, q)
     assert all(g.device == dev and torch.equal(g.cpu(), w.cpu()) for g, w in zip(got, want))
+
+
+# --------------------------------------------------------------------------- large tensors
+def test_offsets_beyond_32_bits_in_4_bit_tensors():
+    rows, K = 262144 + 3, 16400                                  # 4.3e9 elements
+    x = torch.empty(rows, K, dtype=torch.bfloat16, device="cuda")
+    x[:-200] = 1.0
+    x[-200:] = torch.randn(200, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    t = lowp.fp4_quantize(x, "nvfp4")
+    n = rows - 128 * 2023                                        # enough rows for the same order of sums
+    tail = lowp.fp4_quantize(x[-n:], "nvfp4")
+    assert torch.equal(t.data[-n:], tail.data) and torch.equal(t.scales[2023:], tail.scales)
+    del x
+    out = lowp.fp4_dequantize(t)
+    # a block of ones: scale e4m3(1 / 6) = 11 / 64, code e2m1(64 / 11) = 6
+    assert torch.equal(out[-n:], lowp.fp4_dequantize(tail)) and bool((out[:300] == 66 / 64).all())
+    del out
+    w = lowp.fp4_quantize(torch.randn(8208, K, generator=torch.Generator().manual_seed(2)).cuda(), "nvfp4", 2.0 ** -7)
+    y = lowp.fp4_linear(t, w)                                    # 2.15e9 outputs
+    assert torch.equal(y[-n:], lowp.fp4_linear(tail, w)) and torch.equal(y[7], y[100000])
+
+
+@pytest.mark.parametrize("Lq", [1, 64])
+def test_offsets_beyond_32_bits_in_the_cache(Lq):
+    L, D = (1 << 25) + 70, 128                                   # 4.3e9 elements
+    k = torch.zeros(1, L, 1, D, dtype=torch.bfloat16, device="cuda")
+    last = torch.randn(70, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    k[0, -70:, 0] = last * 64
+    cache = lowp.kv8_quantize(k, k)
+    del k
+    tail = lowp.kv8_quantize(last.view(1, 70, 1, D) * 64, last.view(1, 70, 1, D) * 64)
+    for a, b in ((cache.k, tail.k), (cache.v, tail.v)):
+        assert torch.equal(a[0, 0, -2:].view(torch.uint8), b[0, 0].view(torch.uint8))
+    assert torch.equal(cache.k_scale[0, 0, -2:], tail.k_scale[0, 0]) and bool((cache.v_scale[0, 0, :-2] == 1).all())
+    # only the last 70 keys and values are not zero: every key before them has score 0
+    q = (torch.randn(1, Lq, 1, D, generator=torch.Generator().manual_seed(2)) / 16).to(torch.bfloat16).cuda()
+    got = lowp.kv8_attention(q, cache)[0, :, 0].double()
+    kd, vd = (x[0, :, 0].double() for x in lowp.kv8_dequantize(tail, torch.float32))
+    s = q[0, :, 0].double() @ kd.T / math.sqrt(D)
+    top = s.amax(1, keepdim=True).clamp_min(0)
+    p = torch.exp(s - top)
+    total = p.sum(1, keepdim=True) + (L - 70) * torch.exp(-top)
+    want, mass = p @ vd / total, p @ vd.abs() / total
+    # a row sum of up to 4096 steps one behind the other, each rounded by 2^-24
+    tol = want.abs() * 2.0 ** -8 + mass * (2.0 ** -11 + (float(s.abs().max()) + 1) * 2.0 ** -20 + 2.0 ** -12)
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
 
 
 # --------------------------------------------------------------------------- in the model
