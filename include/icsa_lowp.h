@@ -125,10 +125,13 @@ ICSA_API int icsa_kv8_dequantize(const icsa_kv8_cache* cache, void* k_out, void*
  * h' = h / (Hq / H), len = lengths[b]; zero where len is 0.  Replaces the
  * reference's flash_attention call (wanx/attention.py:18-85, with its k_lens)
  * for keys and values that are kept over many calls.  float32 scores, softmax
- * and accumulation; the probabilities enter the second product as 16-bit
- * floats; one rounding of the result.
+ * and accumulation; the probabilities enter the second product as fp16, and
+ * as bf16 for many queries over a long cache; one rounding of the result.
  *   q: bf16 [B, Lq, Hq, D] with batch, token, head strides (multiples of 8
- *   elements, 16-byte aligned), contiguous features; Hq a multiple of H
+ *   elements, 16-byte aligned), contiguous features; Hq a multiple of H.
+ *   (ICSA_ERR_UNSUPPORTED for many queries over a long cache whose heads are
+ *   not contiguous, or whose tokens or batch elements overlap or have gaps
+ *   between batch elements: that path reads q as rows.)
  *   out: bf16 [B, Lq, Hq, D], contiguous
  *   workspace: icsa_kv8_attention_workspace_size() bytes, 256-byte aligned;
  *   its contents do not matter before the call and mean nothing after it

@@ -1,6 +1,7 @@
 // Parameter blocks and launchers of the low-precision operators: microscaled
-// 4-bit quantisation and linear layers (icsa_fp4.cu, icsa_fp4_gemm.cu) and
-// the 8-bit key/value cache with the attention that reads it (icsa_kv8.cu).
+// 4-bit quantisation and linear layers (icsa_fp4.cu, icsa_fp4_gemm.cu,
+// icsa_fp4_rows.cu) and the 8-bit key/value cache with the attention that
+// reads it (icsa_kv8.cu, icsa_kv8_tc.cu).
 #pragma once
 
 #include "icsa_kernels.cuh"
@@ -35,7 +36,7 @@ struct Fp4QuantParams {
   float global_scale;
   uint8_t* data;
   uint8_t* scales;
-  float inv_hi, inv_lo;  // 1 / (6 global_scale) as a sum of two floats (0: out of their range); set by the launcher
+  float inv_hi, inv_lo;  // 1 / (6 global_scale) as a sum of two floats (0: divide instead); set by the launcher
 };
 cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, int x_dtype, int format, cudaStream_t stream);
 

@@ -389,6 +389,22 @@ def test_attention_takes_strided_queries(Lq):
     assert lowp.kv8_attention(wide[:0, :H * D].view(0, 1, H, D).new_zeros(B, 0, H, D), cache).shape == (B, 0, H, D)
 
 
+def test_strided_heads_over_a_long_cache_are_copied_by_python_and_refused_by_c():
+    import ctypes
+    k, v = kv_rows(1, 5000, 2, 128, torch.bfloat16)
+    cache = lowp.kv8_quantize(k.cuda(), v.cuda())
+    q = torch.randn(1, 2, 4000, 128, device="cuda").to(torch.bfloat16).transpose(1, 2)
+    want = lowp.kv8_attention(q.contiguous(), cache)
+    assert torch.equal(lowp.kv8_attention(q, cache), want)
+    lib, desc = lowp._load(), cache._desc()
+    size = lib.icsa_kv8_attention_workspace_size(ctypes.byref(desc), 4000, 2)
+    ws, out = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.zeros_like(want)
+    assert lib.icsa_kv8_attention(ctypes.byref(desc), q.data_ptr(), (ctypes.c_int64 * 3)(0, 128, 4000 * 128),
+                                  out.data_ptr(), 4000, 2, ws.data_ptr(), size,
+                                  torch.cuda.current_stream().cuda_stream) == 2
+    assert not bool(out.any())
+
+
 def test_attention_refuses_other_shapes_and_devices():
     k, v = kv_rows(2, 64, 2, 64, torch.bfloat16)
     cache = lowp.kv8_quantize(k.cuda(), v.cuda())
