@@ -27,6 +27,9 @@ constexpr int kTileRows = 128;      // Q rows per attention tile (two 64-token b
 // is visible).  Kernels launched without the attribute pass the wait at once.
 // ---------------------------------------------------------------------------
 ICSA_DEV void wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets a chained kernel behind this one start once every CTA has got here (it
+// still waits for this grid's end before it reads what it wrote).
+ICSA_DEV void release_next_grid() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... Params, typename... Args>
 inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,

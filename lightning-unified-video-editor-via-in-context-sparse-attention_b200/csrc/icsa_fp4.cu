@@ -257,6 +257,7 @@ ICSA_DEV uint32_t top_bits(const float (&v)[16]) {
 template <typename T, int FMT, int ALIGN>
 __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantParams p, int chunks_per_cta) {
   constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
+  release_next_grid();  // a linear layer sets itself up meanwhile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = tile_row(blockIdx.x, warp);
   const int k_tiles = (p.K + kFp4TileK - 1) / kFp4TileK;

@@ -167,7 +167,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
+  const auto load_w = [&](int s, int tile, int kb) {
+    mbar_arrive_expect_tx(&sm.full[s], kBytes);
+    tma_load_2d(sm.w[s], &maps.w, &sm.full[s], kb * 128, tile * kTileN);
+    tma_load_2d(sm.sw[s], &maps.sw, &sm.full[s], 0, (tile * p.k_steps + kb) * kAtoms);
+  };
+  // the weight's first stages while the kernel before quantises a
+  int early = 0;
+  if (p.w_ready && warp == kProducerWarp && lane == 0)
+    for (; early < kStages && x0 + early < x1; ++early)
+      load_w(early, int((x0 + early) / p.k_steps), int((x0 + early) % p.k_steps));
   wait_prior_grid();  // the operands are the previous kernels' outputs
+  release_next_grid();
   if (warp < 4) {
     int count = 0;
     for (int64_t x = x0; x < x1; ++count) {
@@ -212,11 +223,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         x += g.k1 - g.k0;
         for (int kb = g.k0; kb < g.k1; ++kb, ++it) {
           const int s = it % kStages;
-          ok = mbar_wait(&sm.empty[s], (uint32_t(it / kStages) & 1u) ^ 1u, nullptr, kErrEmpty, abort_flag);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&sm.full[s], kBytes);
-          tma_load_2d(sm.w[s], &maps.w, &sm.full[s], kb * 128, g.tile * kTileN);
-          tma_load_2d(sm.sw[s], &maps.sw, &sm.full[s], 0, (g.tile * p.k_steps + kb) * kAtoms);
+          if (it >= early) {
+            ok = mbar_wait(&sm.empty[s], (uint32_t(it / kStages) & 1u) ^ 1u, nullptr, kErrEmpty, abort_flag);
+            if (!ok) break;
+            load_w(s, g.tile, kb);
+          }
           tma_load_2d(sm.a[s], &maps.a, &sm.full[s], kb * 128, 0);
           tma_load_2d(sm.sa[s], &maps.sa, &sm.full[s], 0, kb * kAtoms);
         }

@@ -68,6 +68,7 @@ struct Fp4GemmParams {
   int splits;
   int m_tiles, n_tiles, units, k_steps;
   int tma_out;                 // the output's rows are 16-byte aligned: written by TMA
+  int w_ready;                 // the kernel before this one in the stream did not write w
 };
 // Splits of K for an M x N x K product on `num_sms` SMs (1: none).
 int fp4_gemm_splits(int M, int N, int K, int num_sms);

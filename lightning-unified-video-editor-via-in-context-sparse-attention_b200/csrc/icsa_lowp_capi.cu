@@ -389,6 +389,7 @@ int icsa_fp4_linear_rows(int format, const void* x, int x_dtype, int64_t ldx, co
                            M > 0 ? workspace_bytes - data - scales : 0)) != ICSA_OK)
     return rc;
   if ((rc = icsa_fp4_quantize(x, x_dtype, ldx, M, K, format, 1.f, ws, ws + data, stream)) != ICSA_OK) return rc;
+  call.p.w_ready = 1;  // that kernel is an ordinary launch, behind whatever wrote the weight
   return launch_linear(call, format, stream);
 }
 
