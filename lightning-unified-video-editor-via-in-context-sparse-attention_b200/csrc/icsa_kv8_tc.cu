@@ -159,6 +159,20 @@ ICSA_DEV Point locate(const Kv8TcParams& p, const Kv8Cache& c, const Extent& e, 
 
 // (Computed once per CTA, a thread per batch element: inlined into every role
 // its 64-bit divisions would be half of the kernel's code.)
+// The batch element, round and step at which a cluster's range starts.
+ICSA_DEV int4 cluster_start(const Kv8TcParams& p, const Kv8Cache& c, int cluster, int clusters) {
+  int64_t total = 0;
+  for (int i = 0; i < c.B; ++i) total += extent(p, cache_length(c, i)).head * c.H;
+  int64_t x = total * cluster / clusters;
+  int b = 0;
+  Extent e = extent(p, cache_length(c, 0));
+  while (x >= e.head * c.H && b + 1 < c.B) {
+    x -= e.head * c.H;
+    e = extent(p, cache_length(c, ++b));
+  }
+  const Point q = locate(p, c, e, x);
+  return make_int4(b, q.round, q.step, 0);
+}
 ICSA_DEV Range cluster_range(const Kv8TcParams& p, const Kv8Cache& c, int b, int cluster, int clusters) {
   int64_t total = 0, base = 0;
 #pragma unroll 1
@@ -409,6 +423,10 @@ ICSA_DEV void copy_queries(const Kv8TcParams& p, const Round& w, int tile, uint3
 // lie across the lanes, are innermost.
 ICSA_DEV float* partial_tile(const Kv8TcParams& p, int cluster, int part, int slot, int D) {
   return p.partial + (size_t(cluster * 2 + part) * 2 + slot) * kPairRows * (D + 2);
+}
+// behind the parts: where each cluster's range starts
+ICSA_DEV int4* cluster_starts(const Kv8TcParams& p, int clusters, int D) {
+  return reinterpret_cast<int4*>(p.partial + size_t(clusters) * 4 * kPairRows * (D + 2));
 }
 
 // O of a tile (of both slots where they took the steps in turn) to the
@@ -974,6 +992,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (q0) drain_wait(&sm.q_full[0], (q0 - 1) & 1u, nullptr);
         if (q1) drain_wait(&sm.q_full[1], (q1 - 1) & 1u, nullptr);
       }
+    } else if (!p.whole && rank == 0 && threadIdx.x == kThreads - 32) {
+      // for the kernel that joins the parts
+      cluster_starts(p, gridDim.x >> 1, D)[blockIdx.x >> 1] = cluster_start(p, c, blockIdx.x >> 1, gridDim.x >> 1);
     }
   }
   __syncwarp();
@@ -994,24 +1015,17 @@ template <int D>
 __global__ void __launch_bounds__(256) kv8_tc_join_kernel(const Kv8TcParams p, const Kv8Cache c, int clusters) {
   const int k = int(blockIdx.x) + 1;
   wait_prior_grid();
-  int64_t total = 0;
-  for (int i = 0; i < c.B; ++i) total += extent(p, cache_length(c, i)).head * c.H;
-  // cluster k covers [total k / clusters, total (k + 1) / clusters)
-  int64_t base = 0;
-  const int64_t x = total * k / clusters;
-  int b = 0;
-  Extent ext = extent(p, cache_length(c, 0));
-  while (x >= base + ext.head * c.H && b + 1 < c.B) {
-    base += ext.head * c.H;
-    ext = extent(p, cache_length(c, ++b));
-  }
-  auto at = [&](int j) { return locate(p, c, ext, total * j / clusters - base); };
-  const Point q0 = at(k), before = at(k - 1);
-  if (q0.step == 0 || (before.round == q0.round && before.step > 0)) return;
-  const int k0 = k - 1;
+  extern __shared__ int4 at[];  // where the clusters' ranges start
+  for (int j = threadIdx.x; j <= clusters; j += 256)
+    at[j] = j < clusters ? cluster_starts(p, clusters, D)[j] : make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  const auto same_round = [&](int i, int j) { return at[i].x == at[j].x && at[i].y == at[j].y; };
+  const int4 q0 = at[k];
+  if (q0.z == 0 || (same_round(k - 1, k) && at[k - 1].z > 0)) return;
+  const int k0 = k - 1, b = q0.x;
   int k1 = k;
-  while (at(k1 + 1).round == q0.round) ++k1;
-  const int h = q0.round / p.rounds, r = q0.round - h * p.rounds;
+  while (same_round(k1 + 1, k)) ++k1;
+  const int h = q0.y / p.rounds, r = q0.y - h * p.rounds;
   // the round starts in cluster k0's range (its last partial buffer) and
   // before those of the clusters behind it; lanes are rows
   const int tr = blockIdx.y * 32 + (threadIdx.x & 31), slot = tr / kPairRows, row = tr % kPairRows;
@@ -1021,20 +1035,33 @@ __global__ void __launch_bounds__(256) kv8_tc_join_kernel(const Kv8TcParams p, c
   float mm = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-  for (int j = k0; j <= k1; ++j) {
-    const Point lo = at(j), hi = at(j + 1);
-    if (lo.round == hi.round && lo.step == hi.step) continue;  // no step falls to this cluster
-    const float* src = partial_tile(p, j, j == k0 ? 1 : 0, slot, D) + row;
-    float x[kPer];
-    const float m = src[D * kPairRows], lk = src[(D + 1) * kPairRows];
+  constexpr int kAhead = 4;  // parts whose loads are on their way together
+  for (int j = k0; j <= k1; j += kAhead) {
+    float x[kAhead][kPer], m[kAhead], lk[kAhead];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = src[(d0 + e) * kPairRows];
-    const float top = fmaxf(mm, m), ref = top == -INFINITY ? 0.f : top;
-    const float f = ex2(mm - ref), g = ex2(m - ref);
+    for (int i = 0; i < kAhead; ++i) {
+      m[i] = -INFINITY;
+      lk[i] = 0.f;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * f + x[e] * g;
-    l = l * f + lk * g;
-    mm = top;
+      for (int e = 0; e < kPer; ++e) x[i][e] = 0.f;
+      const int n = j + i;
+      // (a cluster without a step between two others has no part)
+      if (n > k1 || (same_round(n, n + 1) && at[n].z == at[n + 1].z)) continue;
+      const float* src = partial_tile(p, n, n == k0 ? 1 : 0, slot, D) + row;
+      m[i] = src[D * kPairRows];
+      lk[i] = src[(D + 1) * kPairRows];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[i][e] = src[(d0 + e) * kPairRows];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float top = fmaxf(mm, m[i]), ref = top == -INFINITY ? 0.f : top;
+      const float f = ex2(mm - ref), g = ex2(m[i] - ref);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * f + x[i][e] * g;
+      l = l * f + lk[i] * g;
+      mm = top;
+    }
   }
   __shared__ float tile[32][D + 1];
 #pragma unroll
@@ -1058,8 +1085,8 @@ cudaError_t launch_as(const Kv8TcParams& p, const Kv8TcMaps& maps, const Kv8Cach
   kv8_tc_kernel<D><<<2 * clusters, kThreads, smem, stream>>>(p, c, maps);
   if ((e = cudaGetLastError()) != cudaSuccess || p.whole || clusters == 1) return e;
   const int rows = std::min(p.rows, 2 * kPairRows);
-  return launch_chained(kv8_tc_join_kernel<D>, dim3(clusters - 1, (rows + 31) / 32), dim3(256), 0, stream, p, c,
-                        clusters);
+  return launch_chained(kv8_tc_join_kernel<D>, dim3(clusters - 1, (rows + 31) / 32), dim3(256),
+                        (clusters + 1) * sizeof(int4), stream, p, c, clusters);
 }
 
 }  // namespace
@@ -1072,7 +1099,7 @@ Kv8TcPlan kv8_tc_plan(const Kv8Cache& c, int rows, int num_sms) {
   t.whole = steps <= (c.D == 128 ? Cfg<128>::kStages : Cfg<64>::kStages);
   const int64_t work = int64_t(c.B) * c.H * t.rounds * (t.whole ? 1 : steps);
   t.clusters = int(std::max<int64_t>(1, std::min<int64_t>(num_sms / 2, work)));
-  t.bytes = t.whole ? 0 : size_t(t.clusters) * 4 * kPairRows * (c.D + 2) * sizeof(float);
+  t.bytes = t.whole ? 0 : size_t(t.clusters) * (4 * kPairRows * (c.D + 2) * sizeof(float) + sizeof(int4));
   return t;
 }
 
