@@ -25,7 +25,8 @@
 // Both products run in f16 with float32 accumulation: e4m3 codes are exact in
 // f16, a query row is scaled by a power of two to [2^14, 2^15) (bf16 has 8
 // significant bits, f16 11; only elements 2^-28 below the row's largest lose
-// bits), and the probabilities have 11 bits.  The scale of a value block
+// bits), and the probabilities have 11 bits (below 2^-14 of the largest they
+// are multiples of 2^-24 of it).  The scale of a value block
 // joins the exponent: with s the base-2 scores and v the log2 of the scale,
 //   p = 2^(s + v - m),  m the running maximum of s + v,
 // p enters the product with the codes, and 2^-v p the row sum.
@@ -592,7 +593,7 @@ cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out
   return out_dtype == ICSA_BF16 ? dequantize_as<__nv_bfloat16>(c, out, stream) : dequantize_as<float>(c, out, stream);
 }
 
-int kv8_decode_splits(int B, int H, int rows, int L, int D, int num_sms) {
+Kv8DecodePlan kv8_decode_plan(int B, int H, int rows, int L, int D, int num_sms) {
   const int64_t ctas = int64_t(B) * H * ((rows + 7) / 8), slots = int64_t(num_sms) * decode_ctas(D);
   const int64_t nb = (L + kTokens - 1) / kTokens;
   // Waves of CTAs times the steps of a warp, two steps' time for a CTA's start
@@ -601,16 +602,12 @@ int kv8_decode_splits(int B, int H, int rows, int L, int D, int num_sms) {
   // on 296 places) 284 us, seven 232 us; D = 64, one row: three (two to an
   // SM) 83 us, eleven 69 us.
   const int64_t most = std::min<int64_t>(nb / kDWarps, 32);
-  int64_t best = 1;
-  double best_cost = 0;
+  Kv8DecodePlan best = {1, 0.0};
   for (int64_t s = 1; s <= std::max<int64_t>(most, 1); ++s) {
-    const double cost = double((ctas * s + slots - 1) / slots) * (double(nb) / double(s * kDWarps) + 2.0);
-    if (s == 1 || cost < best_cost) {
-      best = s;
-      best_cost = cost;
-    }
+    const double steps = double((ctas * s + slots - 1) / slots) * (double(nb) / double(s * kDWarps) + 2.0);
+    if (s == 1 || steps < best.steps) best = {int(s), steps};
   }
-  return int(best);
+  return best;
 }
 
 cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream) {

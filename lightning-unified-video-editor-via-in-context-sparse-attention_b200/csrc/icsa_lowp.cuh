@@ -115,7 +115,11 @@ struct Kv8AttnParams {
   int splits;
   float* partial;          // [rows, splits, D + 2] when splits > 1
 };
-int kv8_decode_splits(int B, int H, int rows, int L, int D, int num_sms);
+struct Kv8DecodePlan {
+  int splits;
+  double steps;            // its time, in steps of a warp (one block each)
+};
+Kv8DecodePlan kv8_decode_plan(int B, int H, int rows, int L, int D, int num_sms);
 cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream);
 
 // The same for many query rows, on the tensor cores of SM pairs, for at most

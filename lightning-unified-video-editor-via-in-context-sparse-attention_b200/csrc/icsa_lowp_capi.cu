@@ -196,13 +196,6 @@ int check_cache_buffers(const char* who, const icsa_kv8_cache* c, bool k, bool v
   return ICSA_OK;
 }
 
-// Few query rows per cache head: the register-fed kernel, which takes 8 rows a
-// CTA.  Measured against the pair kernel, us: 2 x 40 heads, D = 128, 32760
-// keys, 32 rows 542 / 566, 64 rows 818 / 566; 300 keys, 48 rows 24 / 28, 64
-// rows 35 / 28; 1 x 8 heads, 32760 keys, 48 rows 60 / 97; 2 x 40, D = 64,
-// 32760 keys, 48 rows 349 / 417.
-constexpr int kDecodeRows = 48;
-
 enum AttnPath { kDecode, kPairs, kDense };
 
 struct AttnPlan {
@@ -213,17 +206,24 @@ struct AttnPlan {
   size_t bytes;          // workspace
 };
 
-// Estimated times of the two ways to attend over a cache whose steps do not
-// fit the pair kernel's ring.  The dense kernels run a 256-row tile per SM
-// pair (D = 128) or SM (D = 64) at a time, 0.86 / 1.87 us a step of 128 keys,
-// in waves of about 7 us beside the steps, on a bf16 copy that is written and
-// read (6 bytes an element).  The pair kernel takes 2.6 us (D = 64: 2.0) for
-// a step of two tiles and 2.2 us (1.6) for one, deals the steps evenly to all
-// pairs and has about 40 us of its own (the join among them).
-// Measured, us, dense / pairs, D = 128: 1 x 40 heads, 1560 rows, 32760 keys
-// 1036 / 1228; 4096 rows 2091 / 2453; 2 x 40, 512 rows 973 / 640; 256 rows
-// 762 / 585; 1 x 8, 2000 rows, 4096 keys 47 / 77.  D = 64: 2 x 40, 2048 rows,
-// 8192 keys 651 / 583; 2 x 8, 512 rows 143 / 64.
+// Estimated times of the three ways to attend, us.
+//  * The register-fed kernel (decode) reads the cache once for every 8 rows;
+//    2.6 us (D = 64: 1.7) for the four blocks of a step of its warps.
+//  * The pair kernel deals its steps evenly to all SM pairs, 2.7 us (2.0) for
+//    a step of two 256-row tiles and 1.8 us (1.65) for one; where rounds are
+//    cut their parts are joined, the more the fewer rounds there are.
+//  * The dense kernels run a 256-row tile per SM pair (D = 128) or SM (D = 64)
+//    at a time, 0.86 / 1.87 us a step of 128 keys, in waves of about 7 us
+//    beside the steps, on a bf16 copy that is written and read (6 bytes an
+//    element).  Their probabilities are bf16, so few rows do without them.
+// Constants fitted to 324 sizes (1, 8 and 2 x 40 heads, D = 64 and 128, 100 to
+// 32000 keys, 16 to 4096 rows): the choice is within 1 % of the best of the
+// three on average, at worst a quarter slower.  Measured, us, decode / pairs /
+// dense, D = 128: 1 x 8 heads, 8000 keys, 64 rows 23 / 37 / 67, 512 rows 121 /
+// 47 / 67, 4096 rows - / 159 / 128; 2 x 40 heads, 300 keys, 48 rows 21 / 25 /
+// 29, 256 rows 86 / 25 / 29; 32000 keys, 16 rows 216 / 591 / 757, 1024 rows
+// 12653 / 1559 / 1542, 2048 rows - / 2799 / 2387.
+constexpr int kNoCopyRows = 48, kDecodeMost = 8 * 65535;
 double dense_us(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   const bool wide = c.D == 128;
   const int64_t tiles = int64_t(c.B) * Hq * ((Lq + 255) / 256), units = std::max(1, wide ? sms / 2 : sms);
@@ -232,29 +232,43 @@ double dense_us(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
 }
 double pairs_us(const icsa::Kv8Cache& c, const icsa::Kv8TcPlan& t, int sms) {
   const bool wide = c.D == 128;
-  const double steps = (double(c.L) + 127) / 128;
-  const double head = (t.tiles / 2) * (wide ? 2.6 : 2.0) + (t.tiles & 1) * (wide ? 2.2 : 1.6);
-  return double(c.B) * c.H * steps * head / std::max(1, sms / 2) + 40.0;
+  const double steps = double((int64_t(c.L) + 127) / 128), clusters = std::max(1, sms / 2);
+  const double two = wide ? 2.74 : 2.02, one = wide ? 1.83 : 1.65;  // a step of two tiles, of one
+  const double heads = double(c.B) * c.H;
+  if (t.whole) {
+    const double end = 1.76;  // of a round
+    const double head = (t.tiles / 2) * (steps * two + end) + (t.tiles & 1) * (steps * one + end);
+    const double round = steps * (t.tiles > 1 ? two : one) + end;
+    return 9.1 + std::max(heads * head / clusters, t.tiles == 1 ? round * std::ceil(heads / clusters) : round);
+  }
+  const double head = (t.tiles / 2) * two + (t.tiles & 1) * one;
+  return 27.4 + 0.19 * std::max(1.0, clusters / (heads * t.rounds)) + heads * steps * head / clusters;
+}
+double decode_us(const icsa::Kv8Cache& c, const icsa::Kv8DecodePlan& d) {
+  return 4.0 + d.steps * (c.D == 128 ? 2.6 : 1.7) + (d.splits > 1 ? 2.0 : 0.0);
 }
 
 AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   AttnPlan a = {};
   const int64_t rows = int64_t(Lq) * (Hq / c.H);
-  if (rows <= kDecodeRows) {
-    a.path = kDecode;
-    a.splits = icsa::kv8_decode_splits(c.B, c.H, int(rows), c.L, c.D, sms);
-    a.bytes = a.splits == 1 ? 0 : align256(size_t(c.B) * c.H * rows * a.splits * (c.D + 2) * sizeof(float));
-    return a;
-  }
   a.tc = icsa::kv8_tc_plan(c, int(rows), sms);
-  if (!a.tc.whole && c.nb <= 16384 && dense_us(c, Lq, Hq, sms) < pairs_us(c, a.tc, sms)) {
+  a.path = kPairs;
+  a.bytes = align256(a.tc.bytes);
+  double us = pairs_us(c, a.tc, sms);
+  if (rows <= kDecodeMost) {
+    const icsa::Kv8DecodePlan d = icsa::kv8_decode_plan(c.B, c.H, int(rows), c.L, c.D, sms);
+    if (decode_us(c, d) < us) {
+      us = decode_us(c, d);
+      a.path = kDecode;
+      a.splits = d.splits;
+      a.bytes = a.splits == 1 ? 0 : align256(size_t(c.B) * c.H * rows * a.splits * (c.D + 2) * sizeof(float));
+    }
+  }
+  if (rows > kNoCopyRows && c.nb <= 16384 && dense_us(c, Lq, Hq, sms) < us) {
     a.path = kDense;
     a.v_offset = align256(size_t(c.B) * c.L * c.H * c.D * 2);
     a.bytes = 2 * a.v_offset;
-    return a;
   }
-  a.path = kPairs;
-  a.bytes = align256(a.tc.bytes);
   return a;
 }
 
