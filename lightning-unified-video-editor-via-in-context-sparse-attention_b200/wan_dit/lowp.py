@@ -83,20 +83,20 @@ def _device(where, *tensors):
     for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{where}: expected CUDA tensors")
-        i = t.get_device()
-        if index is None:
+        i = t.get_device() if isinstance(t, torch.Tensor) else -1     # -1 on the CPU
+        if i != index:
+            if i < 0 or not t.is_cuda:
+                raise ValueError(f"{where}: expected CUDA tensors")
+            if index is not None:
+                raise ValueError(f"{where}: tensors on cuda:{index} and cuda:{i}")
             index = i
-        elif i != index:
-            raise ValueError(f"{where}: tensors on cuda:{index} and cuda:{i}")
     return index
 
 
 def _on(index, fn, *args):
     """fn(library, raw handle of the device's current stream, *args) with the device current."""
     lib = _lib or _load()
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         return fn(lib, torch._C._cuda_getCurrentRawStream(index), *args)
     with torch.cuda.device(index):
         return fn(lib, torch._C._cuda_getCurrentRawStream(index), *args)
@@ -150,6 +150,7 @@ class Fp4Tensor:
         return self.data.device
 
 
+@functools.lru_cache(maxsize=1024)
 def fp4_storage(rows: int, K: int, fmt: str):
     """Shapes of `data` and `scales` of a [rows, K] Fp4Tensor."""
     tiles = 256 // (4 * FP4_BLOCK[fmt])
@@ -175,14 +176,17 @@ def fp4_global_scale(x: torch.Tensor) -> float:
 
 
 def _rows2d(where, x):
-    if x.dim() != 2 or x.dtype not in _DT:
-        raise ValueError(f"{where}: expected a 2-D bf16 or f32 tensor, got {x.dtype} {tuple(x.shape)}")
-    if x.shape[1] < 1:
+    """x as rows of contiguous elements that do not overlap, and their distance."""
+    shape = x.shape
+    if len(shape) != 2 or x.dtype not in _DT:
+        raise ValueError(f"{where}: expected a 2-D bf16 or f32 tensor, got {x.dtype} {tuple(shape)}")
+    rows, K = shape
+    if K < 1:
         raise ValueError(f"{where}: no columns")
-    # rows of contiguous elements, not overlapping
-    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+    ld, step = x.stride()
+    if (K > 1 and step != 1) or (rows > 1 and ld < K):
+        x, ld = x.contiguous(), K
+    return x, (ld if rows > 1 else K)
 
 
 def fp4_quantize(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0) -> Fp4Tensor:
@@ -349,9 +353,9 @@ def _int64x3(a, b, c):
     return (ctypes.c_int64 * 3)(a, b, c)
 
 
-def _strides(t):
+def _strides(shape, strides):
     """Batch, token and head strides; 0 for an axis of one."""
-    (B, L, H, _), (sb, st, sh, _) = t.shape, t.stride()
+    (B, L, H, _), (sb, st, sh, _) = shape, strides
     return _int64x3(sb if B > 1 else 0, st if L > 1 else 0, sh if H > 1 else 0)
 
 
@@ -363,33 +367,39 @@ def kv8_quantize(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tenso
     index = _device("kv8_quantize", k, v, lengths)
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DT:
         raise ValueError(f"kv8_quantize: k {tuple(k.shape)} and v {tuple(v.shape)} must be bf16 or f32 [B, L, H, D]")
-    B, L, H, D = k.shape
-    if D not in (64, 128):
+    B, L, H, D = shape = k.shape
+    if D != 64 and D != 128:
         raise ValueError(f"kv8_quantize: head dim {D} (supported: 64, 128)")
-    if min(B, L, H) < 1:
-        raise ValueError(f"kv8_quantize: empty k, v {tuple(k.shape)}")
-    _check_lengths("kv8_quantize", lengths, B)
-    if k.stride(3) != 1:
+    if B < 1 or L < 1 or H < 1:
+        raise ValueError(f"kv8_quantize: empty k, v {tuple(shape)}")
+    if lengths is not None:
+        _check_lengths("kv8_quantize", lengths, B)
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1:
         k = k.contiguous()
-    if v.stride(3) != 1:
+        ks = k.stride()
+    if vs[3] != 1:
         v = v.contiguous()
-    return _on(index, _quantize_kv, k, v, lengths)
+        vs = v.stride()
+    return _on(index, _quantize_kv, k, v, lengths, shape, ks, vs)
 
 
-def _quantize_kv(lib, stream, k, v, lengths):
-    B, L, H, D = k.shape
+def _quantize_kv(lib, stream, k, v, lengths, shape, ks, vs):
+    B, L, H, D = shape
     nb = -(-L // KV8_TOKENS)
     device, T, n = k.device, KV8_TOKENS, nb * KV8_TOKENS * D
-    c = object.__new__(Kv8Cache)        # its tensors are as the constructor wants them
-    c.__dict__.update(
-        k=_empty((B, H, nb, T, D), (H * n, n, T * D, D, 1), dtype=torch.float8_e4m3fn, device=device),
-        v=_empty((B, H, nb, D, T), (H * n, n, T * D, T, 1), dtype=torch.float8_e4m3fn, device=device),
-        k_scale=_empty((B, H, nb), (H * nb, nb, 1), dtype=torch.float32, device=device),
-        v_scale=_empty((B, H, nb), (H * nb, nb, 1), dtype=torch.float32, device=device), L=L, lengths=lengths)
-    code = lib.icsa_kv8_quantize(ctypes.byref(c._desc()), k.data_ptr(), v.data_ptr(), _DT[k.dtype], _strides(k),
-                                 _strides(v), stream)
+    codes = _empty((B, H, nb, T, D), (H * n, n, T * D, D, 1), dtype=torch.float8_e4m3fn, device=device)
+    values = _empty((B, H, nb, D, T), (H * n, n, T * D, T, 1), dtype=torch.float8_e4m3fn, device=device)
+    k_scale = _empty((B, H, nb), (H * nb, nb, 1), dtype=torch.float32, device=device)
+    v_scale = torch.empty_like(k_scale)
+    desc = _Kv8Desc(B, H, L, D, codes.data_ptr(), values.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                    lengths.data_ptr() if lengths is not None else None)
+    code = lib.icsa_kv8_quantize(ctypes.byref(desc), k.data_ptr(), v.data_ptr(), _DT[k.dtype], _strides(shape, ks),
+                                 _strides(shape, vs), stream)
     if code:
         _capi.check(code, "icsa_kv8_quantize")
+    c = object.__new__(Kv8Cache)        # its tensors are as the constructor wants them
+    c.__dict__.update(k=codes, v=values, k_scale=k_scale, v_scale=v_scale, L=L, lengths=lengths)
     return c
 
 
@@ -402,9 +412,8 @@ def kv8_dequantize(cache: Kv8Cache, dtype: torch.dtype = torch.bfloat16):
 
 def _dequantize_kv(lib, stream, cache, dtype):
     (B, H, _, _, D), L, device = cache.k.shape, cache.L, cache.k.device
-    shape, strides = (B, L, H, D), (L * H * D, H * D, D, 1)
-    k = _empty(shape, strides, dtype=dtype, device=device)
-    v = _empty(shape, strides, dtype=dtype, device=device)
+    k = _empty((B, L, H, D), (L * H * D, H * D, D, 1), dtype=dtype, device=device)
+    v = torch.empty_like(k)
     code = lib.icsa_kv8_dequantize(ctypes.byref(cache._desc()), k.data_ptr(), v.data_ptr(), _DT[dtype], stream)
     if code:
         _capi.check(code, "icsa_kv8_dequantize")
@@ -418,9 +427,10 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache) -> torch.Tensor:
     cache head h // (Hq / H))."""
     index = _device("kv8_attention", q, cache.k)
     B, H, _, _, D = cache.k.shape
-    if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != B or q.shape[3] != D or q.shape[2] % H or not q.shape[2]:
-        raise ValueError(f"kv8_attention: q must be bf16 [{B}, Lq, a multiple of {H}, {D}], got {q.dtype} {tuple(q.shape)}")
-    return _on(index, _attention, q, cache)
+    shape = q.shape
+    if len(shape) != 4 or q.dtype != torch.bfloat16 or shape[0] != B or shape[3] != D or shape[2] % H or not shape[2]:
+        raise ValueError(f"kv8_attention: q must be bf16 [{B}, Lq, a multiple of {H}, {D}], got {q.dtype} {tuple(shape)}")
+    return _on(index, _attention, index, q, shape, cache, H)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -428,9 +438,8 @@ def _attention_workspace(index, B, H, L, D, Lq, Hq):
     return _lib.icsa_kv8_attention_workspace_size(ctypes.byref(_Kv8Desc(B, H, L, D)), Lq, Hq)
 
 
-def _attention(lib, stream, q, cache):
-    B, Lq, Hq, D = q.shape
-    H = cache.k.shape[1]
+def _attention(lib, stream, index, q, shape, cache, H):
+    B, Lq, Hq, D = shape
     out = _empty((B, Lq, Hq, D), (Lq * Hq * D, Hq * D, D, 1), dtype=torch.bfloat16, device=q.device)
     if Lq == 0:
         return out
@@ -442,7 +451,7 @@ def _attention(lib, stream, q, cache):
         st = Hq * D
     if Lq == 1 and B == 1:
         st = Hq * D
-    size = _attention_workspace(q.get_device(), B, H, cache.L, D, Lq, Hq)
+    size = _attention_workspace(index, B, H, cache.L, D, Lq, Hq)
     ws, ptr = _bytes(out, size)
     code = lib.icsa_kv8_attention(ctypes.byref(cache._desc()), q.data_ptr(), _int64x3(Lq * st, st, D), out.data_ptr(),
                                   Lq, Hq, ptr, size, stream)
