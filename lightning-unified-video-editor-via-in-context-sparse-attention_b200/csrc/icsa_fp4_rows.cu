@@ -9,16 +9,19 @@
 // bytes, 8 or 10 K steps of 256 columns (16 KB of codes, 2 KB of scales) on
 // their way at a time, and accumulators are narrow enough for two in TMEM.
 //
-// Work is dealt in K steps: with T = tiles x steps, CTA c of C takes steps
-// [T c / C, T (c + 1) / C), so every SM reads the same number of bytes
-// whatever the tile count (30720 outputs are 240 tiles: dealt whole, 92 of
-// 148 SMs would read two and the others one).  Parts of a tile cut between
-// CTAs go to the workspace as float32, at most two for a CTA, and a second
-// kernel adds them in the order of K.
+// Work: CTAs take whole tiles where that is fast enough.  Few tiles with a
+// long K are cut into equal parts, and tiles that do not divide among the SMs
+// may be dealt in K steps (T = tiles x steps, CTA c of C takes steps
+// [T c / C, T (c + 1) / C)).  Parts of a tile go to the workspace as float32,
+// at most two for a CTA, and a second kernel adds them in the order of K.
 //
-// 1 x 5120 -> 30720 (88.6 MB, 13.5 us at the copy rate), the row's
-// quantisation, this kernel and the join: 24.7 us, against 33.2 us in the
-// 256 x 256 tiles of icsa_fp4_gemm.cu; 16 x 5120 -> 5120 17.4 against 20 us.
+// Captured calls of one row, us (whole tiles / in steps over all SMs / as
+// chosen): 5120 -> 30720 (88.6 MB, 13.5 us at the copy rate) 17.7 / 19.8 /
+// 17.7, 5120 -> 5120 8.7 / 9.8 / 8.7, 13824 -> 1024 18.2 / 13.4 / 8.2, 13824 ->
+// 5120 18.5 / 13.1 / 11.8.  With the row's quantisation 5120 -> 30720 takes
+// 21.8 us a call, against 33.2 us in the 256 x 256 tiles of icsa_fp4_gemm.cu.
+// A step of one CTA takes 0.29 us (0.37 where all of them share the memory),
+// so what is left is the start and the end of each CTA's stream.
 //
 // Roles per CTA (192 threads): warps 0-3 epilogue (thread <-> TMEM lane <->
 // weight row <-> output column), warp 4 TMA producer, warp 5 TMEM allocation
@@ -140,7 +143,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &sm.abort_flag;
   const int64_t total = int64_t(p.n_tiles) * p.k_steps;
-  const int64_t x0 = first_step(total, blockIdx.x, gridDim.x), x1 = first_step(total, blockIdx.x + 1, gridDim.x);
+  // cut tiles: equal numbers of steps; whole tiles: equal numbers of tiles
+  const int64_t grain = p.splits > 1 ? 1 : p.k_steps;
+  const int64_t x0 = first_step(total / grain, blockIdx.x, gridDim.x) * grain;
+  const int64_t x1 = first_step(total / grain, blockIdx.x + 1, gridDim.x) * grain;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.full[i], 1);
@@ -295,11 +301,21 @@ __global__ void __launch_bounds__(kTileN) fp4_rows_join_kernel(const Fp4GemmPara
   if (c0 == c1 || n >= p.N) return;  // one CTA wrote the tile
   const int m0 = blockIdx.y * kJoinRows;
   float acc[kJoinRows] = {};
-  for (int c = c0; c <= c1; ++c) {
-    const float* src = partial_tile(p, c, first_step(total, c, ctas) <= t0) + threadIdx.x;
+  constexpr int kAhead = 4;  // parts whose loads are on their way together
+  for (int c = c0; c <= c1; c += kAhead) {
+    float x[kAhead][kJoinRows] = {};
 #pragma unroll
-    for (int i = 0; i < kJoinRows; ++i)
-      if (m0 + i < p.M) acc[i] += src[(m0 + i) * kTileN];
+    for (int j = 0; j < kAhead; ++j) {
+      if (c + j > c1) break;
+      const float* src = partial_tile(p, c + j, first_step(total, c + j, ctas) <= t0) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < kJoinRows; ++i)
+        if (m0 + i < p.M) x[j][i] = src[(m0 + i) * kTileN];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int i = 0; i < kJoinRows; ++i) acc[i] += x[j][i];
   }
   const float bias = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
 #pragma unroll
@@ -323,9 +339,21 @@ int tiles_of(int N) { return (N + kTileN - 1) / kTileN; }
 Fp4RowsPlan fp4_rows_plan(int M, int N, int K, int num_sms) {
   Fp4RowsPlan r = {};
   const int64_t k_steps = (K + kFp4TileK - 1) / kFp4TileK, tiles = tiles_of(N), total = tiles * k_steps;
-  // at least two steps a CTA, unless that leaves SMs without a whole tile
-  r.ctas = int(std::min<int64_t>(num_sms, std::max(tiles, total / 2)));
-  for (int c = 1; c < r.ctas && !r.join; ++c) r.join = first_step(total, c, r.ctas) % k_steps != 0;
+  // A step takes 0.29 us, 0.37 where all SMs read the weight at once; joining
+  // parts 3 us and a launch, and 0.15 us for each part of a tile.
+  const auto step = [&](int64_t ctas) { return std::max(0.29, 0.37 * double(ctas) / num_sms); };
+  r.ctas = int(std::min<int64_t>(num_sms, tiles));
+  double best = double((tiles + r.ctas - 1) / r.ctas * k_steps) * step(r.ctas);
+  const auto consider = [&](int64_t ctas, int64_t steps, double parts) {
+    const double us = double(steps) * step(ctas) + 4.0 + 0.15 * parts;
+    if (us >= best) return;
+    best = us;
+    r.ctas = int(ctas);
+    r.join = true;
+  };
+  for (int64_t parts = 2; parts <= k_steps && tiles * parts <= num_sms; ++parts)
+    consider(tiles * parts, (k_steps + parts - 1) / parts, double(parts));
+  if (tiles * 2 > num_sms && tiles % num_sms != 0 && total > num_sms) consider(num_sms, (total + num_sms - 1) / num_sms, 2.0);
   r.bytes = r.join ? size_t(2) * r.ctas * M * kTileN * sizeof(float) : 0;
   return r;
 }
@@ -336,6 +364,7 @@ cudaError_t launch_fp4_rows(Fp4GemmParams p, const Fp4GemmMaps& maps, int format
                             cudaStream_t stream) {
   p.k_steps = (p.K + kFp4TileK - 1) / kFp4TileK;
   p.n_tiles = tiles_of(p.N);
+  p.splits = plan.join ? 2 : 1;
   const bool nv = format == ICSA_NVFP4;
   cudaError_t e;
   if (fp4_rows_box(p.M) == 16)

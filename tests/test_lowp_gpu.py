@@ -149,7 +149,8 @@ def test_linear_layer(fmt, M, N, K, bias, act):
 @pytest.mark.parametrize("M,N,K,bias,act", [
     (1, 30001, 1030, True, None), (1, 128, 65536, False, None), (16, 19001, 520, True, "gelu_tanh"),
     (17, 129, 8192, True, None), (32, 3000, 256, False, None), (33, 40000, 300, True, None),
-    (64, 2560, 5120, True, "gelu_tanh"), (65, 2560, 5120, True, "gelu_tanh")])
+    (64, 2560, 5120, True, "gelu_tanh"), (65, 2560, 5120, True, "gelu_tanh"),
+    (1, 20000, 5120, False, None), (5, 19001, 5300, True, "gelu_tanh"), (40, 19001, 5300, True, None)])
 def test_linear_layer_of_few_rows(fmt, M, N, K, bias, act):
     """Tiles cut between CTAs at every kind of boundary: many tiles, one tile, whole tiles."""
     test_linear_layer(fmt, M, N, K, bias, act)
@@ -193,7 +194,7 @@ def test_linear_layer_refuses_mixed_formats_and_devices():
     assert lowp.fp4_linear(x[:0], w, b).shape == (0, 32)
 
 
-@pytest.mark.parametrize("M,K", [(3, 2048), (70, 4096)])
+@pytest.mark.parametrize("M,K", [(3, 8192), (70, 4096)])
 def test_linear_layer_checks_its_workspace_and_leaves_what_is_behind_its_rows(M, K):
     lib = lowp._load()
     x, w, b, want, tol = linear_case(M, 40, K, "nvfp4", True, None)
@@ -514,6 +515,7 @@ def test_second_kernels_in_two_graphs_and_on_two_streams():
     joins partial results from its workspace."""
     g = torch.Generator().manual_seed(4)
     w = lowp.fp4_quantize((torch.randn(300, 4096, generator=g) / 64).cuda(), "nvfp4", 2.0 ** -9)
+    long = lowp.fp4_quantize((torch.randn(300, 16384, generator=g) / 64).cuda(), "nvfp4", 2.0 ** -9)
     k, v = kv_rows(1, 9000, 2, 128, torch.bfloat16)
     cache = lowp.kv8_quantize(k.cuda(), v.cuda())
     k, v = kv_rows(1, 8000, 8, 128, torch.bfloat16)
@@ -521,11 +523,11 @@ def test_second_kernels_in_two_graphs_and_on_two_streams():
 
     def inputs(seed):
         g = torch.Generator().manual_seed(seed)
-        return [torch.randn(n, 4096, generator=g).to(torch.bfloat16).cuda() for n in (9, 70)] + [
+        return [torch.randn(n, m, generator=g).to(torch.bfloat16).cuda() for n, m in ((9, 16384), (70, 4096))] + [
             torch.randn(1, n, h, 128, generator=g).to(torch.bfloat16).cuda() for n, h in ((1, 2), (60, 2), (512, 8))]
 
     def run(x9, x70, q1, q60, q512):
-        return (lowp.fp4_linear(x9, w), lowp.fp4_linear(x70, w), lowp.kv8_attention(q1, cache),
+        return (lowp.fp4_linear(x9, long), lowp.fp4_linear(x70, w), lowp.kv8_attention(q1, cache),
                 lowp.kv8_attention(q60, cache), lowp.kv8_attention(q512, cache8))
     want = [run(*inputs(s)) for s in (0, 1, 2)]
     static = inputs(0)
