@@ -234,7 +234,7 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
   int count = 0;
   for (int u = cluster; u < p.units; u += clusters, ++count) {
     const Unit t = decode_unit(p, u);
-    const int row0 = t.mt * (2 * kRows) + int(rank) * kRows + 32 * (warp & 3), r = row0 + lane;
+    const int row0 = t.mt * (2 * kRows) + int(rank) * kRows + 32 * (warp & 3);
     const int c0 = t.nt * kCols + 128 * w;
     {
       const int c = c0 + int(threadIdx.x & 127);
@@ -253,11 +253,29 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
     __syncwarp();
     if (!ok || row0 >= p.M) continue;
     if (p.splits > 1) {
-      if (r >= p.M) continue;
-      // n_pad is a multiple of 256: whole rows of the tile are stored
-      float4* dst = reinterpret_cast<float4*>(p.partial + (size_t(t.split) * p.M + r) * p.n_pad + c0);
+      // through the box, so that a warp stores whole lines (rows straight from
+      // registers, 32 lines an instruction, took 4 us a tile); n_pad is a
+      // multiple of 256: whole rows of the tile are stored
+      const int unit = lane & 7;
+      float* dst = p.partial + (size_t(t.split) * p.M + row0) * p.n_pad + c0 + 4 * unit;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) dst[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+      for (int q = 0; q < 4; ++q) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float* x = acc + 32 * q + 4 * i;
+          *reinterpret_cast<float4*>(box + lane * 128 + ((uint32_t(i) ^ uint32_t(lane & 7)) << 4)) =
+              make_float4(x[0], x[1], x[2], x[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = 4 * i + (lane >> 3);
+          const float4 v =
+              *reinterpret_cast<const float4*>(box + row * 128 + ((uint32_t(unit) ^ uint32_t(row & 7)) << 4));
+          if (row0 + row < p.M) *reinterpret_cast<float4*>(dst + size_t(row) * p.n_pad + 32 * q) = v;
+        }
+      }
       continue;
     }
 #pragma unroll
@@ -363,15 +381,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// out = bf16(act(alpha * (sum of the splits, in order) + bias))
+// out = bf16(act(alpha * (sum of the splits, in order) + bias)); a thread
+// takes four columns of one row.
 __global__ void __launch_bounds__(256) fp4_reduce_kernel(const Fp4GemmParams p) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  const int r = blockIdx.y;
+  const int quads = p.n_pad / 4;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int r = int(i / quads), c = 4 * int(i - int64_t(r) * quads);
   wait_prior_grid();
-  if (c >= p.N) return;
-  float acc = 0.f;
-  for (int s = 0; s < p.splits; ++s) acc += p.partial[(size_t(s) * p.M + r) * p.n_pad + c];
-  p.out[size_t(r) * p.ldo + c] = __float2bfloat16_rn(finish(p, acc, p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.f));
+  if (r >= p.M || c >= p.N) return;
+  const float4* src = reinterpret_cast<const float4*>(p.partial + size_t(r) * p.n_pad + c);
+  const size_t step = size_t(p.M) * quads;
+  float4 a = *src;
+#pragma unroll 4
+  for (int s = 1; s < p.splits; ++s) {
+    const float4 x = src[s * step];
+    a.x += x.x;
+    a.y += x.y;
+    a.z += x.z;
+    a.w += x.w;
+  }
+  const float v[4] = {a.x, a.y, a.z, a.w};
+  __nv_bfloat16* out = p.out + size_t(r) * p.ldo + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < p.N)
+      out[e] = __float2bfloat16_rn(finish(p, v[e], p.bias != nullptr ? __bfloat162float(p.bias[c + e]) : 0.f));
 }
 
 }  // namespace
@@ -380,14 +414,16 @@ int fp4_gemm_splits(int M, int N, int K, int num_sms) {
   const int64_t tiles = int64_t((M + 2 * kRows - 1) / (2 * kRows)) * ((N + kCols - 1) / kCols);
   const int k_steps = (K + kFp4TileK - 1) / kFp4TileK;
   const int clusters = std::max(1, num_sms / 2);
-  if (tiles <= 0 || tiles * 2 > clusters || M > 65535) return 1;
-  // a step takes about 0.37 us; splitting costs the second kernel (3 us) and
-  // the partial sums, written and read at about 4 TB/s
+  if (tiles <= 0 || tiles * 2 > clusters) return 1;
+  // A step takes 0.33 us; splitting costs a second kernel (2.5 us with its
+  // launch) and the partial sums, written and read at 8 TB/s.  Captured calls,
+  // us, one / two / three splits: 256 x 13824 -> 5120 24.9 / 19.8 / 18.3, 256 x
+  // 5120 -> 5120 14.2 / 14.1 / 13.8, 1024 x 1024 -> 1024 8.4 / 9.9 / 10.4.
   const int most = int(std::min<int64_t>(clusters / tiles, k_steps));
   int best = 1;
-  double best_us = k_steps * 0.37;
+  double best_us = k_steps * 0.33;
   for (int s = 2; s <= most; ++s) {
-    const double us = (k_steps + s - 1) / s * 0.37 + 3.0 + 8.0 * s * M * double(N) / 4e6;
+    const double us = (k_steps + s - 1) / s * 0.33 + 2.5 + 8.0 * s * M * double(N) / 8e6;
     if (us < best_us) {
       best_us = us;
       best = s;
@@ -409,7 +445,8 @@ cudaError_t launch_fp4_gemm(Fp4GemmParams p, const Fp4GemmMaps& maps, int format
   if (e != cudaSuccess) return e;
   e = launch_chained(kernel, dim3(2 * clusters), dim3(kThreads), smem, stream, p, maps);
   if (e != cudaSuccess || p.splits == 1) return e;
-  return launch_chained(fp4_reduce_kernel, dim3((p.N + 255) / 256, p.M), dim3(256), 0, stream, p);
+  const int64_t threads = int64_t(p.M) * (p.n_pad / 4);
+  return launch_chained(fp4_reduce_kernel, dim3(unsigned((threads + 255) / 256)), dim3(256), 0, stream, p);
 }
 
 ICSA_DEFINE_STICKY_ACCESSOR(sticky_status_fp4)
