@@ -29,6 +29,13 @@
 // Few tiles (few rows, or few outputs): K is split over clusters, each
 // writing float32 partial sums that a second kernel adds in a fixed order.
 //
+// 65536 x 5120 -> 13824: 1810 us (5.1 PFLOP/s; nvfp4 and mxfp4 alike), with
+// GELU 1980; 18901 x 13824 -> 5120 517 us.  A K step takes about 700 clk
+// against 512 of its MMAs: filling its 38 KB per SM takes about 600, and
+// operands, fills and scale copies share the 128 B/clk of shared memory.
+// Between tiles the accumulator is drained and refilled once, in about 3600
+// clk of a K = 5120 tile's 17600.
+//
 // Every wait is bounded (about one second); a wait that gives up records a
 // status code (report_error) and the kernel winds down.
 #include "icsa_fp4_mma.cuh"
