@@ -275,7 +275,7 @@ AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
 int check_queries(const char* who, const icsa::Kv8Cache& c, int Lq, int Hq) {
   if (Lq < 1 || Hq < 1 || Hq % c.H != 0)
     return fail(ICSA_ERR_INVALID, "%s: Lq=%d must be positive and Hq=%d a multiple of H=%d", who, Lq, Hq, c.H);
-  if (Lq > (1 << 28) || int64_t(Lq) * Hq > 0x7FFFFFFFll)
+  if (Lq > (1 << 28) || int64_t(Lq) * Hq > 0x7FFFFF00ll)  // rows are rounded up to tiles
     return fail(ICSA_ERR_UNSUPPORTED, "%s: Lq=%d, Hq=%d exceed this build's limits", who, Lq, Hq);
   return ICSA_OK;
 }

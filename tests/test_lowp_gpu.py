@@ -549,6 +549,29 @@ def test_second_kernels_in_two_graphs_and_on_two_streams():
             assert all(torch.equal(a, b) for a, b in zip(out, want[s]))
 
 
+@pytest.mark.parametrize("Lq,H,L", [(2, 2, 9000), (300, 16, 200), (512, 8, 8000), (700, 2, 900)])
+def test_lengths_may_change_between_replays(Lq, H, L):
+    """The few-row kernel, SM pairs with and without a join, the bf16 copy."""
+    k, v = kv_rows(2, L, H, 128, torch.bfloat16)
+    k, v = k.cuda(), v.cuda()
+    q = torch.randn(2, Lq, H, 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    n = torch.tensor([L, L // 3], dtype=torch.int32, device="cuda")
+
+    def run():
+        cache = lowp.kv8_quantize(k, v, n)
+        return lowp.kv8_attention(q, cache), *lowp.kv8_dequantize(cache)
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for lengths in ([L // 2, 0], [1, L], [0, 0], [L, L]):
+        n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, run()))
+        assert all(not bool(out[0][b].any()) for b in range(2) if lengths[b] == 0)
+
+
 def test_calls_on_two_streams_at_once():
     w1, b1, w2 = together_weights()
     inputs = [together_inputs(s, 200) for s in range(2)]
