@@ -17,10 +17,12 @@
 // (rows r, r + 1 and those 32, 64, 96 further), so that the scattered words
 // reach memory as whole sectors.
 //
-// Bound by memory: 65536 x 5120, quantised and back, float32 239 and 236 us
-// (6.4 TB/s), bfloat16 mxfp4 150 and 150 us (5.6 TB/s); bfloat16 nvfp4, with
-// twice the scales and quotients by steps that are no powers of two, 178 us
-// (4.8 TB/s, bound by issue).  Loading a chunk ahead changed none of them.
+// Bound by memory: 65536 x 5120, quantised and back, float32 233 and 236 us
+// (6.5 TB/s), bfloat16 mxfp4 145 and 150 us (5.7 TB/s); bfloat16 nvfp4, with
+// twice the scales and quotients by steps that are no powers of two, 168 us
+// (5.1 TB/s, bound by issue; 178 us without the two-lane float instructions).
+// Loading a chunk ahead changed none of them.
+#include "icsa_attn_common.cuh"
 #include "icsa_lowp.cuh"
 
 #include <cuda_fp16.h>
@@ -91,10 +93,12 @@ ICSA_DEV void store16x2(void* p, const Words8& r) {
 }
 
 // Elements [c0 + 16 lane, + 16) of a row of K (zeros from column K on); called
-// by whole warps.
+// by whole warps.  Returns their largest magnitude as float32 bits: NaN and
+// infinity stay above every number.  (Elements of 16 bits are compared in pairs.)
 template <typename T, int ALIGN>
-ICSA_DEV void load16(const T* row, int c0, int lane, int K, float* stage, float (&v)[16]) {
+ICSA_DEV uint32_t load16(const T* row, int c0, int lane, int K, float* stage, float (&v)[16]) {
   const int k0 = c0 + 16 * lane;
+  uint32_t top = 0u;
   if constexpr (ALIGN > 0) {
     if (k0 + 16 <= K) {
 #pragma unroll
@@ -106,15 +110,17 @@ ICSA_DEV void load16(const T* row, int c0, int lane, int K, float* stage, float 
           if constexpr (sizeof(T) == 2) {
             v[2 * i] = __uint_as_float(r.w[i] << 16);
             v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+            top = __vmaxu2(top, r.w[i] & 0x7FFF7FFFu);
           } else {
             v[8 * h + i] = __uint_as_float(r.w[i]);
+            top = max(top, r.w[i] & 0x7FFFFFFFu);
           }
         }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = k0 + i < K ? to_float<T>(row[k0 + i]) : 0.f;
+      return sizeof(T) == 2 ? max(top << 16, top & 0xFFFF0000u) : top;
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = k0 + i < K ? to_float<T>(row[k0 + i]) : 0.f;
   } else {
     __syncwarp();
 #pragma unroll
@@ -126,6 +132,9 @@ ICSA_DEV void load16(const T* row, int c0, int lane, int K, float* stage, float 
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = stage[17 * lane + i];
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return top;
 }
 
 template <typename T, int ALIGN>
@@ -218,8 +227,8 @@ ICSA_DEV int tile_row(int cta, int warp) {
 // float x is no closer to it than a relative 2^-33.  Such steps are those of
 // a global scale that is a power of two; others divide, as do blocks beyond
 // the largest scale, whose quotients might overflow.  Two operations an
-// element instead of a division: 65536 x 5120 bfloat16 178 us, with the
-// divisions (a global scale of 0.9) 268 us.
+// element instead of a division: 65536 x 5120 bfloat16 168 us, with the
+// divisions (a global scale of 0.9) 258 us.
 ICSA_DEV bool short_step(float d) { return (__float_as_uint(d) & 0xFFFFu) == 0u; }
 ICSA_DEV void quotient_codes(const float (&v)[16], float amax, float d, uint32_t (&code)[2]) {
   float q[16];
@@ -228,30 +237,17 @@ ICSA_DEV void quotient_codes(const float (&v)[16], float amax, float d, uint32_t
     asm("rcp.approx.f32 %0, %1;" : "=f"(rh) : "f"(d));  // any value near 1 / d: rl is what it lacks
     const float rl = fmaf(-d, rh, 1.0f) * rh;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = fmaf(v[i], rh, v[i] * rl);
+    for (int i = 0; i < 16; i += 2) {
+      float a, b;
+      attn::fmul2(a, b, v[i], v[i + 1], rl, rl);
+      attn::ffma2(q[i], q[i + 1], v[i], v[i + 1], rh, rh, a, b);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) q[i] = __fdiv_rn(v[i], d);
   }
   code[0] = e2m1x8(q);
   code[1] = e2m1x8(q + 8);
-}
-
-// Largest magnitude of 16 elements as float32 bits: NaN and infinity stay
-// above every number.  Elements of 16 bits are compared in pairs.
-template <typename T>
-ICSA_DEV uint32_t top_bits(const float (&v)[16]) {
-  uint32_t top = 0;
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      top = __vmaxu2(top, __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632) & 0x7FFF7FFFu);
-    return max(top << 16, top & 0xFFFF0000u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    return top;
-  }
 }
 
 template <typename T, int FMT, int ALIGN>
@@ -274,13 +270,13 @@ __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantP
     const int k0 = c * kQChunk + lane * 16;
     if (c * kQChunk >= k_end) break;
     float v[16];
+    uint32_t top = 0u;
     if (row_ok) {
-      load16<T, ALIGN>(xrow, c * kQChunk, lane, p.K, stage, v);
+      top = load16<T, ALIGN>(xrow, c * kQChunk, lane, p.K, stage, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.f;
     }
-    uint32_t top = top_bits<T>(v);
     uint32_t code[2] = {0u, 0u};
     uint32_t sbyte;
     if (FMT == ICSA_NVFP4) {
@@ -301,7 +297,7 @@ __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantP
         const float inv = __uint_as_float(uint32_t(127 - e) << 23);  // 2^-e, exact products
         float q[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = v[i] * inv;
+        for (int i = 0; i < 16; i += 2) attn::fmul2(q[i], q[i + 1], v[i], v[i + 1], inv, inv);
         code[0] = e2m1x8(q);
         code[1] = e2m1x8(q + 8);
       }
