@@ -34,9 +34,10 @@
 // Long caches are split over CTAs (and over the warps of a CTA); partial
 // results (unnormalised O, m, sum) are joined in a fixed order.
 //
-// Bound by memory while one group of 8 rows reads a cache head: one query, 2 x
-// 40 heads x 32760 keys, D = 128, 104 us (587 MB, 5.6 TB/s); more groups by
-// the conversion of the codes (16 rows 212 us).  Joining in order with one
+// A CTA takes one group of 8 query rows, or two, which share the conversion
+// of the codes (16 a clock and SM, which bounds anything beyond 8 rows).
+// One query, 2 x 40 heads x 32760 keys, D = 128: 103 us (587 MB, 5.7 TB/s);
+// 16 rows 122 us, 48 rows 341 us.  Joining in order with one
 // part loaded after the other cost 5 us of 16 for 1 x 8 heads x 8000 keys;
 // eight at a time, and launched while the parts are computed, 11 us in all.
 //
@@ -57,7 +58,8 @@ namespace {
 
 constexpr int kTokens = 64;
 constexpr int kDWarps = 4;           // warps of a decode CTA
-constexpr int decode_ctas(int D) { return D == 128 ? 2 : 3; }  // that fit an SM, by their registers
+// CTAs of NQ groups of 8 rows that fit an SM, by their registers
+constexpr int decode_ctas(int D, int NQ) { return D == 128 || NQ == 2 ? 2 : 3; }
 constexpr float kNegInf = -INFINITY;
 
 ICSA_DEV int valid_tokens(const Kv8Cache& c, int b) {
@@ -355,8 +357,8 @@ ICSA_DEV float scale_log2(float s) { return s != s ? s : float(int(__float_as_ui
 
 // Rows of the 8-query tile blockIdx.z of (b, cache head): row r is query
 // token r / group, head h * group + r % group.
-template <int D>
-__global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kernel(const Kv8AttnParams p, const Kv8Cache c) {
+template <int D, int NQ>
+__global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_kernel(const Kv8AttnParams p, const Kv8Cache c) {
   constexpr int kHalves = D / 64;            // 64-byte halves of a key row
   constexpr int kSteps = D / 16;             // 16-feature steps of S
   constexpr int kOTiles = D / 16;            // 16-feature tiles of O^T
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kerne
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x, bh = blockIdx.y, b = bh / c.H, h = bh % c.H;
-  const int rows = p.Lq * p.group, row0 = blockIdx.z * 8;
+  const int rows = p.Lq * p.group, row0 = blockIdx.z * 8 * NQ;
   const int len = valid_tokens(c, b);
   const int nb = (len + kTokens - 1) / kTokens;
   const int blk0 = int(int64_t(nb) * split / p.splits), blk1 = int(int64_t(nb) * (split + 1) / p.splits);
@@ -373,18 +375,19 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kerne
     return p.q + int64_t(b) * p.q_sb + int64_t(r / p.group) * p.q_st + int64_t(h * p.group + r % p.group) * p.q_sh;
   };
   // Q^T operand: query row g, features 64 hf + 16 t + 4 j + {0,1 | 2,3} for step 4 hf + j
-  uint32_t qf[kSteps][2];
-  float q_scale;
-  {
+  uint32_t qf[NQ][kSteps][2];
+  float q_scale[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
     uint32_t raw[kHalves][8];
-    const bool ok = row0 + g < rows;
+    const bool ok = row0 + 8 * n + g < rows;
     uint32_t top = 0;
 #pragma unroll
     for (int hf = 0; hf < kHalves; ++hf) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (ok) u = __ldg(reinterpret_cast<const uint4*>(q_row(row0 + g) + 64 * hf + 16 * t) + i);
+        if (ok) u = __ldg(reinterpret_cast<const uint4*>(q_row(row0 + 8 * n + g) + 64 * hf + 16 * t) + i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) raw[hf][4 * i + k] = word(u, k);
       }
@@ -398,24 +401,28 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kerne
     // an infinity makes all its scores NaN
     const int e = min(max(int(top >> 7) - 127 - 14, -126), 126);
     const float inv = __uint_as_float(uint32_t(127 - e) << 23);
-    q_scale = top >= 0x7F80u ? __uint_as_float(0x7FC00000u) : __uint_as_float(uint32_t(127 + e) << 23);
+    q_scale[n] = top >= 0x7F80u ? __uint_as_float(0x7FC00000u) : __uint_as_float(uint32_t(127 + e) << 23);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t w = raw[s >> 2][2 * (s & 3) + i];
-        qf[s][i] = pack_f16x2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xFFFF0000u) * inv);
+        qf[n][s][i] = pack_f16x2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xFFFF0000u) * inv);
       }
   }
   // columns 2 t, 2 t + 1 of this thread's accumulators
-  float qs[2];
+  float qs[NQ][2], o[NQ][kOTiles][4], m[NQ][2], l[NQ][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) qs[i] = __shfl_sync(0xffffffffu, q_scale, (2 * t + i) * 4) * p.scale_log2;
-
-  float o[kOTiles][4];
+  for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-  for (int i = 0; i < kOTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+    for (int i = 0; i < 2; ++i) {
+      qs[n][i] = __shfl_sync(0xffffffffu, q_scale[n], (2 * t + i) * 4) * p.scale_log2;
+      m[n][i] = kNegInf;
+      l[n][i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kOTiles; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+  }
 
   const size_t slot0 = size_t(bh) * c.nb;
   // key row of S row (tile i, row r): 16 (r' / 2) + 4 i + r' % 2, + 2 for rows r = r' + 8
@@ -435,60 +442,78 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kerne
         for (int hf = 0; hf < kHalves; ++hf) kr[i][r][hf] = load_stream16(kp + (4 * i + 2 * r) * D + 64 * hf);
     const float ks = c.k_scale[slot0 + blk], lv = scale_log2(c.v_scale[slot0 + blk]);
     uint4 vr[kOTiles][2];
+    const auto load_values = [&]() {
 #pragma unroll
-    for (int i = 0; i < kOTiles; ++i)
+      for (int i = 0; i < kOTiles; ++i)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) vr[i][r] = load_stream16(vp + (16 * i + 8 * r) * kTokens);
+        for (int r = 0; r < 2; ++r) vr[i][r] = load_stream16(vp + (16 * i + 8 * r) * kTokens);
+    };
+    // one group of rows: the read is what counts, both loads at once; two
+    // groups leave no registers for that
+    if (NQ == 1) load_values();
 
-    float s[4][4];
+    float s[NQ][4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.f;
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
         const uint32_t w0 = word(kr[i][0][st >> 2], st & 3), w1 = word(kr[i][1][st >> 2], st & 3);
-        mma_f16(s[i], e4m3x2_f16x2(uint16_t(w0)), e4m3x2_f16x2(uint16_t(w1)), e4m3x2_f16x2(uint16_t(w0 >> 16)),
-                e4m3x2_f16x2(uint16_t(w1 >> 16)), qf[st][0], qf[st][1]);
+        const uint32_t a0 = e4m3x2_f16x2(uint16_t(w0)), a1 = e4m3x2_f16x2(uint16_t(w1));
+        const uint32_t a2 = e4m3x2_f16x2(uint16_t(w0 >> 16)), a3 = e4m3x2_f16x2(uint16_t(w1 >> 16));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) mma_f16(s[n][i], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
       }
     }
+    if (NQ > 1) load_values();
     const int left = len - blk * kTokens;  // valid tokens of this block
-    float mx[2] = {kNegInf, kNegInf};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // rows g (e < 2) and g + 8, columns 2 t + (e & 1)
-        float x = s[i][e] * (qs[e & 1] * ks) + lv;
-        if (left < kTokens && key_g + 4 * i + 2 * (e >> 1) >= left) x = kNegInf;
-        s[i][e] = x;
-        mx[e & 1] = fmaxf(mx[e & 1], x);
-      }
-    float neg[2], a[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int d = 4; d < 32; d *= 2) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
-      const float mn = fmaxf(m[i], mx[i]);
-      const float ref = mn == kNegInf ? 0.f : mn;
-      a[i] = attn::ex2(m[i] - ref);
-      m[i] = mn;
-      neg[i] = -ref;
-    }
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] = attn::ex2(s[i][e] + neg[e & 1]);
-        sum[e & 1] += s[i][e];
-      }
     const float wl = attn::ex2(-lv);
+    uint32_t pb[NQ][4][2];  // P^T operands
 #pragma unroll
-    for (int i = 0; i < 2; ++i) l[i] = l[i] * a[i] + sum[i] * wl;
+    for (int n = 0; n < NQ; ++n) {
+      float mx[2] = {kNegInf, kNegInf};
 #pragma unroll
-    for (int i = 0; i < kOTiles; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] *= a[e & 1];
+        for (int e = 0; e < 4; ++e) {
+          // rows g (e < 2) and g + 8, columns 2 t + (e & 1)
+          float x = s[n][i][e] * (qs[n][e & 1] * ks) + lv;
+          if (left < kTokens && key_g + 4 * i + 2 * (e >> 1) >= left) x = kNegInf;
+          s[n][i][e] = x;
+          mx[e & 1] = fmaxf(mx[e & 1], x);
+        }
+      float neg[2], a[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
+        const float mn = fmaxf(m[n][i], mx[i]);
+        const float ref = mn == kNegInf ? 0.f : mn;
+        a[i] = attn::ex2(m[n][i] - ref);
+        m[n][i] = mn;
+        neg[i] = -ref;
+      }
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][i][e] = attn::ex2(s[n][i][e] + neg[e & 1]);
+          sum[e & 1] += s[n][i][e];
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) l[n][i] = l[n][i] * a[i] + sum[i] * wl;
+#pragma unroll
+      for (int i = 0; i < kOTiles; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][i][e] *= a[e & 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pb[n][i][0] = transpose8x8(pack_f16x2(s[n][i][0], s[n][i][1]));
+        pb[n][i][1] = transpose8x8(pack_f16x2(s[n][i][2], s[n][i][3]));
+      }
+    }
     if (left < kTokens) {
       // a probability of zero does not hide a NaN code
 #pragma unroll
@@ -498,38 +523,43 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D)) kv8_decode_kerne
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t b0 = transpose8x8(pack_f16x2(s[i][0], s[i][1]));
-      const uint32_t b1 = transpose8x8(pack_f16x2(s[i][2], s[i][3]));
 #pragma unroll
       for (int d = 0; d < kOTiles; ++d) {
         const uint32_t w0 = word(vr[d][0], i), w1 = word(vr[d][1], i);
-        mma_f16(o[d], e4m3x2_f16x2(uint16_t(w0)), e4m3x2_f16x2(uint16_t(w1)), e4m3x2_f16x2(uint16_t(w0 >> 16)),
-                e4m3x2_f16x2(uint16_t(w1 >> 16)), b0, b1);
+        const uint32_t a0 = e4m3x2_f16x2(uint16_t(w0)), a1 = e4m3x2_f16x2(uint16_t(w1));
+        const uint32_t a2 = e4m3x2_f16x2(uint16_t(w0 >> 16)), a3 = e4m3x2_f16x2(uint16_t(w1 >> 16));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) mma_f16(o[n][d], a0, a1, a2, a3, pb[n][i][0], pb[n][i][1]);
       }
     }
   }
   // the threads of a column hold different keys: join their sums (m is equal)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int n = 0; n < NQ; ++n)
 #pragma unroll
-    for (int d = 4; d < 32; d *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
 
   // join the warps: [warp][column][feature]
-  __shared__ float so[kDWarps][8][D + 4];
-  __shared__ float sm[kDWarps][8], sl[kDWarps][8];
+  __shared__ float so[kDWarps][8 * NQ][D + 4];
+  __shared__ float sm[kDWarps][8 * NQ], sl[kDWarps][8 * NQ];
 #pragma unroll
-  for (int d = 0; d < kOTiles; ++d)
+  for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) so[warp][2 * t + (e & 1)][16 * d + g + 8 * (e >> 1)] = o[d][e];
-  if (g == 0) {
+    for (int d = 0; d < kOTiles; ++d)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sm[warp][2 * t + i] = m[i];
-      sl[warp][2 * t + i] = l[i];
+      for (int e = 0; e < 4; ++e) so[warp][8 * n + 2 * t + (e & 1)][16 * d + g + 8 * (e >> 1)] = o[n][d][e];
+    if (g == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sm[warp][8 * n + 2 * t + i] = m[n][i];
+        sl[warp][8 * n + 2 * t + i] = l[n][i];
+      }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 8 * D; i += kDWarps * 32) {
+  for (int i = threadIdx.x; i < 8 * NQ * D; i += kDWarps * 32) {
     const int col = i / D, d = i % D, r = row0 + col;
     if (r >= rows) break;
     float mm = kNegInf;
@@ -622,27 +652,34 @@ cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out
 }
 
 Kv8DecodePlan kv8_decode_plan(int B, int H, int rows, int L, int D, int num_sms) {
-  const int64_t ctas = int64_t(B) * H * ((rows + 7) / 8), slots = int64_t(num_sms) * decode_ctas(D);
-  const int64_t nb = (L + kTokens - 1) / kTokens;
+  const int64_t nb = (int64_t(L) + kTokens - 1) / kTokens;
   // Waves of CTAs times the steps of a warp, two steps' time for a CTA's start
   // and its part of the join; a split keeps at least one block for each warp.
-  // 2 x 40 heads x 32760 tokens, D = 128, 16 query rows: one split (160 CTAs
-  // on 296 places) 284 us, seven 232 us; D = 64, one row: three (two to an
-  // SM) 83 us, eleven 69 us.
-  const int64_t most = std::min<int64_t>(nb / kDWarps, 32);
-  Kv8DecodePlan best = {1, 0.0};
-  for (int64_t s = 1; s <= std::max<int64_t>(most, 1); ++s) {
-    const double steps = double((ctas * s + slots - 1) / slots) * (double(nb) / double(s * kDWarps) + 2.0);
-    if (s == 1 || steps < best.steps) best = {int(s), steps};
+  // 2 x 40 heads x 32760 tokens, D = 64, one row: three splits (two CTAs to an
+  // SM) 83 us, eleven 69 us.  One or two groups of 8 rows a CTA, us: D = 128, 2 x
+  // 40 x 32000, 16 rows 208 / 122, 48 rows 569 / 341; 1 x 8 x 2000, 64 rows
+  // 15 / 17; D = 64, 2 x 40 x 32000, 48 rows 300 / 224.
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(nb / kDWarps, 32));
+  Kv8DecodePlan best = {1, 1, 0.0};
+  for (int groups = 1; groups <= (rows > 8 ? 2 : 1); ++groups) {
+    const int64_t ctas = int64_t(B) * H * ((rows + 8 * groups - 1) / (8 * groups));
+    const int64_t slots = int64_t(num_sms) * decode_ctas(D, groups);
+    const double step = groups == 1 ? (D == 128 ? 2.4 : 1.5) : (D == 128 ? 3.2 : 1.8);
+    for (int64_t s = 1; s <= most; ++s) {
+      const double us = double((ctas * s + slots - 1) / slots) * (double(nb) / double(s * kDWarps) + 2.0) * step +
+                        (s > 1 ? 6.0 : 4.0);
+      if (best.us == 0.0 || us < best.us) best = {int(s), groups, us};
+    }
   }
   return best;
 }
 
 cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream) {
   const int rows = p.Lq * p.group;
-  const dim3 grid(p.splits, c.B * c.H, (rows + 7) / 8);
-  if (c.D == 128) kv8_decode_kernel<128><<<grid, kDWarps * 32, 0, stream>>>(p, c);
-  else kv8_decode_kernel<64><<<grid, kDWarps * 32, 0, stream>>>(p, c);
+  const dim3 grid(p.splits, c.B * c.H, (rows + 8 * p.groups - 1) / (8 * p.groups));
+  const auto kernel = c.D == 128 ? (p.groups == 2 ? kv8_decode_kernel<128, 2> : kv8_decode_kernel<128, 1>)
+                                 : (p.groups == 2 ? kv8_decode_kernel<64, 2> : kv8_decode_kernel<64, 1>);
+  kernel<<<grid, kDWarps * 32, 0, stream>>>(p, c);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;
   const dim3 jgrid(rows, c.B * c.H);

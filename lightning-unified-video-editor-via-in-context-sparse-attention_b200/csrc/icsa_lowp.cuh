@@ -112,12 +112,13 @@ struct Kv8AttnParams {
   __nv_bfloat16* out;      // [B, Lq, Hq, D] contiguous
   int Lq, Hq, group;       // group = Hq / H
   float scale_log2;
-  int splits;
+  int splits, groups;
   float* partial;          // [rows, splits, D + 2] when splits > 1
 };
 struct Kv8DecodePlan {
   int splits;
-  double steps;            // its time, in steps of a warp (one block each)
+  int groups;              // of 8 rows a CTA
+  double us;               // estimated time
 };
 Kv8DecodePlan kv8_decode_plan(int B, int H, int rows, int L, int D, int num_sms);
 cudaError_t launch_kv8_decode(const Kv8AttnParams& p, const Kv8Cache& c, cudaStream_t stream);

@@ -200,15 +200,15 @@ enum AttnPath { kDecode, kPairs, kDense };
 
 struct AttnPlan {
   AttnPath path;
-  int splits;            // kDecode
+  int splits, groups;            // kDecode
   icsa::Kv8TcPlan tc;    // kPairs
   size_t v_offset;       // kDense: bf16 copy of the values, behind that of the keys
   size_t bytes;          // workspace
 };
 
 // Estimated times of the three ways to attend, us.
-//  * The register-fed kernel (decode) reads the cache once for every 8 rows;
-//    2.6 us (D = 64: 1.7) for the four blocks of a step of its warps.
+//  * The register-fed kernel (decode) reads the cache once for every 8 or 16
+//    rows (kv8_decode_plan).
 //  * The pair kernel deals its steps evenly to all SM pairs, 2.7 us (2.0) for
 //    a step of two 256-row tiles and 1.8 us (1.65) for one; where rounds are
 //    cut their parts are joined, the more the fewer rounds there are.
@@ -218,11 +218,12 @@ struct AttnPlan {
 //    element).  Their probabilities are bf16, so few rows do without them.
 // Constants fitted to 324 sizes (1, 8 and 2 x 40 heads, D = 64 and 128, 100 to
 // 32000 keys, 16 to 4096 rows): the choice is within 1 % of the best of the
-// three on average, at worst a quarter slower.  Measured, us, decode / pairs /
-// dense, D = 128: 1 x 8 heads, 8000 keys, 64 rows 23 / 37 / 67, 512 rows 121 /
-// 47 / 67, 4096 rows - / 159 / 128; 2 x 40 heads, 300 keys, 48 rows 21 / 25 /
-// 29, 256 rows 86 / 25 / 29; 32000 keys, 16 rows 216 / 591 / 757, 1024 rows
-// 12653 / 1559 / 1542, 2048 rows - / 2799 / 2387.
+// three on average, at worst a third slower.  Measured, us, decode / pairs /
+// dense, D = 128: 1 x 8 heads, 8000 keys, 64 rows 21 / 37 / 67, 512 rows 72 /
+// 47 / 67, 4096 rows - / 159 / 128; 2 x 40 heads, 600 keys, 48 rows 19 / 33 /
+// 33, 256 rows 82 / 40 / 33; 32000 keys, 16 rows 122 / 569 / 740, 48 rows 341 /
+// 555 / 734, 128 rows 909 / 550 / 749, 1024 rows - / 1559 / 1542, 2048 rows -
+// / 2799 / 2387.
 constexpr int kNoCopyRows = 48, kDecodeMost = 8 * 65535;
 double dense_us(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   const bool wide = c.D == 128;
@@ -244,10 +245,6 @@ double pairs_us(const icsa::Kv8Cache& c, const icsa::Kv8TcPlan& t, int sms) {
   const double head = (t.tiles / 2) * two + (t.tiles & 1) * one;
   return 27.4 + 0.19 * std::max(1.0, clusters / (heads * t.rounds)) + heads * steps * head / clusters;
 }
-double decode_us(const icsa::Kv8Cache& c, const icsa::Kv8DecodePlan& d) {
-  return 4.0 + d.steps * (c.D == 128 ? 2.6 : 1.7) + (d.splits > 1 ? 2.0 : 0.0);
-}
-
 AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   AttnPlan a = {};
   const int64_t rows = int64_t(Lq) * (Hq / c.H);
@@ -257,10 +254,11 @@ AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   double us = pairs_us(c, a.tc, sms);
   if (rows <= kDecodeMost) {
     const icsa::Kv8DecodePlan d = icsa::kv8_decode_plan(c.B, c.H, int(rows), c.L, c.D, sms);
-    if (decode_us(c, d) < us) {
-      us = decode_us(c, d);
+    if (d.us < us) {
+      us = d.us;
       a.path = kDecode;
       a.splits = d.splits;
+      a.groups = d.groups;
       a.bytes = a.splits == 1 ? 0 : align256(size_t(c.B) * c.H * rows * a.splits * (c.D + 2) * sizeof(float));
     }
   }
@@ -478,6 +476,7 @@ int icsa_kv8_attention(const icsa_kv8_cache* cache, const void* q, const int64_t
     p.Lq = Lq; p.Hq = Hq; p.group = Hq / c.H;
     p.scale_log2 = scale_log2;
     p.splits = plan.splits;
+    p.groups = plan.groups;
     p.partial = static_cast<float*>(workspace);
     cudaError_t e = icsa::launch_kv8_decode(p, c, stream);
     return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "kv8_attention");

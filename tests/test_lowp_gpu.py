@@ -312,7 +312,8 @@ def check_attention(q, cache, lengths=None, k=None, v=None):
     # no box of queries holds; more sequences than a launch takes; many splits
     (3, 700, 900, 2, 3, [0, 900, 65]), (1, 60, 9000, 2, 1, [8777]), (2, 20, 5000, 3, 5, [4999, 129]),
     (1, 130, 6000, 1, 3, None), (130, 49, 70, 1, 1, list(range(-30, 100))), (129, 51, 1100, 1, 1, None),
-    (1, 1, 32000, 1, 2, None),
+    (1, 1, 32000, 1, 2, None), (2, 9, 3000, 40, 1, [3000, 1]), (2, 16, 700, 40, 1, None), (1, 37, 5000, 8, 1, [4990]),
+    (1, 5, 6000, 16, 5, None),
     # SM pairs: one step, shared heads, an odd number of tiles, rounds cut between clusters; then the bf16 copy
     (2, 300, 100, 16, 1, [100, 37]), (2, 40, 120, 4, 8, None), (4, 100, 331, 8, 3, [331, 0, 5, 331]),
     (3, 70, 500, 16, 5, None), (2, 700, 331, 16, 1, [331, 200]), (1, 512, 8000, 8, 1, [7900]),
