@@ -63,12 +63,12 @@ struct Fp4GemmParams {
   int activation;
   __nv_bfloat16* out;          // [M, ldo]
   int64_t ldo;
-  float* partial;              // [splits, M, n_pad] when splits > 1
+  float* partial;              // [splits, M, n_pad] when splits > 1 (launch_fp4_rows: parts of tiles)
   int n_pad;
-  int splits;
+  int splits;                  // of K (launch_fp4_rows: 1 whole tiles, 2 cut ones)
   int m_tiles, n_tiles, units, k_steps;
-  int tma_out;                 // the output's rows are 16-byte aligned: written by TMA
-  int w_ready;                 // the kernel before this one in the stream did not write w
+  int tma_out;                 // the output's rows are 16-byte aligned: written by TMA (launch_fp4_gemm)
+  int w_ready;                 // the kernel before this one in the stream did not write w (launch_fp4_rows)
 };
 // Splits of K for an M x N x K product on `num_sms` SMs (1: none).
 int fp4_gemm_splits(int M, int N, int K, int num_sms);
