@@ -25,19 +25,24 @@
 // Both products run in f16 with float32 accumulation: e4m3 codes are exact in
 // f16, a query row is scaled by a power of two to [2^14, 2^15) (bf16 has 8
 // significant bits, f16 11; only elements 2^-28 below the row's largest lose
-// bits), and the probabilities have 11 bits (below 2^-14 of the largest they
-// are multiples of 2^-24 of it).  The scale of a value block
-// joins the exponent: with s the base-2 scores and v the log2 of the scale,
-//   p = 2^(s + v - m),  m the running maximum of s + v,
-// p enters the product with the codes, and 2^-v p the row sum.
+// bits), and the probabilities have 11 bits (those below 2^-14 of the row's
+// largest at least are multiples of 2^-24 of it).  With s the base-2 scores, m
+// their running maximum and v the log2 of a value block's scale,
+//   P = 2^(s - m + d),  d = v - R,  O = 2^R sum P code,  l = sum 2^-d P:
+// the block's scale enters P against the reference R, and d in [0, 15] keeps P
+// within f16 and every bit that p = 2^(s - m) has there.  A block outside that
+// window moves R and rescales O (see value_spread); O is float32, so what one
+// block's values are does not cost another block bits.  (With the scale in the
+// maximum instead, m the largest s + v, a block of zeros, whose scale is 1,
+// takes the bits of the small values beside it.)
 //
 // Long caches are split over CTAs (and over the warps of a CTA); partial
-// results (unnormalised O, m, sum) are joined in a fixed order.
+// results (O / l, m, l) are joined in a fixed order.
 //
 // A CTA takes one group of 8 query rows, or two, which share the conversion
 // of the codes (16 a clock and SM, which bounds anything beyond 8 rows).
 // One query, 2 x 40 heads x 32760 keys, D = 128: 103 us (587 MB, 5.7 TB/s);
-// 16 rows 122 us, 48 rows 341 us.  Joining in order with one
+// 16 rows 130 us, 48 rows 361 us.  Joining in order with one
 // part loaded after the other cost 5 us of 16 for 1 x 8 heads x 8000 keys;
 // eight at a time, and launched while the parts are computed, 11 us in all.
 //
@@ -58,9 +63,11 @@ namespace {
 
 constexpr int kTokens = 64;
 constexpr int kDWarps = 4;           // warps of a decode CTA
+constexpr int kMaxSplits = 32;       // of the keys over CTAs
 // CTAs of NQ groups of 8 rows that fit an SM, by their registers
 constexpr int decode_ctas(int D, int NQ) { return D == 128 || NQ == 2 ? 2 : 3; }
 constexpr float kNegInf = -INFINITY;
+constexpr float kWindow = 15.f;      // most of d = v - R: P up to 2^15 is in f16's range
 
 ICSA_DEV int valid_tokens(const Kv8Cache& c, int b) {
   return c.lengths == nullptr ? c.L : min(max(c.lengths[b], 0), c.L);
@@ -355,8 +362,8 @@ ICSA_DEV uint4 keep_bytes(uint4 u, int n) {
 // exponent of a power of two as a float; NaN stays NaN
 ICSA_DEV float scale_log2(float s) { return s != s ? s : float(int(__float_as_uint(s) >> 23) - 127); }
 
-// Rows of the 8-query tile blockIdx.z of (b, cache head): row r is query
-// token r / group, head h * group + r % group.
+// The 8 NQ rows blockIdx.z of (b, cache head): row r is query token r / group,
+// head h * group + r % group.
 template <int D, int NQ>
 __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_kernel(const Kv8AttnParams p, const Kv8Cache c) {
   constexpr int kHalves = D / 64;            // 64-byte halves of a key row
@@ -412,6 +419,12 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
   }
   // columns 2 t, 2 t + 1 of this thread's accumulators
   float qs[NQ][2], o[NQ][kOTiles][4], m[NQ][2], l[NQ][2];
+  // R (the same in all lanes; below any v, so that the first block sets it), and
+  // for the rare moves an upper bound of the v so far
+  float ref_v = -1000.f;
+  __shared__ float top_v[kDWarps];
+  if (lane == 0) top_v[warp] = -1000.f;
+  __syncwarp();
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
 #pragma unroll
@@ -430,7 +443,34 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
   const uint8_t* kbase = c.k + slot0 * kTokens * D + key_g * D + 16 * t;
   const uint8_t* vbase = c.v + slot0 * kTokens * D + g * kTokens + 16 * t;
 
+  const auto move_reference = [&](float lv) {
+    if (lv < ref_v || lv > ref_v + kWindow) {
+      // (8 binades more than the spread: p is at most 1 here)
+      const float top = fmaxf(fmaxf(top_v[warp], ref_v + kWindow), lv);
+      const float r = fmaxf(lv - 8.f, top - value_spread(len) - 8.f), f = attn::ex2(ref_v - r);
+      __syncwarp();
+      if (lane == 0) top_v[warp] = top;
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < kOTiles; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
+      ref_v = r;
+    }
+  };
+  // two groups: the scale comes a block ahead, and R moves before the loads
+  // (after the scores it cost 8 us of 131 for 2 x 40 heads, 16 rows); one
+  // group: after the scores, where the loads hide it
+  float vs = NQ > 1 && blk0 + warp < blk1 ? c.v_scale[slot0 + blk0 + warp] : 1.f;
   for (int blk = blk0 + warp; blk < blk1; blk += kDWarps) {
+    float lv = 0.f;
+    if constexpr (NQ > 1) {
+      lv = scale_log2(vs);
+      if (blk + kDWarps < blk1) vs = c.v_scale[slot0 + blk + kDWarps];
+      move_reference(lv);
+    }
     const uint8_t* kp = kbase + size_t(blk) * kTokens * D;
     const uint8_t* vp = vbase + size_t(blk) * kTokens * D;
     uint4 kr[4][2][kHalves];
@@ -440,7 +480,8 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int hf = 0; hf < kHalves; ++hf) kr[i][r][hf] = load_stream16(kp + (4 * i + 2 * r) * D + 64 * hf);
-    const float ks = c.k_scale[slot0 + blk], lv = scale_log2(c.v_scale[slot0 + blk]);
+    const float ks = c.k_scale[slot0 + blk];
+    if constexpr (NQ == 1) lv = scale_log2(c.v_scale[slot0 + blk]);
     uint4 vr[kOTiles][2];
     const auto load_values = [&]() {
 #pragma unroll
@@ -468,7 +509,8 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
     }
     if (NQ > 1) load_values();
     const int left = len - blk * kTokens;  // valid tokens of this block
-    const float wl = attn::ex2(-lv);
+    if constexpr (NQ == 1) move_reference(lv);
+    const float dv = lv - ref_v, wl = attn::ex2(-dv);
     uint32_t pb[NQ][4][2];  // P^T operands
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -478,7 +520,7 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           // rows g (e < 2) and g + 8, columns 2 t + (e & 1)
-          float x = s[n][i][e] * (qs[n][e & 1] * ks) + lv;
+          float x = s[n][i][e] * (qs[n][e & 1] * ks);
           if (left < kTokens && key_g + 4 * i + 2 * (e >> 1) >= left) x = kNegInf;
           s[n][i][e] = x;
           mx[e & 1] = fmaxf(mx[e & 1], x);
@@ -492,7 +534,7 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
         const float ref = mn == kNegInf ? 0.f : mn;
         a[i] = attn::ex2(m[n][i] - ref);
         m[n][i] = mn;
-        neg[i] = -ref;
+        neg[i] = dv - ref;
       }
       float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -541,15 +583,21 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
 
-  // join the warps: [warp][column][feature]
+  // join the warps: O / l in the values' own unit, [warp][column][feature] (a
+  // warp without a key has l = 0 and O = 0)
+  const float unit = attn::ex2(ref_v);
   __shared__ float so[kDWarps][8 * NQ][D + 4];
   __shared__ float sm[kDWarps][8 * NQ], sl[kDWarps][8 * NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
+    float inv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) inv[i] = l[n][i] == 0.f ? 0.f : 1.0f / l[n][i];
 #pragma unroll
     for (int d = 0; d < kOTiles; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) so[warp][8 * n + 2 * t + (e & 1)][16 * d + g + 8 * (e >> 1)] = o[n][d][e];
+      for (int e = 0; e < 4; ++e)
+        so[warp][8 * n + 2 * t + (e & 1)][16 * d + g + 8 * (e >> 1)] = o[n][d][e] * inv[e & 1] * unit;
     if (g == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -566,19 +614,22 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
 #pragma unroll
     for (int w = 0; w < kDWarps; ++w) mm = fmaxf(mm, sm[w][col]);
     const float ref = mm == kNegInf ? 0.f : mm;
-    float acc = 0.f, lt = 0.f;
+    float f[kDWarps], lt = 0.f;
 #pragma unroll
     for (int w = 0; w < kDWarps; ++w) {
-      const float f = attn::ex2(sm[w][col] - ref);
-      acc += so[w][col][d] * f;
-      lt += sl[w][col] * f;
+      f[w] = sl[w][col] * attn::ex2(sm[w][col] - ref);
+      lt += f[w];
     }
+    // the warps' shares of the sum: a weighted mean, which no value overflows
+    const float inv = lt == 0.f && blk0 == blk1 ? 0.f : 1.0f / lt;
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDWarps; ++w) y += so[w][col][d] * (f[w] * inv);
     if (p.splits == 1) {
-      const float y = len == 0 ? 0.f : acc / lt;
       p.out[((size_t(b) * p.Lq + r / p.group) * p.Hq + h * p.group + r % p.group) * D + d] = __float2bfloat16_rn(y);
     } else {
       float* dst = p.partial + ((size_t(bh) * rows + r) * p.splits + split) * (D + 2);
-      dst[d] = acc;
+      dst[d] = y;
       if (d == 0) {
         dst[D] = mm;
         dst[D + 1] = lt;
@@ -587,40 +638,36 @@ __global__ void __launch_bounds__(kDWarps * 32, decode_ctas(D, NQ)) kv8_decode_k
   }
 }
 
-// joins the splits of one query row; one CTA per (b, cache head, row)
+// joins the splits of one query row, at most kMaxSplits; one CTA per (b, cache
+// head, row).  Every lane takes one split's weight l 2^(m - max m).
 template <int D>
 __global__ void __launch_bounds__(D) kv8_join_kernel(const Kv8AttnParams p, const Kv8Cache c) {
+  static_assert(kMaxSplits == 32, "a lane for each split");
   const int rows = p.Lq * p.group;
-  const int r = blockIdx.x, bh = blockIdx.y, b = bh / c.H, h = bh % c.H, d = threadIdx.x;
+  const int r = blockIdx.x, bh = blockIdx.y, b = bh / c.H, h = bh % c.H, d = threadIdx.x, lane = threadIdx.x & 31;
   wait_prior_grid();
   const float* src = p.partial + (size_t(bh) * rows + r) * p.splits * (D + 2);
-  float mm = kNegInf, acc = 0.f, lt = 0.f;
   constexpr int kAhead = 8;  // splits whose loads are on their way together
+  float x[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) x[i] = i < p.splits ? src[i * (D + 2) + d] : 0.f;
+  const float m = lane < p.splits ? src[lane * (D + 2) + D] : kNegInf;
+  float w = lane < p.splits ? src[lane * (D + 2) + D + 1] : 0.f;
+  float top = m;
+#pragma unroll
+  for (int i = 16; i > 0; i /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+  w *= attn::ex2(m - (top == kNegInf ? 0.f : top));
+  float total = w;
+#pragma unroll
+  for (int i = 16; i > 0; i /= 2) total += __shfl_xor_sync(0xffffffffu, total, i);
+  w *= valid_tokens(c, b) == 0 ? 0.f : 1.0f / total;
+  float y = 0.f;
   for (int s0 = 0; s0 < p.splits; s0 += kAhead) {
-    float x[kAhead], m[kAhead], l[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const float* part = src + (s0 + i) * (D + 2);
-      const bool in = s0 + i < p.splits;
-      x[i] = in ? part[d] : 0.f;
-      m[i] = in ? part[D] : kNegInf;
-      l[i] = in ? part[D + 1] : 0.f;
-    }
-    float top = mm;
+    for (int i = 0; i < kAhead; ++i) y += x[i] * __shfl_sync(0xffffffffu, w, s0 + i);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) top = fmaxf(top, m[i]);
-    const float ref = top == kNegInf ? 0.f : top, f = attn::ex2(mm - ref);
-    acc *= f;
-    lt *= f;
-    mm = top;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const float g = attn::ex2(m[i] - ref);
-      acc += x[i] * g;
-      lt += l[i] * g;
-    }
+    for (int i = 0; i < kAhead; ++i) x[i] = s0 + kAhead + i < p.splits ? src[(s0 + kAhead + i) * (D + 2) + d] : 0.f;
   }
-  const float y = valid_tokens(c, b) == 0 ? 0.f : acc / lt;
   p.out[((size_t(b) * p.Lq + r / p.group) * p.Hq + h * p.group + r % p.group) * D + d] = __float2bfloat16_rn(y);
 }
 
@@ -657,9 +704,9 @@ Kv8DecodePlan kv8_decode_plan(int B, int H, int rows, int L, int D, int num_sms)
   // and its part of the join; a split keeps at least one block for each warp.
   // 2 x 40 heads x 32760 tokens, D = 64, one row: three splits (two CTAs to an
   // SM) 83 us, eleven 69 us.  One or two groups of 8 rows a CTA, us: D = 128, 2 x
-  // 40 x 32000, 16 rows 208 / 122, 48 rows 569 / 341; 1 x 8 x 2000, 64 rows
+  // 40 x 32000, 16 rows 208 / 130, 48 rows 569 / 361; 1 x 8 x 2000, 64 rows
   // 15 / 17; D = 64, 2 x 40 x 32000, 48 rows 300 / 224.
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(nb / kDWarps, 32));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(nb / kDWarps, kMaxSplits));
   Kv8DecodePlan best = {1, 1, 0.0};
   for (int groups = 1; groups <= (rows > 8 ? 2 : 1); ++groups) {
     const int64_t ctas = int64_t(B) * H * ((rows + 8 * groups - 1) / (8 * groups));

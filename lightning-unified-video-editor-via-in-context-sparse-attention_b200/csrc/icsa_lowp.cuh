@@ -102,6 +102,12 @@ struct Kv8Rows {
   const void* x[2];    // k, v: [B, L, H, D], features contiguous
   int64_t sb[2], st[2], sh[2];
 };
+// The attention kernels hold O in units of 2^R, R a reference that follows the
+// scales of the value blocks.  It stays within 2^-value_spread of the largest
+// scale so far, so that O < keys x 2^8 x 448 x 2^spread stays below 2^127;
+// blocks whose scale lies further below (95 binades at 16384 keys) lose bits of
+// their probabilities.
+__device__ __forceinline__ float value_spread(int keys) { return float(78 + __clz(keys)); }
 cudaError_t launch_kv8_quantize(const Kv8Rows& x, int dtype, const Kv8Cache& c, cudaStream_t stream);
 // out[i]: [B, L, H, D] contiguous of out_dtype; rows behind a length are zero
 cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out_dtype, cudaStream_t stream);

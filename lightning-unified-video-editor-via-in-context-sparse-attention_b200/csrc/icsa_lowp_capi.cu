@@ -221,7 +221,7 @@ struct AttnPlan {
 // three on average, at worst a third slower.  Measured, us, decode / pairs /
 // dense, D = 128: 1 x 8 heads, 8000 keys, 64 rows 21 / 37 / 67, 512 rows 72 /
 // 47 / 67, 4096 rows - / 159 / 128; 2 x 40 heads, 600 keys, 48 rows 19 / 33 /
-// 33, 256 rows 82 / 40 / 33; 32000 keys, 16 rows 122 / 569 / 740, 48 rows 341 /
+// 33, 256 rows 82 / 40 / 33; 32000 keys, 16 rows 130 / 569 / 740, 48 rows 361 /
 // 555 / 734, 128 rows 909 / 550 / 749, 1024 rows - / 1559 / 1542, 2048 rows -
 // / 2799 / 2387.
 constexpr int kNoCopyRows = 48, kDecodeMost = 8 * 65535;
