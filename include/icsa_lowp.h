@@ -125,8 +125,11 @@ ICSA_API int icsa_kv8_dequantize(const icsa_kv8_cache* cache, void* k_out, void*
  * h' = h / (Hq / H), len = lengths[b]; zero where len is 0.  Replaces the
  * reference's flash_attention call (wanx/attention.py:18-85, with its k_lens)
  * for keys and values that are kept over many calls.  float32 scores, softmax
- * and accumulation; the probabilities enter the second product as fp16, and
- * as bf16 for many queries over a long cache; one rounding of the result.
+ * and accumulation; the probabilities p enter the second product as fp16 (off
+ * by 2^-11 of themselves, below 2^-14 of the row's largest by 2^-25 of that
+ * one, whatever the scales of the value blocks, as long as these lie within
+ * 2^80 of each other), and as bf16 (2^-8) for many queries over a long cache;
+ * one rounding of the result.
  *   q: bf16 [B, Lq, Hq, D] with batch, token, head strides (multiples of 8
  *   elements, 16-byte aligned), contiguous features; Hq a multiple of H.
  *   (ICSA_ERR_UNSUPPORTED for many queries over a long cache whose heads are

@@ -4,14 +4,20 @@
 // takes them in rounds of two 256-row tiles, each CTA 128 rows of a tile.
 //
 //   S = Q K^T            bf16 (e4m3 codes are exact in bf16)
-//   x = S ks c + lv      ks: the key block's scale, c = log2(e) / sqrt(D),
-//                        lv: log2 of the value block's scale
-//   p = 2^(x - m)        m: running maximum of x, raised when x exceeds it by 8
-//   l += p 2^-lv,  O += p V8      p and the value codes in f16
-//   out = O / l
+//   x = S ks c           ks: the key block's scale, c = log2(e) / sqrt(D)
+//   P = 2^(x - m + d)    m: running maximum of x, raised when x exceeds it by 8;
+//                        d = lv - R, lv: log2 of the value block's scale
+//   l += P 2^-d,  O += P V8       P and the value codes in f16
+//   out = 2^R O / l
 //
 // so the cache's bytes enter the products as they are and its scales cost one
-// fused multiply-add that the exponent needs anyway; p keeps 11 bits.
+// fused multiply-add that the exponent needs anyway.  The reference R is one
+// for all rows and keeps d in [0, 7], P within f16: P has every bit there that
+// p = 2^(x - m) has.  Blocks outside the window move R, and O with it.  Where a
+// step's two blocks lie further apart than the window, its P.V runs in two
+// parts, the other block's probabilities zero and R moved in between.  (With
+// the scale in the maximum instead, m the largest x + lv, a block of zeros,
+// whose scale is 1, takes the bits of the small values beside it.)
 //
 // Per step of 128 keys each CTA converts its half of the pair's operands from
 // the cache (64 keys x D, and D / 2 features x 128 tokens; the cache keeps
@@ -28,7 +34,7 @@
 //
 // Work is dealt to the clusters in step space by the lengths on the device:
 // equal numbers of steps each, whole rounds where all steps fit the ring,
-// else rounds cut at the cluster boundaries, whose parts (unnormalised O, m,
+// else rounds cut at the cluster boundaries, whose parts (2^R O / l, m,
 // l) a second kernel joins in a fixed order.
 //
 // Roles per CTA (512 threads):
@@ -36,11 +42,12 @@
 //   warps 8-11        cache conversion, epilogue
 //   warps 12, 14      in the leader, the issuers of S and of P.V; TMEM allocation (12)
 //   warp 13           query loads (TMA, or copies where a box cannot hold whole tokens)
+//   warp 15           the scales: R, d and the factors of each step, for the softmax
 // Every wait is bounded (about one second).
 //
-// 2 x 40 heads, D = 128: 32760 queries over 512 keys 683 us (1.0 PFLOP/s; the
-// bf16 rate would be 426 us), 256 over 32760 602 us, of which filling the
-// stages is the larger part.  In whole rounds a unit (a step of one tile)
+// 2 x 40 heads, D = 128: 32760 queries over 512 keys 635 to 680 us with the
+// clock (1.0 PFLOP/s; the bf16 rate would be 426 us), 256 over 32000 540 us, of
+// which filling the stages is the larger part.  In whole rounds a unit (a step of one tile)
 // takes 1930 clk against 1049 of its products and 1024 of its exponentials:
 // with the softmax's arithmetic left out it still takes 1500, the round trip
 // of the one S buffer (product, read, next product), and a softmax warpgroup
@@ -62,7 +69,7 @@ namespace {
 using namespace attn;
 
 constexpr int kThreads = 512;
-constexpr int kIssuerWarp = 12, kQueryWarp = 13, kPvWarp = 14;
+constexpr int kIssuerWarp = 12, kQueryWarp = 13, kPvWarp = 14, kScaleWarp = 15;
 constexpr int kPairRows = 256, kCtaRows = 128;
 constexpr int kStepKeys = 128;
 constexpr int kMaxBatch = kKv8TcMaxBatch;
@@ -70,7 +77,8 @@ constexpr uint32_t kTmP = 128, kTmO = 256, kTmemCols = 512;
 
 enum : int {
   kErrKvFull = 0x501, kErrKvEmpty = 0x502, kErrQFull = 0x503, kErrQEmpty = 0x504, kErrSFull = 0x505, kErrSFree = 0x506,
-  kErrPFull = 0x507, kErrPvDone = 0x508, kErrOFull = 0x509, kErrOFree = 0x50A, kErrMlFull = 0x50B, kErrMlFree = 0x50C
+  kErrPFull = 0x507, kErrPvDone = 0x508, kErrOFull = 0x509, kErrOFree = 0x50A, kErrMlFull = 0x50B, kErrMlFree = 0x50C,
+  kErrUnitFull = 0x50D, kErrUnitEmpty = 0x50E, kErrXFull = 0x50F, kErrXDone = 0x510
 };
 
 template <int D>
@@ -90,6 +98,16 @@ struct Range {
   int first, last;  // steps cut off the first and the last round
 };
 
+// What the softmax needs of a step's scales, in chunks of kChunk units of a slot.
+constexpr int kChunk = 32;
+struct __align__(16) Unit {
+  float c0, c1;          // base-2 score of a product, for the step's first and second block
+  float d0, d1;          // lv - R
+  float w0, w1;          // 2^-d
+  float ref0, ref1;      // R; where the two differ the step's P.V runs in two parts
+  uint32_t stage, pad[3];  // the step's place in the ring of stages, counted on
+};
+
 template <int D>
 struct __align__(1024) Smem {
   using C = Cfg<D>;
@@ -97,7 +115,10 @@ struct __align__(1024) Smem {
   uint8_t kv[C::kStages][C::kKBytes + C::kVBytes];  // [keys | values]
   uint8_t out[4][32 * 128];                         // output box of each helper warp
   Range ranges[kMaxBatch];
-  float ml[2][2][kCtaRows];                         // [slot][m, l] of a finished tile
+  float ml[2][3][kCtaRows];                         // [slot][m, 2^-R l, 2^R] of a finished tile
+  Unit units[2][2][kChunk];                         // [slot][buffer]
+  uint32_t any_two[2][2];                         // whether a chunk has units that run in two parts
+  uint64_t unit_full[2][2], unit_empty[2][2], x_full[2], x_done[2];
   uint64_t kv_full[C::kStages], kv_empty[C::kStages];
   uint64_t q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2], pv_done[2], o_full[2], o_free[2];
   uint64_t ml_full[2], ml_free[2];
@@ -226,6 +247,11 @@ ICSA_DEV bool new_kv(const Kv8TcParams& p, const Round& a, const Round& before) 
 // step of the round's only tile.
 ICSA_DEV bool has_tile(const Kv8TcParams& p, const Round& w, int s) { return 2 * w.r + s < p.tiles; }
 ICSA_DEV bool alternate(const Kv8TcParams& p, const Round& w) { return !has_tile(p, w, 1); }
+// What a slot's chunk of units in whole rounds depends on: rounds of the same
+// kind follow each other and share it.
+ICSA_DEV int unit_kind(const Kv8TcParams& p, const Kv8Cache& c, const Round& w) {
+  return 2 * (w.b * c.H + w.h) + int(alternate(p, w));
+}
 ICSA_DEV int slot_steps(const Kv8TcParams& p, const Round& w, int s) {
   return alternate(p, w) ? (w.steps() + 1 - s) >> 1 : w.steps();
 }
@@ -419,14 +445,20 @@ ICSA_DEV void copy_queries(const Kv8TcParams& p, const Round& w, int tile, uint3
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// A tile's partial result, [D + 2][256 rows] (O, then m and l): the rows, which
-// lie across the lanes, are innermost.
+// A tile's partial result, [D + 2][256 rows] (2^R O / l, then m and l): the
+// rows, which lie across the lanes, are innermost.
 ICSA_DEV float* partial_tile(const Kv8TcParams& p, int cluster, int part, int slot, int D) {
   return p.partial + (size_t(cluster * 2 + part) * 2 + slot) * kPairRows * (D + 2);
 }
 // behind the parts: where each cluster's range starts
 ICSA_DEV int4* cluster_starts(const Kv8TcParams& p, int clusters, int D) {
   return reinterpret_cast<int4*>(p.partial + size_t(clusters) * 4 * kPairRows * (D + 2));
+}
+
+ICSA_DEV float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // O of a tile (of both slots where they took the steps in turn) to the
@@ -438,10 +470,20 @@ ICSA_DEV void epilogue(const Kv8TcParams& p, const Kv8TcMaps& maps, const Round&
   const int row = quad * 32 + lane;
   const uint32_t o0 = tmem + (uint32_t(quad * 32) << 16) + kTmO + 128u * uint32_t(slot), o1 = o0 + 128u;
   const float ma = sm.ml[slot][0][row], la = sm.ml[slot][1][row];
-  const float mb = two ? sm.ml[1][0][row] : -INFINITY, lb = two ? sm.ml[1][1][row] : 0.f;
-  const float m = fmaxf(ma, mb), ref = m == -INFINITY ? 0.f : m;
-  float fa = two ? ex2(ma - ref) : 1.f, fb = two ? ex2(mb - ref) : 0.f;
-  const float l = two ? la * fa + lb * fb : la;
+  float m = ma, l = 1.f, fa = reciprocal(la), fb = 0.f;
+  if (two) {
+    // each slot's part of the row sum
+    const float mb = sm.ml[1][0][row], lb = sm.ml[1][1][row];
+    m = fmaxf(ma, mb);
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float wa = la * sm.ml[slot][2][row] * ex2(ma - ref), wb = lb * sm.ml[1][2][row] * ex2(mb - ref);
+    l = wa + wb;
+    const float inv = reciprocal(l);
+    fa *= wa * inv;
+    fb = wb * inv * reciprocal(lb);
+  } else if (w.part >= 0) {
+    l = la * sm.ml[slot][2][row];
+  }
   const int tile = 2 * w.r + slot;
   const int tile_row = int(rank) * kCtaRows + row, r = tile * kPairRows + tile_row;
   const bool ok = r < p.rows;
@@ -452,9 +494,6 @@ ICSA_DEV void epilogue(const Kv8TcParams& p, const Kv8TcMaps& maps, const Round&
   __nv_bfloat16* out = nullptr;
   if (w.part >= 0) part = partial_tile(p, blockIdx.x >> 1, w.part, slot, D) + tile_row;
   else if (!p.o_tma) out = p.out + ((size_t(w.b) * p.Lq + token) * p.Hq + w.h * p.group + (r - token * p.group)) * D;
-  const float inv = part != nullptr ? 1.f : 1.0f / l;
-  fa *= inv;
-  fb *= inv;
 #pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
     uint32_t x[32];
@@ -464,7 +503,8 @@ ICSA_DEV void epilogue(const Kv8TcParams& p, const Kv8TcMaps& maps, const Round&
       tc::tmem_ld32(o1 + 32u * uint32_t(c), y);
       tc::tmem_wait_ld();
 #pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fa + __uint_as_float(y[e]) * fb);
+      for (int e = 0; e < 32; ++e)
+        x[e] = __float_as_uint(__uint_as_float(x[e]) * fa + __uint_as_float(y[e]) * fb);
     } else {
       tc::tmem_wait_ld();
 #pragma unroll
@@ -657,6 +697,118 @@ ICSA_DEV void load_queries(const Kv8TcParams& p, const Kv8TcMaps& maps, const Kv
   }
 }
 
+// ------------------------------------------------------------ scales (warp) --
+// exponent of a power of two; NaN stays NaN
+ICSA_DEV float exponent(float s) { return s != s ? s : float(int(__float_as_uint(s) >> 23) - 127); }
+constexpr float kWindow = 7.f;  // most of d = lv - R: P up to 2^15 with the 2^8 of the lazy maximum
+
+// R of a slot, moved as little as the window allows.
+struct Reference {
+  float r = 0.f, top = -1000.f;  // R, and the largest lv of the round so far
+  // scales lo to hi, no further apart than the window
+  ICSA_DEV void cover(float lo, float hi, float spread) {
+    top = fmaxf(top, hi);
+    if (lo < r || hi > r + kWindow) r = fmaxf(lo - floorf(0.5f * (kWindow - (hi - lo))), top - spread);
+  }
+};
+
+// The units of every slot, a unit for each lane: where a chunk's scales fit the
+// window one R serves it (nearly always), else R goes from unit to unit, and
+// where it has to move between the blocks of a step, that step runs in two
+// parts.  Both CTAs of a pair come to the same R, as they read the same scales.
+// (A NaN scale moves nothing and makes its row NaN.)  Done by the softmax and
+// the issuer themselves it took 606 us instead of 545 for 2 x 40 heads, 256 over
+// 32000, and 738 instead of 635 for the text.
+template <int D>
+ICSA_DEV void prepare_units(const Kv8TcParams& p, const Kv8Cache& c, Smem<D>& sm) {
+  const int lane = threadIdx.x & 31;
+  uint32_t count0 = 0, count1 = 0;  // chunks of each slot
+  uint32_t kv_base = 0, kv_next = 0;  // stages, as the issuers count them
+  int kind0 = -1, kind1 = -1;
+  Reference ref0, ref1;
+  Walk walk(sm.ranges);
+  Round w, before;
+  before.b = -1;
+  while (walk.next(p, c, w)) {
+    if (new_kv(p, w, before)) {
+      kv_base = kv_next;
+      kv_next += uint32_t(w.steps());
+    }
+    before = w;
+    const size_t slot0 = (size_t(w.b) * c.H + w.h) * c.nb;
+    const float spread = value_spread(w.len);
+    const bool alt = alternate(p, w);
+    const int nbl = (w.len + 63) >> 6, most = slot_steps(p, w, 0);  // (slot 1 has no more)
+    ref0.top = ref1.top = -1000.f;
+#pragma unroll 1
+    for (int q = 0; q < 2 * most; ++q) {
+      // chunk q / 2 of slot q & 1
+      const int s = q & 1, k0 = (q >> 1) * kChunk, n = slot_steps(p, w, s);
+      if (k0 >= most) break;
+      if (k0 >= n) continue;
+      if (p.whole) {
+        const int kind = unit_kind(p, c, w);
+        if (kind == (s ? kind1 : kind0)) continue;
+        if (s) kind1 = kind;
+        else kind0 = kind;
+      }
+      const int k = k0 + lane, j = w.n0 + (alt ? s + 2 * k : k);
+      float ks0 = 0.f, ks1 = 0.f, e0 = __uint_as_float(0x7FC00000u), e1 = e0;
+      if (k < n) {
+        const int b0 = 2 * j, b1 = min(2 * j + 1, nbl - 1);  // (a block behind the length has no key)
+        ks0 = __ldg(c.k_scale + slot0 + b0);
+        ks1 = __ldg(c.k_scale + slot0 + b1);
+        e0 = exponent(__ldg(c.v_scale + slot0 + b0));
+        e1 = exponent(__ldg(c.v_scale + slot0 + b1));
+      }
+      // (fminf and fmaxf pass over a NaN)
+      const float lo = float(__reduce_min_sync(0xffffffffu, int(fminf(fminf(e0, e1), 1000.f))));
+      const float hi = float(__reduce_max_sync(0xffffffffu, int(fmaxf(fmaxf(e0, e1), -1000.f))));
+      Reference ref = s ? ref1 : ref0;
+      float r0, r1;
+      const bool calm = hi - lo <= kWindow;
+      if (calm) {
+        ref.cover(lo, hi, spread);
+        r0 = r1 = ref.r;
+      } else {
+        r0 = r1 = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < min(kChunk, n - k0); ++i) {
+          const float a0 = __shfl_sync(0xffffffffu, e0, i), a1 = __shfl_sync(0xffffffffu, e1, i);
+          const float lo1 = fminf(a0, a1), hi1 = fmaxf(a0, a1);
+          float first;
+          if (hi1 - lo1 > kWindow) {
+            ref.top = fmaxf(ref.top, hi1);
+            first = fmaxf(a0 - 4.f, ref.top - spread);
+            ref.r = fmaxf(a1 - 4.f, ref.top - spread);
+          } else {
+            ref.cover(lo1, hi1, spread);
+            first = ref.r;
+          }
+          if (lane == i) {
+            r0 = first;
+            r1 = ref.r;
+          }
+        }
+      }
+      if (s) ref1 = ref;
+      else ref0 = ref;
+      const uint32_t count = s ? count1++ : count0++;
+      const int buf = int(count & 1u);
+      if (!warp_mbar_wait(&sm.unit_empty[s][buf], ((count >> 1) & 1u) ^ 1u, nullptr, kErrUnitEmpty, &sm.abort_flag)) return;
+      const float d0 = e0 - r0, d1 = e1 - r1;
+      float4* u = reinterpret_cast<float4*>(&sm.units[s][buf][lane]);
+      u[0] = make_float4(p.scale_log2 * ks0, p.scale_log2 * ks1, d0, d1);
+      u[1] = make_float4(ex2(-d0), ex2(-d1), r0, r1);
+      if (lane == 0) sm.any_two[s][buf] = calm ? 0u : 1u;
+      sm.units[s][buf][lane].stage = kv_base + uint32_t(j - w.n0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.unit_full[s][buf]);
+      __syncwarp();
+    }
+  }
+}
+
 // ----------------------------------------------------------------- issuer --
 template <int D, int KK>
 constexpr uint32_t kQOff = uint32_t(((KK >> 2) * (kCtaRows * 128) + (KK & 3) * 32) >> 4);
@@ -787,13 +939,20 @@ ICSA_DEV void exp_half(float* s, float c, float off, float& l0, float& l1, float
     fadd2(l2, l3, l2, l3, s[e + 2], s[e + 3]);
   }
 }
-ICSA_DEV void store_half(uint32_t taddr, const float* s) {
+ICSA_DEV uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+ICSA_DEV void store_p(uint32_t taddr, const float* s) {
   uint32_t pk[32];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
-    const __half2 v = __floats2half2_rn(s[2 * e], s[2 * e + 1]);
-    pk[e] = *reinterpret_cast<const uint32_t*>(&v);
-  }
+  for (int e = 0; e < 32; ++e) pk[e] = pack_f16x2(s[2 * e], s[2 * e + 1]);
+  tc::tmem_st32(taddr, pk);
+}
+ICSA_DEV void store_zeros(uint32_t taddr) {
+  uint32_t pk[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) pk[e] = 0u;
   tc::tmem_st32(taddr, pk);
 }
 ICSA_DEV float max64(const float* s) {
@@ -806,124 +965,234 @@ ICSA_DEV float max64(const float* s) {
     for (int i = 0; i < 4; ++i) t[i] = fmax3(t[i], s[e + i], s[e + 4 + i]);
   return fmax3(fmaxf(t[0], t[1]), t[2], t[3]);
 }
-// exponent of a power of two; NaN stays NaN
-ICSA_DEV float exponent(float s) { return s != s ? s : float(int(__float_as_uint(s) >> 23) - 127); }
-
-// the scales of a step's two blocks (a block behind the length has no key)
-struct StepScales {
-  float ks0, ks1, vs0, vs1;
-  ICSA_DEV void load(const float* k_scale, const float* v_scale, int j, int nbl) {
-    const int b0 = 2 * j, b1 = min(2 * j + 1, nbl - 1);
-    ks0 = __ldg(k_scale + b0);
-    ks1 = __ldg(k_scale + b1);
-    vs0 = __ldg(v_scale + b0);
-    vs1 = __ldg(v_scale + b1);
-  }
-};
-
+// O of this thread's row times 2^shift
 template <int D>
-ICSA_DEV void softmax(const Kv8TcParams& p, const Kv8Cache& c, int slot, uint32_t rank, Smem<D>& sm, uint32_t tmem) {
-  volatile int* abort_flag = &sm.abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = threadIdx.x & 127;
-  const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-  const uint32_t s_base = tmem + lanes;
-  const uint32_t p_base = tmem + lanes + kTmP + 64u * uint32_t(slot);
-  const uint32_t o_base = tmem + lanes + kTmO + 128u * uint32_t(slot);
-  const uint32_t s_free = pair::mapa(&sm.s_free[slot], 0);
-  const uint32_t p_full = pair::mapa(&sm.p_full[slot], 0);
-  const float sl2 = p.scale_log2;
-  uint32_t count = 0, tiles = 0;
-  Walk walk(sm.ranges);
-  Round w;
-  while (walk.next(p, c, w)) {
-    const int n = slot_steps(p, w, slot);
-    if (n == 0) continue;
-    const bool alt = alternate(p, w);
-    const int stride = alt ? 2 : 1;
-    int j = w.n0 + (alt ? slot : 0);
-    // rows of this warp behind the last one need no exponentials
-    const int tile = 2 * w.r + (alt ? 0 : slot);
-    const bool any_row = tile * kPairRows + int(rank) * kCtaRows + (warp & 3) * 32 < p.rows;
-    const size_t slot0 = (size_t(w.b) * c.H + w.h) * c.nb;
-    const float *k_scale = c.k_scale + slot0, *v_scale = c.v_scale + slot0;
-    const int nbl = (w.len + 63) >> 6;
-    float m = -INFINITY, l = 0.f;
-    StepScales sc;
-    sc.load(k_scale, v_scale, j, nbl);
-    for (int k = 0; k < n; ++k, ++count, j += stride) {
-      warp_mbar_wait(&sm.s_full[slot], count & 1u, nullptr, kErrSFull, abort_flag);
-      tc::fence_after_sync();
-      float s[128];
-      tmem_load_row128(s_base, s);
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) pair::arrive_cluster_relaxed(s_free);
-      __syncwarp();
-      const float c0 = sl2 * sc.ks0, c1 = sl2 * sc.ks1;
-      const float lv0 = exponent(sc.vs0), lv1 = exponent(sc.vs1);
-      if (k + 1 < n) sc.load(k_scale, v_scale, j + stride, nbl);
-      float alpha = 1.f, n0 = 0.f, n1 = 0.f;
-      float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-      bool need = false;
-      if (any_row) {
-        const int hi = w.len - j * kStepKeys;  // valid keys of the step
-        if (hi < kStepKeys) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (e >= hi) s[e] = -INFINITY;
-        }
-        const float top = fmaxf(fmaf(max64(s), c0, lv0), fmaf(max64(s + 64), c1, lv1));
-        need = top - m > kRescaleThreshold;
-        if (need) {
-          alpha = m == -INFINITY ? 0.f : ex2(m - top);
-          l *= alpha;
-          m = top;
-        }
-        n0 = lv0 - m;
-        n1 = lv1 - m;
-        exp_half(s, c0, n0, a0, a1, a2, a3);
-        l += ((a0 + a1) + (a2 + a3)) * ex2(-lv0);
-        a0 = a1 = a2 = a3 = 0.f;
-        exp_half(s + 64, c1, n1, a0, a1, a2, a3);
-        l += ((a0 + a1) + (a2 + a3)) * ex2(-lv1);
-      }
-      // P and O of this slot were last used by its previous P.V
-      if (count > 0) {
-        warp_mbar_wait(&sm.pv_done[slot], (count - 1) & 1u, nullptr, kErrPvDone, abort_flag);
-        tc::fence_after_sync();
-      }
-      if (any_row) {
-        store_half(p_base, s);
-        store_half(p_base + 32u, s + 64);
-      }
-      if (k > 0 && __any_sync(0xffffffffu, need)) {
+ICSA_DEV void rescale(uint32_t o_base, float shift) {
+  const float alpha = ex2(shift);
 #pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t r[32];
-          tc::tmem_ld32(o_base + 32u * uint32_t(q), r);
-          tc::tmem_wait_ld();
+  for (int q = 0; q < D / 32; ++q) {
+    uint32_t r[32];
+    tc::tmem_ld32(o_base + 32u * uint32_t(q), r);
+    tc::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-          tc::tmem_st32(o_base + 32u * uint32_t(q), r);
-        }
-      }
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) pair::arrive_cluster_relaxed(p_full);
-      __syncwarp();
-    }
-    // the helper has read the last tile's statistics
-    warp_mbar_wait(&sm.ml_free[slot], (tiles & 1u) ^ 1u, nullptr, kErrMlFree, abort_flag);
-    ++tiles;
-    sm.ml[slot][0][row] = m;
-    sm.ml[slot][1][row] = l;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.ml_full[slot]);
-    __syncwarp();
+    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+    tc::tmem_st32(o_base + 32u * uint32_t(q), r);
   }
 }
+
+// The softmax of one slot: a warpgroup, a thread for each row.
+template <int D>
+struct Softmax {
+  Smem<D>& sm;
+  uint32_t tmem, rank;
+  int slot;
+  uint32_t count = 0, extra = 0;  // units, and of them those in two parts
+  uint32_t tiles = 0;
+  float m = 0.f, l = 0.f;         // of this thread's row
+  float ref_v = 0.f;              // R (the same in all rows)
+  uint32_t s_free = pair::mapa(&sm.s_free[slot], 0), p_full = pair::mapa(&sm.p_full[slot], 0);
+
+  ICSA_DEV uint32_t lanes() const { return uint32_t(((threadIdx.x >> 5) & 3) * 32) << 16; }
+  ICSA_DEV uint32_t p_base() const { return tmem + lanes() + kTmP + 64u * uint32_t(slot); }
+  ICSA_DEV uint32_t o_base() const { return tmem + lanes() + kTmO + 128u * uint32_t(slot); }
+  ICSA_DEV bool wait(uint64_t* bar, uint32_t phase, int code) {
+    return warp_mbar_wait(bar, phase & 1u, nullptr, code, &sm.abort_flag);
+  }
+  // P and O are written: tells the leader's barrier
+  ICSA_DEV void give(uint32_t bar) {
+    tc::tmem_wait_st();
+    tc::fence_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) pair::arrive_cluster_relaxed(bar);
+    __syncwarp();
+  }
+
+  // Unit k of the round, of which `left` keys are valid.  TWO: its chunk has
+  // units that run in two parts.
+  template <bool TWO>
+  ICSA_DEV void step(const Unit& unit, int k, int left, bool any_row) {
+    const float4 cd = *reinterpret_cast<const float4*>(&unit.c0), wr = *reinterpret_cast<const float4*>(&unit.w0);
+    wait(&sm.s_full[slot], count, kErrSFull);
+    tc::fence_after_sync();
+    float s[128];
+    tmem_load_row128(tmem + lanes(), s);
+    tc::fence_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) pair::arrive_cluster_relaxed(s_free);
+    __syncwarp();
+    float shift = ref_v - wr.z;
+    ref_v = wr.w;
+    bool need = shift != 0.f;  // O is to be multiplied by 2^shift: R's move and the maximum's rise in one exponent
+    if (any_row) {
+      if (left < kStepKeys) {
+#pragma unroll
+        for (int e = 0; e < 128; ++e)
+          if (e >= left) s[e] = -INFINITY;
+      }
+      const float top = fmaxf(max64(s) * cd.x, max64(s + 64) * cd.y);
+      if (top - m > kRescaleThreshold) {
+        if (m > -INFINITY) {
+          l *= ex2(m - top);
+          shift += m - top;
+        }
+        m = top;
+        need = true;
+      }
+      float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+      exp_half(s, cd.x, cd.z - m, a0, a1, a2, a3);
+      l += ((a0 + a1) + (a2 + a3)) * wr.x;
+      a0 = a1 = a2 = a3 = 0.f;
+      exp_half(s + 64, cd.y, cd.w - m, a0, a1, a2, a3);
+      l += ((a0 + a1) + (a2 + a3)) * wr.y;
+    }
+    // P and O of this slot were last used by its previous P.V
+    if constexpr (!TWO) {
+      wait_pv();
+      if (any_row) {
+        store_p(p_base(), s);
+        store_p(p_base() + 32u, s + 64);
+      }
+      if (k > 0 && __any_sync(0xffffffffu, need)) rescale<D>(o_base(), shift);
+      give(p_full);
+    } else {
+      uint32_t pk[64];
+#pragma unroll
+      for (int e = 0; e < 64; ++e) pk[e] = pack_f16x2(s[2 * e], s[2 * e + 1]);
+      wait_pv();
+      const bool two = unit.ref0 != unit.ref1;
+      if (two) {
+        first_part(pk, unit, k, any_row, k > 0 && __any_sync(0xffffffffu, need), shift);
+        shift = unit.ref0 - unit.ref1;
+        need = true;
+        if (any_row) store_zeros(p_base());
+      } else if (any_row) {
+        tc::tmem_st32(p_base(), reinterpret_cast<const uint32_t(&)[32]>(pk[0]));
+      }
+      if (any_row) tc::tmem_st32(p_base() + 32u, reinterpret_cast<const uint32_t(&)[32]>(pk[32]));
+      if (k > 0 && __any_sync(0xffffffffu, need)) rescale<D>(o_base(), shift);
+      if (two && k == 0) join_first(shift);
+      else give(p_full);
+    }
+    ++count;
+  }
+  ICSA_DEV void wait_pv() {
+    if (count > 0) {
+      wait(&sm.pv_done[slot], count - 1, kErrPvDone);
+      tc::fence_after_sync();
+    }
+  }
+  // A step in two parts: P.V of its first block alone.  A warp of the leader's
+  // softmax issues it: the issuer, whose every instruction counts, knows
+  // nothing of it.
+  ICSA_DEV void first_part(const uint32_t (&pk)[64], const Unit& unit, int k, bool any_row, bool need, float shift) {
+    if (any_row) {
+      tc::tmem_st32(p_base(), reinterpret_cast<const uint32_t(&)[32]>(pk[0]));
+      store_zeros(p_base() + 32u);
+    }
+    if (need) rescale<D>(o_base(), shift);
+    give(pair::mapa(&sm.x_full[slot], 0));
+    if (rank == 0 && ((threadIdx.x >> 5) & 3) == 0) {
+      using C = Cfg<D>;
+      const uint32_t st = unit.stage % C::kStages;
+      bool ok = wait(&sm.x_full[slot], extra, kErrXFull) && wait(&sm.kv_full[st], unit.stage / C::kStages, kErrKvFull);
+      // (a tile's first unit: the slot's last tile has been read)
+      if (k == 0) ok = ok && wait(&sm.o_free[slot], tiles ^ 1u, kErrOFree);
+      if (ok) {
+        tc::fence_after_sync();
+        issue_pv<D>(tc::make_sw128_desc(smem_u32(sm.kv[st] + C::kKBytes), 16, 1024),
+                    tmem + kTmP + 64u * uint32_t(slot), tmem + kTmO + 128u * uint32_t(slot), k == 0 ? 0u : 1u,
+                    std::make_integer_sequence<int, 8>{});
+        pair::commit_both_elect(&sm.x_done[slot]);
+        // whatever becomes of the other waits, these products are over before the CTA ends
+        if ((threadIdx.x & 31) == 0) drain_wait(&sm.x_done[slot], extra & 1u, nullptr);
+        __syncwarp();
+      }
+    }
+    wait(&sm.x_done[slot], extra, kErrXDone);
+    tc::fence_after_sync();
+    ++extra;
+  }
+  // The issuer's P.V of a tile's first unit starts O anew: the first part is
+  // kept meanwhile (in local memory, this is rare and registers are not to be
+  // had) and added to it.
+  ICSA_DEV void join_first(float shift) {
+    uint32_t kept[D];
+#pragma unroll 1
+    for (int q = 0; q < D; q += 32) {
+      uint32_t r[32];
+      tc::tmem_ld32(o_base() + uint32_t(q), r);
+      tc::tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) kept[q + e] = r[e];
+    }
+    give(p_full);
+    wait(&sm.pv_done[slot], count, kErrPvDone);
+    tc::fence_after_sync();
+    const float alpha = ex2(shift);
+#pragma unroll 1
+    for (int q = 0; q < D; q += 32) {
+      uint32_t r[32];
+      tc::tmem_ld32(o_base() + uint32_t(q), r);
+      tc::tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(kept[q + e]) * alpha);
+      tc::tmem_st32(o_base() + uint32_t(q), r);
+    }
+    tc::tmem_wait_st();
+    tc::fence_before_sync();
+  }
+
+  ICSA_DEV void run(const Kv8TcParams& p, const Kv8Cache& c) {
+    const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
+    uint32_t chunks = 0;
+    int kind = -1;
+    Walk walk(sm.ranges);
+    Round w;
+    while (walk.next(p, c, w)) {
+      const int n = slot_steps(p, w, slot);
+      if (n == 0) continue;
+      const bool fresh = !p.whole || unit_kind(p, c, w) != kind;
+      kind = unit_kind(p, c, w);
+      const bool alt = alternate(p, w);
+      const int keys = alt ? 2 * kStepKeys : kStepKeys;  // between the slot's steps
+      int left = w.len - (w.n0 + (alt ? slot : 0)) * kStepKeys;
+      // rows of this warp behind the last one need no exponentials
+      const int tile = 2 * w.r + (alt ? 0 : slot);
+      const bool any_row = tile * kPairRows + int(rank) * kCtaRows + (row & ~31) < p.rows;
+      m = -INFINITY;
+      l = 0.f;
+      for (int k0 = 0; k0 < n; k0 += kChunk) {
+        if (fresh) {
+          // the next chunk, and the one before it is free
+          wait(&sm.unit_full[slot][chunks & 1u], chunks >> 1, kErrUnitFull);
+          __syncwarp();
+          if (chunks > 0 && lane == 0) mbar_arrive(&sm.unit_empty[slot][(chunks - 1) & 1u]);
+          __syncwarp();
+          ++chunks;
+        }
+        const int buf = int((chunks - 1) & 1u), kn = min(n - k0, kChunk);
+        const Unit* units = sm.units[slot][buf];
+        if (sm.any_two[slot][buf] == 0) {
+          for (int k = 0; k < kn; ++k) step<false>(units[k], k0 + k, left - k * keys, any_row);
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < kn; ++k) step<true>(units[k], k0 + k, left - k * keys, any_row);
+        }
+        left -= kn * keys;
+      }
+      // the helper has read the last tile's statistics
+      wait(&sm.ml_free[slot], tiles ^ 1u, kErrMlFree);
+      ++tiles;
+      sm.ml[slot][0][row] = m;
+      sm.ml[slot][1][row] = l * ex2(-ref_v);  // (O over this is the result)
+      sm.ml[slot][2][row] = ex2(ref_v);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.ml_full[slot]);
+      __syncwarp();
+    }
+  }
+};
 
 template <int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -951,6 +1220,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&sm.ml_free[i], 4);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&sm.fin[i], 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sm.unit_full[i >> 1][i & 1], 1);
+      mbar_init(&sm.unit_empty[i >> 1][i & 1], 4);  // a slot's softmax warps
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.x_full[i], 8);
+      mbar_init(&sm.x_done[i], 1);
+    }
     sm.abort_flag = 0;
     fence_mbarrier_init();
   }
@@ -968,7 +1245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // 256 x 176 + 128 x 104 + 128 x 56 = 512 x 128.
   if (warp < 8) {
     tc::reg_alloc<176>();
-    softmax<D>(p, c, warp >> 2, rank, sm, tmem);
+    Softmax<D>{sm, tmem, rank, warp >> 2}.run(p, c);
   } else if (warp < kIssuerWarp) {
     tc::reg_dealloc<104>();
     Helper<D> h{p, maps, c, sm, tmem, rank};
@@ -992,9 +1269,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (q0) drain_wait(&sm.q_full[0], (q0 - 1) & 1u, nullptr);
         if (q1) drain_wait(&sm.q_full[1], (q1 - 1) & 1u, nullptr);
       }
-    } else if (!p.whole && rank == 0 && threadIdx.x == kThreads - 32) {
+    } else if (warp == kScaleWarp) {
+      prepare_units<D>(p, c, sm);
       // for the kernel that joins the parts
-      cluster_starts(p, gridDim.x >> 1, D)[blockIdx.x >> 1] = cluster_start(p, c, blockIdx.x >> 1, gridDim.x >> 1);
+      if (!p.whole && rank == 0 && (threadIdx.x & 31) == 0)
+        cluster_starts(p, gridDim.x >> 1, D)[blockIdx.x >> 1] = cluster_start(p, c, blockIdx.x >> 1, gridDim.x >> 1);
     }
   }
   __syncwarp();
@@ -1055,17 +1334,19 @@ __global__ void __launch_bounds__(256) kv8_tc_join_kernel(const Kv8TcParams p, c
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
+      // a weighted mean, which no value overflows
       const float top = fmaxf(mm, m[i]), ref = top == -INFINITY ? 0.f : top;
-      const float f = ex2(mm - ref), g = ex2(m[i] - ref);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * f + x[i][e] * g;
-      l = l * f + lk[i] * g;
+      const float f = l * ex2(mm - ref), g = lk[i] * ex2(m[i] - ref);
+      l = f + g;
       mm = top;
+      const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * (f * inv) + x[i][e] * (g * inv);
     }
   }
   __shared__ float tile[32][D + 1];
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) tile[threadIdx.x & 31][d0 + e] = acc[e] / l;
+  for (int e = 0; e < kPer; ++e) tile[threadIdx.x & 31][d0 + e] = acc[e];
   __syncthreads();
   for (int e = threadIdx.x; e < 32 * D; e += 256) {
     const int q = row0 + e / D;

@@ -74,6 +74,9 @@ def check(q, cache, copy=None):
 # One line per path: batch, queries, keys, heads, query heads per cache head, whether it runs on the copy (at D = 128).
 PATHS = {"few rows": (2, 2, 500, 2, 1, False), "few rows, shared heads": (2, 9, 331, 2, 4, False),
          "few rows, splits": (1, 3, 9000, 2, 1, False), "two groups": (2, 16, 700, 40, 1, False),
+         "whole rounds": (2, 300, 450, 40, 1, False), "one tile": (2, 200, 450, 16, 1, False),
+         "whole rounds, two tiles": (2, 700, 331, 16, 1, False),
+         "cut rounds": (1, 512, 8000, 8, 1, False), "cut rounds, shared heads": (1, 150, 8000, 8, 3, False),
          "copy": (1, 4096, 2000, 8, 1, True)}
 
 # exponents of the 64-token blocks' values, repeated over the cache; None: a block of zeros
@@ -101,7 +104,7 @@ def test_value_blocks_of_unequal_scales_cost_no_bits(path, pattern, D):
     check(q, lowp.kv8_quantize(k.cuda(), v.cuda()), copy if D == 128 else None)
 
 
-@pytest.mark.parametrize("path", ["few rows", "few rows, splits", "copy"])
+@pytest.mark.parametrize("path", ["few rows", "few rows, splits", "whole rounds", "cut rounds", "copy"])
 def test_a_row_sees_its_own_key_beside_large_values_of_others(path):
     """Each row's probability lies on one key whose values are 2^-30 of what the other blocks hold; and an
     outlier that no row looks at sets a block's scale, its other values being zero."""
@@ -132,3 +135,20 @@ def test_probabilities_keep_the_bits_of_their_path(path, D):
     q = torch.randn(3, Lq, H * group, D, generator=g).to(torch.bfloat16).cuda()
     n = torch.tensor([L, 0, L - 77], dtype=torch.int32, device="cuda")
     check(q, lowp.kv8_quantize(k, v, n))
+
+
+def test_a_replayed_call_follows_scales_that_change():
+    """Which steps are taken in two parts is read from the cache on the device."""
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(2, 450, 40, 128, generator=g).cuda() for _ in range(2))
+    q = torch.randn(2, 300, 40, 128, generator=g).to(torch.bfloat16).cuda()
+    lowp.kv8_attention(q, lowp.kv8_quantize(k, v))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lowp.kv8_attention(q, lowp.kv8_quantize(k, v))
+    base = v.clone()
+    for pattern in ("far steps", "one large", "zeros beside 2^-20"):
+        v.copy_(base * pattern_rows(450, PATTERNS[pattern]).float().cuda()[None, :, None, None])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, check(q, lowp.kv8_quantize(k, v)))
