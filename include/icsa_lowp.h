@@ -77,13 +77,26 @@ ICSA_API int icsa_fp4_linear(int format, const void* a_data, const void* a_scale
 
 /*
  * The same for x of ICSA_BF16 or ICSA_F32 (rows ldx elements apart), which is
- * quantised to the weight's format (global scale 1) in the workspace first.
+ * quantised to the weight's format in the workspace first: by
+ * icsa_fp4_linear_rows with global scale 1, by icsa_fp4_linear_scaled_rows with
+ * a global scale for each row of x, 2^e with e the smallest with which the
+ * row's largest magnitude is at most 2688 x 2^e (in [-90, 90]; 1 for a row of
+ * zeros and one with a NaN or an infinity).  ICSA_NVFP4 scales end at 2^-9 and
+ * 448, so with scale 1 a block below 0.0059 becomes zero, below 0.09 it loses
+ * bits, and above 2688 it saturates: rows of any magnitude want their own
+ * scales.  ICSA_MXFP4 scales have the range of float; there the two are one.
  */
 ICSA_API size_t icsa_fp4_linear_rows_workspace_size(int format, int M, int N, int K);
 ICSA_API int icsa_fp4_linear_rows(int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
                                   const void* w_scales, float w_global_scale, const void* bias, int activation,
                                   void* out, int64_t ldo, int M, int N, int K, void* workspace,
                                   size_t workspace_bytes, cudaStream_t stream);
+
+ICSA_API size_t icsa_fp4_linear_scaled_rows_workspace_size(int format, int M, int N, int K);
+ICSA_API int icsa_fp4_linear_scaled_rows(int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
+                                         const void* w_scales, float w_global_scale, const void* bias, int activation,
+                                         void* out, int64_t ldo, int M, int N, int K, void* workspace,
+                                         size_t workspace_bytes, cudaStream_t stream);
 
 /*
  * Key/value cache in e4m3 with one power-of-two scale for each block of 64

@@ -6,6 +6,9 @@
 //   nvfp4: s = e4m3(amax / (6 g)), step d = s g    (g: the tensor's global scale)
 //   mxfp4: s = 2^(floor(log2 amax) - 2) (exponent in [-127, 127]), d = s
 //   code = e2m1(x / d), rounded to nearest even, largest magnitude 6; 0 where d = 0
+// or, for the rows of a linear layer, with g a power of two for each row: the
+// smallest with which the row's largest magnitude is in range (448 x 6 g), so
+// that rows of any magnitude keep the format's bits.
 // Quotients are those of IEEE float32 division, so a host computation in
 // float32 gives the same bytes.  A block that holds a NaN or an infinity gets
 // the format's NaN scale (0x7f / 0xff).
@@ -250,7 +253,22 @@ ICSA_DEV void quotient_codes(const float (&v)[16], float amax, float d, uint32_t
   code[1] = e2m1x8(q + 8);
 }
 
-template <typename T, int FMT, int ALIGN>
+// The global scale of a row whose largest magnitude has these float32 bits:
+// 2^e, e the smallest with top <= 2688 2^e = 1.3125 2^(11 + e), in [-90, 90] (as
+// quotient_codes takes them); 1 for a row of zeros, and for one with a NaN or an
+// infinity, of which the blocks without them count nothing.
+ICSA_DEV float row_scale(uint32_t top) {
+  if (top == 0u || top >= 0x7F800000u) return 1.f;
+  const int e = int(top >> 23) - 127 - 11 + ((top & 0x7FFFFFu) > 0x280000u ? 1 : 0);
+  return __uint_as_float(uint32_t(127 + min(max(e, -90), 90)) << 23);
+}
+
+// ROWS: nvfp4 with a global scale for each row.  Every warp reads its whole row
+// for the maximum first (the second time from L2, where the rows at hand fit
+// it).  A linear layer's call, us, with one scale / with the rows' own: 1 x 5120
+// -> 30720 18.6 / 22.3, 1024 x 5120 -> 10240 34.5 / 38.6, 65536 x 5120 -> 5120
+// 818 / 844, 65536 x 13824 -> 5120 2237 / 2621.
+template <typename T, int FMT, int ALIGN, bool ROWS>
 __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantParams p, int chunks_per_cta) {
   constexpr int kAtoms = FMT == ICSA_NVFP4 ? 4 : 2;
   release_next_grid();  // a linear layer sets itself up meanwhile
@@ -266,6 +284,22 @@ __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantP
   __shared__ float stages[ALIGN > 0 ? 1 : kQThreads / 32 * kStage];
   float* stage = stages + (ALIGN > 0 ? 0 : warp * kStage);
   const int c0 = blockIdx.y * chunks_per_cta;
+  float g = p.global_scale, inv_hi = p.inv_hi, inv_lo = p.inv_lo;
+  if constexpr (ROWS) {
+    uint32_t top = 0u;
+    if (row_ok) {
+#pragma unroll 4
+      for (int c = 0; c < (p.K + kQChunk - 1) / kQChunk; ++c) {
+        float v[16];
+        top = max(top, load16<T, ALIGN>(xrow, c * kQChunk, lane, p.K, stage, v));
+      }
+    }
+    g = row_scale(__reduce_max_sync(0xffffffffu, top));
+    if (row_ok && blockIdx.y == 0 && lane == 0) p.row_scales[r] = g;
+    const float inv = __uint_as_float((254u << 23) - __float_as_uint(g));  // 1 / g, an exact factor
+    inv_hi *= inv;
+    inv_lo *= inv;
+  }
   for (int c = c0; c < c0 + chunks_per_cta; ++c) {
     const int k0 = c * kQChunk + lane * 16;
     if (c * kQChunk >= k_end) break;
@@ -282,11 +316,10 @@ __global__ void __launch_bounds__(kQThreads) fp4_quantize_kernel(const Fp4QuantP
     if (FMT == ICSA_NVFP4) {
       const float amax = __uint_as_float(top);
       // (beyond 597 x 6 g the scale is 448 in any case: no product overflows)
-      const float capped = fminf(amax, 3584.f * p.global_scale);
-      const float t = p.inv_hi != 0.f ? fmaf(capped, p.inv_hi, capped * p.inv_lo)
-                                      : __fdiv_rn(amax, 6.0f * p.global_scale);
+      const float capped = fminf(amax, 3584.f * g);
+      const float t = inv_hi != 0.f ? fmaf(capped, inv_hi, capped * inv_lo) : __fdiv_rn(amax, 6.0f * g);
       sbyte = top >= 0x7F800000u ? 0x7Fu : uint32_t(__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3));
-      const float d = e4m3_float(sbyte) * p.global_scale;
+      const float d = e4m3_float(sbyte) * g;
       if (d > 0.f && top < 0x7F800000u) quotient_codes(v, amax, d, code);
     } else {
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -366,10 +399,11 @@ int row_alignment(const void* base, int64_t ld, int elem) {
 // plenty of rows, one where there are not (latency).  K = 5120, bfloat16 to
 // nvfp4, one / four chunks a CTA: 64 rows 1.7 / 3.0 us, 1024 rows 5.0 / 6.1,
 // 4096 rows 13.2 / 11.8, 8192 rows 25.4 / 22.4.
-void quant_grid(int rows, int k_elems, dim3* grid, int* chunks_per_cta) {
+void quant_grid(int rows, int k_elems, dim3* grid, int* chunks_per_cta, bool row_scales = false) {
   const int row_ctas = (rows + kFp4TileRows - 1) / kFp4TileRows * 16;
   const int chunks = (k_elems + kQChunk - 1) / kQChunk;
-  *chunks_per_cta = row_ctas >= 512 ? std::min(chunks, 4) : 1;
+  if (row_scales) *chunks_per_cta = row_ctas >= 512 ? chunks : std::min(chunks, 4);
+  else *chunks_per_cta = row_ctas >= 512 ? std::min(chunks, 4) : 1;
   *grid = dim3(row_ctas, (chunks + *chunks_per_cta - 1) / *chunks_per_cta);
 }
 
@@ -385,11 +419,23 @@ cudaError_t quantize_as(Fp4QuantParams p, cudaStream_t stream) {
   }
   dim3 grid;
   int per;
-  quant_grid(p.rows, (p.K + kFp4TileK - 1) / kFp4TileK * kFp4TileK, &grid, &per);
   const int al = row_alignment(p.x, p.ldx, sizeof(T));
-  const auto kernel = al == 32   ? fp4_quantize_kernel<T, FMT, 32>
-                      : al == 16 ? fp4_quantize_kernel<T, FMT, 16>
-                                 : fp4_quantize_kernel<T, FMT, 0>;
+  if constexpr (FMT == ICSA_NVFP4) {
+    if (p.row_scales != nullptr) {
+      // every CTA reads whole rows first: with plenty of them it quantises
+      // whole rows too, else four chunks
+      quant_grid(p.rows, (p.K + kFp4TileK - 1) / kFp4TileK * kFp4TileK, &grid, &per, true);
+      const auto kernel = al == 32   ? fp4_quantize_kernel<T, FMT, 32, true>
+                          : al == 16 ? fp4_quantize_kernel<T, FMT, 16, true>
+                                     : fp4_quantize_kernel<T, FMT, 0, true>;
+      kernel<<<grid, kQThreads, 0, stream>>>(p, per);
+      return cudaGetLastError();
+    }
+  }
+  quant_grid(p.rows, (p.K + kFp4TileK - 1) / kFp4TileK * kFp4TileK, &grid, &per);
+  const auto kernel = al == 32   ? fp4_quantize_kernel<T, FMT, 32, false>
+                      : al == 16 ? fp4_quantize_kernel<T, FMT, 16, false>
+                                 : fp4_quantize_kernel<T, FMT, 0, false>;
   kernel<<<grid, kQThreads, 0, stream>>>(p, per);
   return cudaGetLastError();
 }

@@ -250,6 +250,7 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
       bias[threadIdx.x & 127] = bv;
       pair::named_sync(1u + uint32_t(w), 128);
     }
+    const float alpha = row0 + lane < p.M ? row_alpha(p, row0 + lane) : 0.f;
     const bool ok = attn::warp_mbar_wait(&sm.acc_full, uint32_t(count) & 1u, nullptr, kErrAccFull, abort_flag);
     tc::fence_after_sync();
     float acc[128];
@@ -298,10 +299,10 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
         const float4 b1 = *reinterpret_cast<const float4*>(bias + 64 * h + 8 * i + 4);
         const float* x = acc + 64 * h + 8 * i;
         uint4 o;
-        o.x = pack_bf16x2(finish(p, x[0], b0.x), finish(p, x[1], b0.y));
-        o.y = pack_bf16x2(finish(p, x[2], b0.z), finish(p, x[3], b0.w));
-        o.z = pack_bf16x2(finish(p, x[4], b1.x), finish(p, x[5], b1.y));
-        o.w = pack_bf16x2(finish(p, x[6], b1.z), finish(p, x[7], b1.w));
+        o.x = pack_bf16x2(finish(p, x[0], alpha, b0.x), finish(p, x[1], alpha, b0.y));
+        o.y = pack_bf16x2(finish(p, x[2], alpha, b0.z), finish(p, x[3], alpha, b0.w));
+        o.z = pack_bf16x2(finish(p, x[4], alpha, b1.x), finish(p, x[5], alpha, b1.y));
+        o.w = pack_bf16x2(finish(p, x[6], alpha, b1.z), finish(p, x[7], alpha, b1.w));
         *reinterpret_cast<uint4*>(box + lane * 128 + ((uint32_t(i) ^ uint32_t(lane & 7)) << 4)) = o;
       }
       if (p.tma_out) {
@@ -407,12 +408,12 @@ __global__ void __launch_bounds__(256) fp4_reduce_kernel(const Fp4GemmParams p) 
     a.z += x.z;
     a.w += x.w;
   }
-  const float v[4] = {a.x, a.y, a.z, a.w};
+  const float v[4] = {a.x, a.y, a.z, a.w}, alpha = row_alpha(p, r);
   __nv_bfloat16* out = p.out + size_t(r) * p.ldo + c;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (c + e < p.N)
-      out[e] = __float2bfloat16_rn(finish(p, v[e], p.bias != nullptr ? __bfloat162float(p.bias[c + e]) : 0.f));
+      out[e] = __float2bfloat16_rn(finish(p, v[e], alpha, p.bias != nullptr ? __bfloat162float(p.bias[c + e]) : 0.f));
 }
 
 }  // namespace

@@ -39,8 +39,13 @@ ICSA_DEV float gelu_tanh(float x) {
   return __fdividef(x, 1.0f + attn::ex2(x * fmaf(c3 * x, x, c1)));
 }
 
-ICSA_DEV float finish(const Fp4GemmParams& p, float acc, float bias) {
-  const float y = fmaf(acc, p.alpha, bias);
+// both global scales of an output row
+ICSA_DEV float row_alpha(const Fp4GemmParams& p, int row) {
+  return p.row_scales != nullptr ? p.alpha * p.row_scales[row] : p.alpha;
+}
+
+ICSA_DEV float finish(const Fp4GemmParams& p, float acc, float alpha, float bias) {
+  const float y = fmaf(acc, alpha, bias);
   return p.activation == ICSA_ACT_GELU_TANH ? gelu_tanh(y) : y;
 }
 

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float bias = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
 #pragma unroll
         for (int m = 0; m < MP; ++m)
-          if (m < p.M) p.out[size_t(m) * p.ldo + n] = __float2bfloat16_rn(finish(p, __uint_as_float(acc[m]), bias));
+          if (m < p.M) p.out[size_t(m) * p.ldo + n] = __float2bfloat16_rn(finish(p, __uint_as_float(acc[m]), row_alpha(p, m), bias));
       }
     }
   } else if (warp == kProducerWarp) {
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kTileN) fp4_rows_join_kernel(const Fp4GemmPara
   const float bias = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
 #pragma unroll
   for (int i = 0; i < kJoinRows; ++i)
-    if (m0 + i < p.M) p.out[size_t(m0 + i) * p.ldo + n] = __float2bfloat16_rn(finish(p, acc[i], bias));
+    if (m0 + i < p.M) p.out[size_t(m0 + i) * p.ldo + n] = __float2bfloat16_rn(finish(p, acc[i], row_alpha(p, m0 + i), bias));
 }
 
 template <int FMT, int MP>

@@ -37,6 +37,7 @@ struct Fp4QuantParams {
   uint8_t* data;
   uint8_t* scales;
   float inv_hi, inv_lo;  // 1 / (6 global_scale) as a sum of two floats (0: divide instead); set by the launcher
+  float* row_scales;     // nvfp4, [rows] or nullptr: a power of two for each row in place of global_scale, written here
 };
 cudaError_t launch_fp4_quantize(const Fp4QuantParams& p, int x_dtype, int format, cudaStream_t stream);
 
@@ -59,6 +60,7 @@ struct Fp4GemmMaps {
 struct Fp4GemmParams {
   int M, N, K;
   float alpha;                 // product of the two global scales
+  const float* row_scales;     // [M] or nullptr: a's global scales by row, on top of alpha
   const __nv_bfloat16* bias;   // [N] or nullptr
   int activation;
   __nv_bfloat16* out;          // [M, ldo]

@@ -169,6 +169,59 @@ int launch_linear(const Fp4Call& call, int format, cudaStream_t stream) {
   return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_linear");
 }
 
+// icsa_fp4_quantize, with the rows' own scales where row_scales is not NULL
+int quantize_rows(const void* x, int x_dtype, int64_t ldx, int rows, int K, int format, float global_scale, void* data,
+                  void* scales, float* row_scales, cudaStream_t stream) {
+  int rc;
+  if ((rc = check_fp4("fp4_quantize", format, rows, K)) != ICSA_OK) return rc;
+  if ((rc = check_global_scale("fp4_quantize", format, global_scale)) != ICSA_OK) return rc;
+  if (!dtype_ok(x_dtype)) return fail(ICSA_ERR_INVALID, "fp4_quantize: x_dtype must be ICSA_BF16 or ICSA_F32");
+  if (ldx < K) return fail(ICSA_ERR_INVALID, "fp4_quantize: ldx=%lld is smaller than K=%d", (long long)ldx, K);
+  if (rows == 0) return ICSA_OK;
+  if ((rc = check_fp4_buffers("fp4_quantize", data, scales)) != ICSA_OK) return rc;
+  if (x == nullptr || !aligned(x, x_dtype == ICSA_F32 ? 4 : 2))
+    return fail(ICSA_ERR_INVALID, "fp4_quantize: x must be non-NULL and aligned to its elements");
+  icsa::Fp4QuantParams p = {x, ldx, rows, K, global_scale, static_cast<uint8_t*>(data), static_cast<uint8_t*>(scales),
+                            0.f, 0.f, row_scales};
+  cudaError_t e = icsa::launch_fp4_quantize(p, x_dtype, format, stream);
+  return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_quantize");
+}
+
+// Bytes of the quantised rows in a linear layer's workspace: data, scales, row scales.
+size_t rows_bytes(int format, int M, int K, bool scaled) {
+  return align256(size_t(M) * size_t(icsa::fp4_row_bytes(K))) + align256(size_t(icsa::fp4_scale_bytes(format, M, K))) +
+         (scaled ? align256(size_t(M) * sizeof(float)) : 0);
+}
+
+// A linear layer on rows that are quantised in the workspace first; `scaled`:
+// with a global scale for each row (nvfp4; mxfp4's own scales have the range).
+int linear_rows(const char* who, bool scaled, int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
+                const void* w_scales, float w_global_scale, const void* bias, int activation, void* out, int64_t ldo,
+                int M, int N, int K, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  int rc;
+  if ((rc = check_fp4(who, format, M, K)) != ICSA_OK) return rc;
+  const size_t data = align256(size_t(M) * size_t(icsa::fp4_row_bytes(K)));
+  const size_t scales = align256(size_t(icsa::fp4_scale_bytes(format, M, K)));
+  const size_t need = rows_bytes(format, M, K, scaled);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (M > 0) {
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(ICSA_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu bytes that the "
+                  "quantised rows take", who, workspace == nullptr ? size_t(0) : workspace_bytes, need);
+    if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "%s: the workspace must be 256-byte aligned", who);
+  }
+  // the linear layer's own checks come before anything is launched
+  Fp4Call call;
+  if ((rc = prepare_linear(&call, format, ws, ws + data, 1.f, w_data, w_scales, w_global_scale, bias, activation, out,
+                           ldo, M, N, K, M > 0 ? ws + need : nullptr, M > 0 ? workspace_bytes - need : 0)) != ICSA_OK)
+    return rc;
+  float* row_scales = scaled && format == ICSA_NVFP4 && M > 0 ? reinterpret_cast<float*>(ws + data + scales) : nullptr;
+  if ((rc = quantize_rows(x, x_dtype, ldx, M, K, format, 1.f, ws, ws + data, row_scales, stream)) != ICSA_OK) return rc;
+  call.p.row_scales = row_scales;
+  call.p.w_ready = 1;  // that kernel is an ordinary launch, behind whatever wrote the weight
+  return launch_linear(call, format, stream);
+}
+
 // ------------------------------------------------------------------ 8 bits --
 int check_cache(const char* who, const icsa_kv8_cache* c, icsa::Kv8Cache* out) {
   if (c == nullptr) return fail(ICSA_ERR_INVALID, "%s: the cache is NULL", who);
@@ -327,19 +380,7 @@ size_t icsa_fp4_scale_bytes(int format, int rows, int K) {
 
 int icsa_fp4_quantize(const void* x, int x_dtype, int64_t ldx, int rows, int K, int format, float global_scale,
                       void* data, void* scales, cudaStream_t stream) {
-  int rc;
-  if ((rc = check_fp4("fp4_quantize", format, rows, K)) != ICSA_OK) return rc;
-  if ((rc = check_global_scale("fp4_quantize", format, global_scale)) != ICSA_OK) return rc;
-  if (!dtype_ok(x_dtype)) return fail(ICSA_ERR_INVALID, "fp4_quantize: x_dtype must be ICSA_BF16 or ICSA_F32");
-  if (ldx < K) return fail(ICSA_ERR_INVALID, "fp4_quantize: ldx=%lld is smaller than K=%d", (long long)ldx, K);
-  if (rows == 0) return ICSA_OK;
-  if ((rc = check_fp4_buffers("fp4_quantize", data, scales)) != ICSA_OK) return rc;
-  if (x == nullptr || !aligned(x, x_dtype == ICSA_F32 ? 4 : 2))
-    return fail(ICSA_ERR_INVALID, "fp4_quantize: x must be non-NULL and aligned to its elements");
-  icsa::Fp4QuantParams p = {x, ldx, rows, K, global_scale, static_cast<uint8_t*>(data), static_cast<uint8_t*>(scales),
-                            0.f, 0.f};
-  cudaError_t e = icsa::launch_fp4_quantize(p, x_dtype, format, stream);
-  return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "fp4_quantize");
+  return quantize_rows(x, x_dtype, ldx, rows, K, format, global_scale, data, scales, nullptr, stream);
 }
 
 int icsa_fp4_dequantize(const void* data, const void* scales, int rows, int K, int format, float global_scale,
@@ -376,33 +417,28 @@ int icsa_fp4_linear(int format, const void* a_data, const void* a_scales, float 
 
 size_t icsa_fp4_linear_rows_workspace_size(int format, int M, int N, int K) {
   if (check_fp4("fp4_linear_rows_workspace_size", format, M, K) != ICSA_OK || M < 1 || N < 1) return 0;
-  return align256(icsa_fp4_data_bytes(M, K)) + align256(icsa_fp4_scale_bytes(format, M, K)) +
-         icsa_fp4_linear_workspace_size(M, N, K);
+  return rows_bytes(format, M, K, false) + icsa_fp4_linear_workspace_size(M, N, K);
+}
+
+size_t icsa_fp4_linear_scaled_rows_workspace_size(int format, int M, int N, int K) {
+  if (check_fp4("fp4_linear_scaled_rows_workspace_size", format, M, K) != ICSA_OK || M < 1 || N < 1) return 0;
+  return rows_bytes(format, M, K, true) + icsa_fp4_linear_workspace_size(M, N, K);
 }
 
 int icsa_fp4_linear_rows(int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
                          const void* w_scales, float w_global_scale, const void* bias, int activation, void* out,
                          int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes,
                          cudaStream_t stream) {
-  int rc;
-  if ((rc = check_fp4("fp4_linear_rows", format, M, K)) != ICSA_OK) return rc;
-  const size_t data = align256(icsa_fp4_data_bytes(M, K)), scales = align256(icsa_fp4_scale_bytes(format, M, K));
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (M > 0) {
-    if (workspace == nullptr || workspace_bytes < data + scales)
-      return fail(ICSA_ERR_WORKSPACE, "fp4_linear_rows: workspace of %zu bytes is smaller than the %zu bytes that the "
-                  "quantised rows take", workspace == nullptr ? size_t(0) : workspace_bytes, data + scales);
-    if (!aligned(workspace, 256)) return fail(ICSA_ERR_INVALID, "fp4_linear_rows: the workspace must be 256-byte aligned");
-  }
-  // the linear layer's own checks come before anything is launched
-  Fp4Call call;
-  if ((rc = prepare_linear(&call, format, ws, ws + data, 1.f, w_data, w_scales, w_global_scale, bias, activation, out,
-                           ldo, M, N, K, M > 0 ? ws + data + scales : nullptr,
-                           M > 0 ? workspace_bytes - data - scales : 0)) != ICSA_OK)
-    return rc;
-  if ((rc = icsa_fp4_quantize(x, x_dtype, ldx, M, K, format, 1.f, ws, ws + data, stream)) != ICSA_OK) return rc;
-  call.p.w_ready = 1;  // that kernel is an ordinary launch, behind whatever wrote the weight
-  return launch_linear(call, format, stream);
+  return linear_rows("fp4_linear_rows", false, format, x, x_dtype, ldx, w_data, w_scales, w_global_scale, bias,
+                     activation, out, ldo, M, N, K, workspace, workspace_bytes, stream);
+}
+
+int icsa_fp4_linear_scaled_rows(int format, const void* x, int x_dtype, int64_t ldx, const void* w_data,
+                                const void* w_scales, float w_global_scale, const void* bias, int activation,
+                                void* out, int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes,
+                                cudaStream_t stream) {
+  return linear_rows("fp4_linear_scaled_rows", true, format, x, x_dtype, ldx, w_data, w_scales, w_global_scale, bias,
+                     activation, out, ldo, M, N, K, workspace, workspace_bytes, stream);
 }
 
 int icsa_kv8_quantize(const icsa_kv8_cache* cache, const void* k, const void* v, int dtype, const int64_t k_strides[3],

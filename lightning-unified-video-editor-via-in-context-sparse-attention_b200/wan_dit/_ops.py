@@ -262,8 +262,19 @@ class CudaOps:
 
     @staticmethod
     def fp4_linear(x, w, b=None, activation=None):
-        """bf16 act(x @ w^T + b): x bf16 rows, quantised per call; w from fp4_weight."""
+        """bf16 act(x @ w^T + b): x bf16 rows of order one, quantised per call; w from fp4_weight."""
         return lowp.fp4_linear(x, w, b, activation)
+
+    def fp4_linear_scaled(self, x, w, b=None, activation=None):
+        """fp4_linear of rows of any magnitude (attention and GELU outputs): each
+        takes a global scale of its own, a power of two."""
+        if isinstance(w, lowp.Fp4Tensor):
+            return lowp.fp4_linear(x, w, b, activation, row_scales=True)
+        # operations with weights of their own: their fp4_linear, on rows brought into its range
+        g = lowp.fp4_row_scales(x)
+        y = self.fp4_linear((x / g).to(x.dtype), w) * g
+        y = y if b is None else y + b
+        return self.gelu_tanh(y.to(torch.bfloat16)) if activation == "gelu_tanh" else y.to(torch.bfloat16)
 
     # --- attention ---------------------------------------------------------
     def self_attention(self, q, k, v, alpha, t_seq_len, means=None):

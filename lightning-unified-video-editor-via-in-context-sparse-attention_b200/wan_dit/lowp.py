@@ -27,7 +27,8 @@ from in_context_sparse_attention import _capi
 
 LOWP_EXPORTED = ("icsa_fp4_data_bytes", "icsa_fp4_scale_bytes", "icsa_fp4_quantize", "icsa_fp4_dequantize",
                  "icsa_fp4_linear_workspace_size", "icsa_fp4_linear", "icsa_fp4_linear_rows_workspace_size",
-                 "icsa_fp4_linear_rows", "icsa_kv8_quantize", "icsa_kv8_dequantize",
+                 "icsa_fp4_linear_rows", "icsa_fp4_linear_scaled_rows_workspace_size", "icsa_fp4_linear_scaled_rows",
+                 "icsa_kv8_quantize", "icsa_kv8_dequantize",
                  "icsa_kv8_attention_workspace_size", "icsa_kv8_attention")
 
 FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
@@ -67,6 +68,8 @@ def _load():
             ("icsa_fp4_linear", i, [i, vp, vp, f, vp, vp, f, vp, i, vp, i64, i, i, i, vp, sz, vp]),
             ("icsa_fp4_linear_rows_workspace_size", sz, [i, i, i, i]),
             ("icsa_fp4_linear_rows", i, [i, vp, i, i64, vp, vp, f, vp, i, vp, i64, i, i, i, vp, sz, vp]),
+            ("icsa_fp4_linear_scaled_rows_workspace_size", sz, [i, i, i, i]),
+            ("icsa_fp4_linear_scaled_rows", i, [i, vp, i, i64, vp, vp, f, vp, i, vp, i64, i, i, i, vp, sz, vp]),
             ("icsa_kv8_quantize", i, [desc, vp, vp, i, st, st, vp]),
             ("icsa_kv8_dequantize", i, [desc, vp, vp, i, vp]),
             ("icsa_kv8_attention_workspace_size", sz, [desc, i, i]),
@@ -175,6 +178,17 @@ def fp4_global_scale(x: torch.Tensor) -> float:
     return 1.0 if top == 0 else math.ldexp(1.0, max(min(e - (m == 0.5), 100), -100))
 
 
+def fp4_row_scales(x: torch.Tensor) -> torch.Tensor:
+    """f32 [rows, 1]: the global scales that fp4_linear(row_scales=True) gives
+    the rows of x.  2^e, e the smallest with which the row's largest magnitude
+    is in range (448 x 6 steps), in [-90, 90]; 1 for a row of zeros and for one
+    with a NaN or an infinity."""
+    top = x.detach().float().abs().amax(dim=1, keepdim=True)
+    m, e = torch.frexp(top / (6 * 448))       # (the quotient of floats rounds to a power of two only where it is one)
+    e = (e - (m == 0.5).int()).clamp(-90, 90)
+    return torch.where((top > 0) & torch.isfinite(top), torch.ldexp(torch.ones_like(top), e), 1.0)
+
+
 def _rows2d(where, x):
     """x as rows of contiguous elements that do not overlap, and their distance."""
     shape = x.shape
@@ -233,12 +247,17 @@ def _dequantize(lib, stream, t, dtype):
     return out
 
 
-def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
+def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+               row_scales: bool = False) -> torch.Tensor:
     """bf16 [M, N] = act(x @ w^T + bias) with both operands in 4 bits.
 
     x: an Fp4Tensor [M, K] of w's format, or bf16 / f32 [M, K], which is
-    quantised to it (global scale 1) first.  w: [N, K].  bias: bf16 [N].
-    activation: None or "gelu_tanh"."""
+    quantised to it first.  w: [N, K].  bias: bf16 [N].  activation: None or
+    "gelu_tanh".  row_scales: x is quantised with a global scale for each of
+    its rows, a power of two found on the device, in place of 1.  nvfp4 needs
+    that for rows that are not of order one: with scale 1 a block of 16 below
+    0.0059 becomes zero, below 0.09 it loses bits, and above 2688 it
+    saturates.  (mxfp4 has the range by itself: no difference.)"""
     if activation not in ACTIVATIONS:
         raise ValueError(f"fp4_linear: activation {activation!r}, expected one of {list(ACTIVATIONS)}")
     if not isinstance(w, Fp4Tensor):
@@ -255,17 +274,21 @@ def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation:
     if isinstance(x, Fp4Tensor):
         if x.fmt != w.fmt:
             raise ValueError(f"fp4_linear: x is {x.fmt}, w is {w.fmt}")
+        if row_scales:
+            raise ValueError("fp4_linear: row_scales is for rows that are still to be quantised")
         return _on(_device("fp4_linear", x.data, x.scales, w.data, w.scales, bias), _linear, x, w, bias, activation)
     index = _device("fp4_linear", x, w.data, w.scales, bias)
     x, ld = _rows2d("fp4_linear", x)
-    return _on(index, _linear_rows, x, ld, w, bias, activation)
+    return _on(index, _linear_rows, x, ld, w, bias, activation, row_scales and w.fmt == "nvfp4")
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_workspace(index, fmt, M, N, K):
-    """Workspace bytes of icsa_fp4_linear (fmt None) or icsa_fp4_linear_rows; the device is current."""
+def _linear_workspace(index, fmt, M, N, K, scaled=False):
+    """Workspace bytes of icsa_fp4_linear (fmt None) or icsa_fp4_linear[_scaled]_rows; the device is current."""
     if fmt is None:
         return _lib.icsa_fp4_linear_workspace_size(M, N, K)
+    if scaled:
+        return _lib.icsa_fp4_linear_scaled_rows_workspace_size(FP4_FORMATS[fmt], M, N, K)
     return _lib.icsa_fp4_linear_rows_workspace_size(FP4_FORMATS[fmt], M, N, K)
 
 
@@ -283,17 +306,17 @@ def _linear(lib, stream, a, w, bias, activation):
     return out
 
 
-def _linear_rows(lib, stream, x, ld, w, bias, activation):
+def _linear_rows(lib, stream, x, ld, w, bias, activation, scaled):
     (M, K), N = x.shape, w.shape[0]
     out = _empty((M, N), (N, 1), dtype=torch.bfloat16, device=x.device)
-    size = _linear_workspace(x.get_device(), w.fmt, M, N, K)
+    size = _linear_workspace(x.get_device(), w.fmt, M, N, K, scaled)
     ws, ptr = _bytes(out, size)
-    code = lib.icsa_fp4_linear_rows(FP4_FORMATS[w.fmt], x.data_ptr(), _DT[x.dtype], ld, w.data.data_ptr(),
-                                    w.scales.data_ptr(), w.global_scale,
-                                    bias.data_ptr() if bias is not None else None, ACTIVATIONS[activation],
-                                    out.data_ptr(), N, M, N, K, ptr, size, stream)
+    fn = lib.icsa_fp4_linear_scaled_rows if scaled else lib.icsa_fp4_linear_rows
+    code = fn(FP4_FORMATS[w.fmt], x.data_ptr(), _DT[x.dtype], ld, w.data.data_ptr(), w.scales.data_ptr(),
+              w.global_scale, bias.data_ptr() if bias is not None else None, ACTIVATIONS[activation], out.data_ptr(),
+              N, M, N, K, ptr, size, stream)
     if code:
-        _capi.check(code, "icsa_fp4_linear_rows")
+        _capi.check(code, fn.__name__)
     return out
 
 

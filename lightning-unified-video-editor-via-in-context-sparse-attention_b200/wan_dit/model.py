@@ -104,8 +104,10 @@ class _Block:
         self.modulation = (torch.randn(6, C, generator=g, device=device) / C ** 0.5).to(torch.bfloat16)
 
 
-    # the layers that linear_format applies to
+    # the layers that linear_format applies to, and those of them whose input no
+    # norm brings to order one
     LINEARS = ("w_qkv", "w_o", "wc_q", "wc_kv", "wc_o", "w1", "w2")
+    SCALED = ("w_o", "wc_kv", "wc_o", "w2")
 
     def quantize_linears(self, ops, fmt: str):
         """Replaces the bf16 weights of the linear layers by 4-bit ones."""
@@ -268,14 +270,15 @@ class WanDiT:
     def _linear(self, blk: _Block, w: str, b: str, x, activation=None):
         """bf16 act(x @ w^T + b); w, b: names of the block's weight and bias."""
         if w in blk.fp4:
-            return self.ops.fp4_linear(x, blk.fp4[w], getattr(blk, b), activation)
+            linear = self.ops.fp4_linear_scaled if w in blk.SCALED else self.ops.fp4_linear
+            return linear(x, blk.fp4[w], getattr(blk, b), activation)
         y = self.ops.linear(x, getattr(blk, w), getattr(blk, b))
         return self.ops.gelu_tanh(y) if activation == "gelu_tanh" else y
 
     def _linear_residual_(self, blk: _Block, w: str, b: str, x, a, gate, rows_per_batch):
         """x += (a @ w^T + b) * gate in place (gate None: + ...)."""
         if w in blk.fp4:
-            self.ops.gated_residual_(x, self.ops.fp4_linear(a, blk.fp4[w], getattr(blk, b)), gate, rows_per_batch)
+            self.ops.gated_residual_(x, self._linear(blk, w, b, a), gate, rows_per_batch)
         else:
             self.ops.linear_residual_(x, a, getattr(blk, w), getattr(blk, b), gate, rows_per_batch)
 

@@ -1,0 +1,36 @@
+"""CPU checks of the 4-bit linear layer on rows with their own scales: refusals, before any launch."""
+import math
+
+import pytest
+import torch
+
+from wan_dit import Fp4Tensor, lowp
+
+INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 4
+
+
+def test_row_scales_are_for_rows_that_are_to_be_quantised():
+    data, scales = (torch.zeros(s, dtype=torch.uint8) for s in lowp.fp4_storage(8, 32, "nvfp4"))
+    w = Fp4Tensor(data, scales, (8, 32), "nvfp4")
+    with pytest.raises(ValueError, match="row_scales"):
+        lowp.fp4_linear(w, w, row_scales=True)
+    with pytest.raises(ValueError, match="CUDA"):
+        lowp.fp4_linear(torch.zeros(4, 32), w, row_scales=True)
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_c_abi_refuses_before_any_launch(fmt):
+    lib = lowp._load()
+
+    def rows(fmt=fmt, x=16, dt=0, ldx=32, w=16, sw=128, gw=1.0, bias=None, act=0, out=16, ldo=8, M=4, N=8, K=32, ws=256,
+             size=1 << 20):
+        return lib.icsa_fp4_linear_scaled_rows(fmt, x, dt, ldx, w, sw, gw, bias, act, out, ldo, M, N, K, ws, size, None)
+    for bad in (dict(fmt=7), dict(w=8), dict(sw=None), dict(gw=-1.0), dict(gw=math.nan), dict(bias=3), dict(act=2),
+                dict(out=None), dict(ldo=7), dict(M=-1), dict(N=0), dict(K=0), dict(ws=128)):
+        assert rows(**bad) == INVALID, bad
+    need = 256 + lib.icsa_fp4_scale_bytes(fmt, 4, 32) + 256
+    assert rows(ws=None) == WORKSPACE and rows(size=need - 1) == WORKSPACE
+    assert rows(M=1 << 28) == UNSUPPORTED
+    assert rows(M=0, x=None, out=None, ws=None, size=0) == 0
+    assert lib.icsa_fp4_linear_scaled_rows_workspace_size(fmt, 0, 8, 32) == 0
+    assert lib.icsa_fp4_linear_scaled_rows_workspace_size(7, 4, 8, 32) == 0
