@@ -224,7 +224,8 @@ ICSA_DEV int tile_row(int cta, int warp) {
 
 // The 16 codes of x / d, those of the correctly rounded float32 quotient:
 // with 1 / d as the sum of two floats, rh + rl, the sum x rh + x rl is within
-// a relative 2^-45 of the quotient before its one rounding.  That rounding is
+// a relative 2^-42 of the quotient before its one rounding (both parts are
+// positive, so that an x of -0 stays -0).  That rounding is
 // the quotient's own unless a midpoint m of two floats (25 bits) lies between
 // the two, and with d of at most 8 significant bits m d has at most 33, so a
 // float x is no closer to it than a relative 2^-33.  Such steps are those of
@@ -237,7 +238,8 @@ ICSA_DEV void quotient_codes(const float (&v)[16], float amax, float d, uint32_t
   float q[16];
   if (d > 0x1p-100f && d < 0x1p100f && amax <= 8.f * d && short_step(d)) {
     float rh;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(rh) : "f"(d));  // any value near 1 / d: rl is what it lacks
+    asm("rcp.approx.f32 %0, %1;" : "=f"(rh) : "f"(d));  // within one unit in the last place of 1 / d
+    rh = __uint_as_float(__float_as_uint(rh) - 2u);       // below it: rl > 0
     const float rl = fmaf(-d, rh, 1.0f) * rh;
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {

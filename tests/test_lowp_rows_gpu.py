@@ -173,3 +173,18 @@ def test_workspace_is_checked_and_not_overrun():
     assert call(ws.data_ptr(), size) == 0
     assert torch.equal(out[:M, :N], want)
     assert bool((out[M:] == 7).all()) and bool((out[:, N:] == 7).all()) and bool((ws[size:] == 0xFF).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt,g", [("nvfp4", 1.0), ("nvfp4", 2.0 ** -9), ("nvfp4", 0.37), ("mxfp4", 1.0)])
+def test_negative_zeros_and_tiny_negatives_keep_their_sign(fmt, g, dtype):
+    """The code of -0 is that of the float32 quotient, -0 (GELU and ReLU give such elements)."""
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randn(200, 512, generator=gen)
+    x = torch.where(torch.rand(200, 512, generator=gen) < 0.3, -0.0, x)
+    x[:, 7] = -1e-30
+    x = x.to(dtype)
+    code, sb, _ = ref.fp4_quantize(x, fmt, g)
+    t = lowp.fp4_quantize(x.cuda(), fmt, g)
+    assert torch.equal(t.scales.flatten().cpu(), ref.fp4_scale_bytes(sb, 200, 512, fmt))
+    assert torch.equal(t.data.cpu(), ref.fp4_data_bytes(code, 512))
