@@ -62,7 +62,8 @@ ICSA_API int icsa_fp4_dequantize(const void* data, const void* scales, int rows,
 /*
  * out[r, c] = bf16( act( sum_k a[r, k] w[c, k] + bias[c] ) ), a: [M, K],
  * w: [N, K] (nn.Linear weight) in the same 4-bit format, products and scales
- * in the tensor core, float32 accumulation, one rounding.
+ * in the tensor core, float32 accumulation, one rounding.  The product of the
+ * two global scales must be in float's range.
  *   bias: bf16 [N] or NULL;  activation: enum icsa_activation
  *   out:  bf16 [M, ldo]
  *   workspace: icsa_fp4_linear_workspace_size() bytes (0: none needed), 256-byte

@@ -121,6 +121,10 @@ int prepare_linear(Fp4Call* call, int format, const void* a_data, const void* a_
   if ((rc = check_fp4("fp4_linear", format, N, K)) != ICSA_OK) return rc;
   if ((rc = check_global_scale("fp4_linear", format, a_global_scale)) != ICSA_OK) return rc;
   if ((rc = check_global_scale("fp4_linear", format, w_global_scale)) != ICSA_OK) return rc;
+  const float alpha = a_global_scale * w_global_scale;
+  if (!std::isnormal(alpha) && (std::isinf(alpha) || double(alpha) != double(a_global_scale) * double(w_global_scale)))
+    return fail(ICSA_ERR_INVALID, "fp4_linear: the product of the global scales %g and %g is out of float's range",
+                double(a_global_scale), double(w_global_scale));
   if (N < 1) return fail(ICSA_ERR_INVALID, "fp4_linear: N=%d must be positive", N);
   if (activation != ICSA_ACT_NONE && activation != ICSA_ACT_GELU_TANH)
     return fail(ICSA_ERR_INVALID, "fp4_linear: unknown activation %d", activation);
@@ -134,7 +138,7 @@ int prepare_linear(Fp4Call* call, int format, const void* a_data, const void* a_
     return fail(ICSA_ERR_INVALID, "fp4_linear: out must be non-NULL, out and bias aligned to their elements");
   if (!sm_count(&sms)) return ICSA_ERR_CUDA;
   p.M = M; p.N = N; p.K = K;
-  p.alpha = a_global_scale * w_global_scale;
+  p.alpha = alpha;
   p.bias = static_cast<const __nv_bfloat16*>(bias);
   p.activation = activation;
   p.out = static_cast<__nv_bfloat16*>(out);

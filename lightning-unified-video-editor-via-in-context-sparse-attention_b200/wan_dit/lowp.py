@@ -161,8 +161,8 @@ def fp4_storage(rows: int, K: int, fmt: str):
 
 
 def _check_global_scale(fmt, g):
-    if not (isinstance(g, (int, float)) and math.isfinite(g) and g > 0):
-        raise ValueError(f"the global scale must be a positive finite number, got {g!r}")
+    if not (isinstance(g, (int, float)) and 2.0 ** -149 <= g < 2.0 ** 128):     # (false for a NaN)
+        raise ValueError(f"the global scale must be a positive finite float32 number, got {g!r}")
     if fmt == "mxfp4" and g != 1:
         raise ValueError("mxfp4 has no global scale (must be 1)")
 

@@ -34,3 +34,21 @@ def test_c_abi_refuses_before_any_launch(fmt):
     assert rows(M=0, x=None, out=None, ws=None, size=0) == 0
     assert lib.icsa_fp4_linear_scaled_rows_workspace_size(fmt, 0, 8, 32) == 0
     assert lib.icsa_fp4_linear_scaled_rows_workspace_size(7, 4, 8, 32) == 0
+
+
+def test_global_scales_whose_product_leaves_float_are_refused():
+    """alpha = a_global_scale w_global_scale is one float: beyond its range it would be an infinity or zero."""
+    lib = lowp._load()
+
+    def linear(ga, gw):
+        return lib.icsa_fp4_linear(0, 16, 128, ga, 16, 128, gw, None, 0, 16, 8, 0, 8, 32, None, 0, None)
+    for ga, gw in ((1e-30, 1e-30), (1e30, 1e30), (2.0 ** -100, 2.0 ** -50), (1e-22, 1e-22)):
+        assert linear(ga, gw) == INVALID and b"product" in lib.icsa_last_error()
+    for ga, gw in ((1e-30, 1e30), (2.0 ** -60, 2.0 ** -60), (2.0 ** 60, 2.0 ** 60), (1.0, 1e-38),
+                   (2.0 ** -70, 2.0 ** -70)):                    # (small, but exact)
+        assert linear(ga, gw) == 0                               # no rows: nothing to launch
+    # a scale that is no float
+    data, scales = (torch.zeros(s, dtype=torch.uint8) for s in lowp.fp4_storage(8, 32, "nvfp4"))
+    for g in (1e-60, 1e60):
+        with pytest.raises(ValueError, match="global scale"):
+            Fp4Tensor(data, scales, (8, 32), "nvfp4", g)
