@@ -11,7 +11,8 @@ fallback).
 
 Every function takes and returns torch tensors on one CUDA device (which need
 not be the current one) and runs on that device's current stream.  They
-compute values only: no gradient is recorded.
+compute values only: no gradient is recorded, and fp4_linear and kv8_attention
+refuse an input that requires one where gradients are enabled.
 """
 from __future__ import annotations
 
@@ -94,6 +95,11 @@ def _device(where, *tensors):
                 raise ValueError(f"{where}: tensors on cuda:{index} and cuda:{i}")
             index = i
     return index
+
+
+def _no_gradient(where, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{where}: no gradient is recorded; detach the inputs or call it under torch.no_grad()")
 
 
 def _on(index, fn, *args):
@@ -270,6 +276,7 @@ def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation:
     if bias is not None:
         if bias.dtype != torch.bfloat16 or bias.shape != (N,):
             raise ValueError(f"fp4_linear: bias must be bf16 [{N}]")
+        _no_gradient("fp4_linear", bias)
         bias = bias.contiguous()
     if isinstance(x, Fp4Tensor):
         if x.fmt != w.fmt:
@@ -277,6 +284,7 @@ def fp4_linear(x, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, activation:
         if row_scales:
             raise ValueError("fp4_linear: row_scales is for rows that are still to be quantised")
         return _on(_device("fp4_linear", x.data, x.scales, w.data, w.scales, bias), _linear, x, w, bias, activation)
+    _no_gradient("fp4_linear", x)
     index = _device("fp4_linear", x, w.data, w.scales, bias)
     x, ld = _rows2d("fp4_linear", x)
     return _on(index, _linear_rows, x, ld, w, bias, activation, row_scales and w.fmt == "nvfp4")
@@ -448,6 +456,7 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache) -> torch.Tensor:
     [B, Lq, Hq, D]; zero for a sequence of length 0.  q: bf16 [B, Lq, Hq, D],
     Hq a multiple of the cache's heads (query heads h of one group share
     cache head h // (Hq / H))."""
+    _no_gradient("kv8_attention", q)
     index = _device("kv8_attention", q, cache.k)
     B, H, _, _, D = cache.k.shape
     shape = q.shape

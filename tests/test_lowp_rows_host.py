@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from wan_dit import Fp4Tensor, lowp
+from wan_dit import Fp4Tensor, Kv8Cache, lowp
 
 INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 4
 
@@ -52,3 +52,22 @@ def test_global_scales_whose_product_leaves_float_are_refused():
     for g in (1e-60, 1e60):
         with pytest.raises(ValueError, match="global scale"):
             Fp4Tensor(data, scales, (8, 32), "nvfp4", g)
+
+
+def test_inputs_that_require_a_gradient_are_refused_where_gradients_are_enabled():
+    data, scales = (torch.zeros(s, dtype=torch.uint8) for s in lowp.fp4_storage(8, 32, "nvfp4"))
+    w = Fp4Tensor(data, scales, (8, 32), "nvfp4")
+    x, bias = torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(8, dtype=torch.bfloat16)
+    cache = Kv8Cache(torch.zeros(1, 2, 1, 64, 128).to(torch.float8_e4m3fn),
+                     torch.zeros(1, 2, 1, 128, 64).to(torch.float8_e4m3fn), torch.ones(1, 2, 1), torch.ones(1, 2, 1), 5)
+    q = torch.zeros(1, 3, 2, 128, dtype=torch.bfloat16)
+
+    def leaf(t):
+        return t.clone().requires_grad_()
+    calls = (lambda: lowp.fp4_linear(leaf(x), w), lambda: lowp.fp4_linear(x, w, leaf(bias)),
+             lambda: lowp.fp4_linear(w, w, leaf(bias)), lambda: lowp.kv8_attention(leaf(q), cache))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):      # as without one: tensors on the CPU
+            call()
