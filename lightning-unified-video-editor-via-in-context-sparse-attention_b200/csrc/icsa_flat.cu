@@ -1,6 +1,7 @@
 // Dense attention for the "flat" query blocks (the reference's
 // flash_attn_func call, editing_sparse_attention.py:211-215, fused with the
-// scatter and residual of :217-232).
+// scatter and residual of :217-232), head dim 64; head dim 128 runs on SM
+// pairs (icsa_dense_pair.cu).
 //
 // Per CTA: two 128-row query tiles (four 64-token blocks of the flat list)
 // share every K/V tile, which halves the L2 -> SM traffic per FLOP.  Roles:
@@ -36,8 +37,8 @@ template <int D>
 struct FCfg {
   static constexpr int kOpBytes = 128 * D * 2;
   static constexpr int kChunks = D / 64;
-  static constexpr int kKStages = (D == 128) ? 3 : 4;
-  static constexpr int kVStages = (D == 128) ? 2 : 4;
+  static constexpr int kKStages = 4;
+  static constexpr int kVStages = 4;
 };
 
 template <int D>
@@ -54,7 +55,6 @@ struct __align__(1024) FSmem {
   int abort_flag;
 };
 
-static_assert(sizeof(FSmem<128>) + 1024 <= 232448, "flat kernel shared memory exceeds 227 KB");
 static_assert(sizeof(FSmem<64>) + 1024 <= 232448, "flat kernel shared memory exceeds 227 KB");
 
 struct FTile {
@@ -388,21 +388,12 @@ cudaError_t launch_flat_attention(const AttnParams& p, const AttnMaps& maps, int
   const int ctas = p.B * p.H * ((p.num_flat + 3) / 4);
   if (ctas == 0) return cudaSuccess;
   if (D == 128) return launch_dense_pair_attention(p, maps, stream);
-  if (D == 128) {
-    const size_t smem = sizeof(FSmem<128>) + 1024;
-    const auto kernel = is_ragged(p) ? flat_kernel<128, true> : flat_kernel<128, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-    kernel<<<ctas, kFThreads, smem, stream>>>(p, maps);
-  } else if (D == 64) {
-    const size_t smem = sizeof(FSmem<64>) + 1024;
-    const auto kernel = is_ragged(p) ? flat_kernel<64, true> : flat_kernel<64, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-    kernel<<<ctas, kFThreads, smem, stream>>>(p, maps);
-  } else {
-    return cudaErrorInvalidValue;
-  }
+  if (D != 64) return cudaErrorInvalidValue;
+  const size_t smem = sizeof(FSmem<64>) + 1024;
+  const auto kernel = is_ragged(p) ? flat_kernel<64, true> : flat_kernel<64, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  kernel<<<ctas, kFThreads, smem, stream>>>(p, maps);
   return cudaGetLastError();
 }
 
