@@ -215,9 +215,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (m < p.M) dst[m * kTileN] = __uint_as_float(acc[m]);
       } else if (n < p.N) {
         const float bias = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
+        const auto store = [&](auto alpha) {
 #pragma unroll
-        for (int m = 0; m < MP; ++m)
-          if (m < p.M) p.out[size_t(m) * p.ldo + n] = __float2bfloat16_rn(finish(p, __uint_as_float(acc[m]), row_alpha(p, m), bias));
+          for (int m = 0; m < MP; ++m)
+            if (m < p.M) p.out[size_t(m) * p.ldo + n] = __float2bfloat16_rn(finish(p, __uint_as_float(acc[m]), alpha(m), bias));
+        };
+        // (the choice outside the loop: 64 rows x 5120 -> 13824 14.3 us, inside it 15.3)
+        if (p.row_scales == nullptr) store([&](int) { return p.alpha; });
+        else store([&](int m) { return row_alpha(p, m); });
       }
     }
   } else if (warp == kProducerWarp) {
@@ -300,7 +305,9 @@ __global__ void __launch_bounds__(kTileN) fp4_rows_join_kernel(const Fp4GemmPara
   const int n = blockIdx.x * kTileN + threadIdx.x;
   if (c0 == c1 || n >= p.N) return;  // one CTA wrote the tile
   const int m0 = blockIdx.y * kJoinRows;
-  float acc[kJoinRows] = {};
+  float acc[kJoinRows] = {}, alpha[kJoinRows];
+#pragma unroll
+  for (int i = 0; i < kJoinRows; ++i) alpha[i] = m0 + i < p.M ? row_alpha(p, m0 + i) : 0.f;
   constexpr int kAhead = 4;  // parts whose loads are on their way together
   for (int c = c0; c <= c1; c += kAhead) {
     float x[kAhead][kJoinRows] = {};
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(kTileN) fp4_rows_join_kernel(const Fp4GemmPara
   const float bias = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
 #pragma unroll
   for (int i = 0; i < kJoinRows; ++i)
-    if (m0 + i < p.M) p.out[size_t(m0 + i) * p.ldo + n] = __float2bfloat16_rn(finish(p, acc[i], row_alpha(p, m0 + i), bias));
+    if (m0 + i < p.M) p.out[size_t(m0 + i) * p.ldo + n] = __float2bfloat16_rn(finish(p, acc[i], alpha[i], bias));
 }
 
 template <int FMT, int MP>
