@@ -142,8 +142,10 @@ ICSA_API int icsa_kv8_dequantize(const icsa_kv8_cache* cache, void* k_out, void*
  * and accumulation; the probabilities p enter the second product as fp16 (off
  * by 2^-11 of themselves, below 2^-14 of the row's largest by 2^-25 of that
  * one, whatever the scales of the value blocks, as long as these lie within
- * 2^80 of each other), and as bf16 (2^-8) for many queries over a long cache;
- * one rounding of the result.
+ * 2^80 of each other); one rounding of the result.  Many queries over a long
+ * cache run on a 16-bit copy of it in the workspace (two bytes there for each
+ * byte of the cache); in that case heads whose value scales lie more than 2^22
+ * apart have their probabilities in bf16 (off by 2^-8 of themselves).
  *   q: bf16 [B, Lq, Hq, D] with batch, token, head strides (multiples of 8
  *   elements, 16-byte aligned), contiguous features; Hq a multiple of H.
  *   (ICSA_ERR_UNSUPPORTED for many queries over a long cache whose heads are

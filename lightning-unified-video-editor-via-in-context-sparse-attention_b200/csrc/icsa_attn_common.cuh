@@ -5,6 +5,8 @@
 #include "icsa_kernels.cuh"
 #include "icsa_tcgen05.cuh"
 
+#include <cuda_fp16.h>
+
 namespace icsa {
 namespace attn {
 
@@ -106,7 +108,33 @@ ICSA_DEV int key_steps(const AttnParams& p, int keys) {
 }
 template <bool RAGGED>
 ICSA_DEV int key_head(const AttnParams& p, int h) { return RAGGED ? h / p.kv_group : h; }
-inline bool is_ragged(const AttnParams& p) { return p.kv_lens != nullptr || p.kv_group > 1; }
+// R of a key/value head whose values are f16 (see AttnParams), NaN where they are bf16.
+template <bool RAGGED>
+ICSA_DEV float value_reference(const AttnParams& p, int b, int kvh) {
+  return RAGGED && p.v_ref ? p.v_ref[b * (p.H / p.kv_group) + kvh] : __uint_as_float(0x7FC00000u);
+}
+template <bool RAGGED>
+ICSA_DEV bool is_f16(float v_ref) { return RAGGED && v_ref == v_ref; }
+// an instruction descriptor of bf16 operands, or the same of f16
+template <bool RAGGED>
+ICSA_DEV uint32_t operand_idesc(uint32_t bf16, bool f16) {
+  return RAGGED && f16 ? bf16 & ~((1u << 7) | (1u << 10)) : bf16;
+}
+// 64 probabilities as 16-bit pairs
+template <bool RAGGED>
+ICSA_DEV void pack_probabilities(const float* s, bool f16, uint32_t (&pk)[32]) {
+  if (RAGGED && f16) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const __half2 v = __floats2half2_rn(s[2 * e], s[2 * e + 1]);
+      pk[e] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) pk[e] = pack_bf16x2(s[2 * e], s[2 * e + 1]);
+  }
+}
+inline bool is_ragged(const AttnParams& p) { return p.kv_lens != nullptr || p.kv_group > 1 || p.v_ref != nullptr; }
 
 ICSA_DEV float load_alpha(const AttnParams& p, int b, int token, int h, int d) {
   const long long off = b * p.alpha_strides[0] + token * p.alpha_strides[1] + h * p.alpha_strides[2] +

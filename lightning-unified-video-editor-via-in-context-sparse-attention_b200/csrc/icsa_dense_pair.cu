@@ -73,6 +73,7 @@ struct PTile {
   int write[2];  // 0 for a duplicate filling an incomplete group
   int n_steps;   // key steps of 128 rows
   int keys, kvh;  // valid keys and key/value head
+  float v_ref;    // see AttnParams
   uint32_t rank;
 };
 
@@ -98,6 +99,7 @@ ICSA_DEV PTile decode_pair_tile(const AttnParams& p) {
   t.keys = key_count<RAGGED>(p, t.b);
   t.n_steps = key_steps<RAGGED>(p, t.keys);
   t.kvh = key_head<RAGGED>(p, t.h);
+  t.v_ref = value_reference<RAGGED>(p, t.b, t.kvh);
   return t;
 }
 
@@ -150,9 +152,8 @@ ICSA_DEV void pair_issue_s_seq(uint64_t q_desc, uint64_t k_desc, uint32_t d_tmem
 // O += P V over 128 keys: eight K = 16 steps; P advances 8 TMEM columns, V
 // (MN-major, 128-byte rows of 64 d) advances 16 rows = 2048 bytes.
 template <int... KK>
-ICSA_DEV void pair_issue_pv_seq(uint64_t v_desc, uint32_t p_tmem, uint32_t o_tmem, uint32_t acc,
+ICSA_DEV void pair_issue_pv_seq(uint64_t v_desc, uint32_t p_tmem, uint32_t o_tmem, uint32_t acc, uint32_t idesc,
                                 std::integer_sequence<int, KK...>) {
-  constexpr uint32_t idesc = tc::make_idesc_bf16(256, 128, false, true);
   (pair::mma_ts_elect<uint32_t(KK * 8), uint32_t((KK * 16 * 128) >> 4)>(o_tmem, p_tmem, v_desc, idesc,
                                                                          (KK > 0) ? 1u : acc),
    ...);
@@ -160,6 +161,7 @@ ICSA_DEV void pair_issue_pv_seq(uint64_t v_desc, uint32_t p_tmem, uint32_t o_tme
 
 // MMA issuer: all 32 lanes of warp 9 of the leader run this loop (waits are
 // warp-uniform, one elected lane issues each instruction).
+template <bool RAGGED>
 ICSA_DEV void pair_mma(const AttnParams& p, const PTile& t, PSmem& sm, uint32_t tmem) {
   volatile int* abort_flag = &sm.abort_flag;
   const int n = t.n_steps;
@@ -167,6 +169,7 @@ ICSA_DEV void pair_mma(const AttnParams& p, const PTile& t, PSmem& sm, uint32_t 
   const uint64_t kd0 = tc::make_sw128_desc(smem_u32(sm.kv[0]), 16, 1024);
   const uint64_t vd0 = tc::make_sw128_desc(smem_u32(sm.kv[0] + kPKBytes), kPVBytes, 1024);
   constexpr uint64_t kKStep = uint64_t((kPKBytes + kPVBytes) >> 4), kVStep = kKStep;
+  const uint32_t idesc_pv = operand_idesc<RAGGED>(tc::make_idesc_bf16(256, 128, false, true), is_f16<RAGGED>(t.v_ref));
   if (!warp_mbar_wait(&sm.q_full, 0, p.err, kErrQ, abort_flag)) return;
 
   auto issue_s = [&](int j) -> bool {
@@ -182,7 +185,8 @@ ICSA_DEV void pair_mma(const AttnParams& p, const PTile& t, PSmem& sm, uint32_t 
     if (!warp_mbar_wait(&sm.p_full[j & 1], uint32_t(j >> 1) & 1u, p.err, kErrPFull, abort_flag)) return false;
     tc::fence_after_sync();
     pair_issue_pv_seq(vd0 + uint64_t(s) * kVStep, tmem + kTmP + 64u * uint32_t(j & 1),
-                      tmem + kTmO + 128u * uint32_t(j & 1), j >= 2 ? 1u : 0u, std::make_integer_sequence<int, 8>{});
+                      tmem + kTmO + 128u * uint32_t(j & 1), j >= 2 ? 1u : 0u, idesc_pv,
+                      std::make_integer_sequence<int, 8>{});
     pair::commit_both_elect(&sm.pv_done[j & 1]);
     pair::commit_both_elect(&sm.kv_empty[s]);  // S(j) and P.V(j) have read stage s
     return true;
@@ -297,8 +301,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2) {
       uint32_t pk[32];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) pk[e] = pack_bf16x2(s[64 * h2 + 2 * e], s[64 * h2 + 2 * e + 1]);
+      pack_probabilities<RAGGED>(s + 64 * h2, is_f16<RAGGED>(t.v_ref), pk);
       tc::tmem_st32(p_base + uint32_t(h2) * 32u, pk);
     }
     tc::tmem_wait_st();
@@ -321,7 +324,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
   const float f0 = (m0 == -INFINITY) ? 0.f : ex2((m0 - m_fin) * sl2);
   const float f1 = (!has1 || m1 == -INFINITY) ? 0.f : ex2((m1 - m_fin) * sl2);
   const float lt = sm.lsum[0][row] * f0 + (has1 ? sm.lsum[1][row] * f1 : 0.f);
-  const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+  const float inv = (lt == 0.f ? 0.f : 1.0f / lt) * (is_f16<RAGGED>(t.v_ref) ? ex2(t.v_ref) : 1.f);
   const bool none = RAGGED && t.keys == 0;  // no valid key: the accumulators hold NaN, the output is zero
   const int hb = row >> 6;
   const int blk = hb ? t.blk[1] : t.blk[0];  // (no dynamic indexing: keeps the tile in registers)
@@ -485,7 +488,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
     }
   } else if (warp == kPMmaWarp) {
     if (t.rank == 0) {
-      pair_mma(p, t, sm, tmem);
+      pair_mma<RAGGED>(p, t, sm, tmem);
       pair::commit_both_elect(&sm.mma_fin);
       if (lane == 0) drain_wait(&sm.mma_fin, 0, p.err);
     }

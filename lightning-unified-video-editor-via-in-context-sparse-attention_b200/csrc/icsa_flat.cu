@@ -63,6 +63,7 @@ struct FTile {
   int write[4];  // 0 for a duplicate filling an incomplete group
   int n_steps;   // KV steps of 128 rows
   int keys, kvh;  // valid keys and key/value head
+  float v_ref;    // see AttnParams
 };
 
 template <bool RAGGED>
@@ -85,6 +86,7 @@ ICSA_DEV FTile decode_flat_tile(const AttnParams& p, int cta) {
   t.keys = key_count<RAGGED>(p, t.b);
   t.n_steps = key_steps<RAGGED>(p, t.keys);
   t.kvh = key_head<RAGGED>(p, t.h);
+  t.v_ref = value_reference<RAGGED>(p, t.b, t.kvh);
   return t;
 }
 
@@ -151,12 +153,11 @@ ICSA_DEV void flat_issue_pv_seq(uint64_t v_desc, uint32_t p_tmem, uint32_t o_tme
 }
 
 template <int D>
-ICSA_DEV void flat_issue_pv(uint64_t v_desc, uint32_t p_tmem, uint32_t o_tmem, bool accumulate) {
-  flat_issue_pv_seq(v_desc, p_tmem, o_tmem, accumulate ? 1u : 0u, tc::make_idesc_bf16(128, D, false, true),
-                    std::make_integer_sequence<int, 8>{});
+ICSA_DEV void flat_issue_pv(uint64_t v_desc, uint32_t p_tmem, uint32_t o_tmem, bool accumulate, uint32_t idesc) {
+  flat_issue_pv_seq(v_desc, p_tmem, o_tmem, accumulate ? 1u : 0u, idesc, std::make_integer_sequence<int, 8>{});
 }
 
-template <int D>
+template <int D, bool RAGGED>
 ICSA_DEV void flat_mma(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32_t tmem) {
   using C = FCfg<D>;
   volatile int* abort_flag = &sm.abort_flag;
@@ -167,6 +168,7 @@ ICSA_DEV void flat_mma(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32
   const uint64_t v0 = tc::make_sw128_desc(smem_u32(sm.v[0]), kChunkBytes, 1024);
   constexpr uint64_t kStageStep = uint64_t(C::kOpBytes >> 4);
   const uint32_t s0 = tmem, s1 = tmem + 256, o0 = tmem + 128, o1 = tmem + 384;
+  const uint32_t idesc_pv = operand_idesc<RAGGED>(tc::make_idesc_bf16(128, D, false, true), is_f16<RAGGED>(t.v_ref));
   if (!mbar_wait(&sm.q_full, 0, p.err, kErrQ, abort_flag)) return;
   if (!mbar_wait(&sm.k_full[0], 0, p.err, kErrKFull, abort_flag)) return;
   tc::fence_after_sync();
@@ -184,7 +186,7 @@ ICSA_DEV void flat_mma(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32
     if (!mbar_wait(&sm.v_full[vs], vph, p.err, kErrVFull, abort_flag)) return;
     if (!mbar_spin_wait(&sm.p_full[0], uint32_t(j) & 1u, p.err, kErrPFull, abort_flag)) return;
     tc::fence_after_sync();
-    flat_issue_pv<D>(vd, s0, o0, j > 0);
+    flat_issue_pv<D>(vd, s0, o0, j > 0, idesc_pv);
     tc::mma_commit(&sm.o_done[0]);
     if (next) {
       if (!mbar_wait(&sm.k_full[ks], kph, p.err, kErrKFull, abort_flag)) return;
@@ -194,7 +196,7 @@ ICSA_DEV void flat_mma(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32
     }
     if (!mbar_spin_wait(&sm.p_full[1], uint32_t(j) & 1u, p.err, kErrPFull, abort_flag)) return;
     tc::fence_after_sync();
-    flat_issue_pv<D>(vd, s1, o1, j > 0);
+    flat_issue_pv<D>(vd, s1, o1, j > 0, idesc_pv);
     tc::mma_commit(&sm.o_done[1]);
     tc::mma_commit(&sm.v_empty[vs]);
     if (next) {
@@ -257,8 +259,7 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
       if ((c & 63) == 60) {
         // 64 probabilities done: pack them and write them over S in TMEM
         uint32_t pk[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) pk[e] = pack_bf16x2(s[(c & ~63) + 2 * e], s[(c & ~63) + 2 * e + 1]);
+        pack_probabilities<RAGGED>(s + (c & ~63), is_f16<RAGGED>(t.v_ref), pk);
         tc::tmem_st32(s_col + (c >> 6) * 32, pk);
       }
     }
@@ -290,7 +291,7 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
   const int wr = (q == 0) ? t.write[0] : (q == 1) ? t.write[1] : (q == 2) ? t.write[2] : t.write[3];
   const int token = blk * kBlock + (row & 63);
   const bool write = wr && token < p.S;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float inv = (l == 0.f ? 0.f : 1.0f / l) * (is_f16<RAGGED>(t.v_ref) ? ex2(t.v_ref) : 1.f);
   const bool none = RAGGED && t.keys == 0;  // no valid key: the accumulators hold NaN, the output is zero
   const float* oc = p.outc ? p.outc + (size_t(t.bh) * p.NB + blk) * D : nullptr;  // nullptr: no residual term
   const size_t out_row = ((size_t(t.b) * p.S + token) * p.H + t.h) * D;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(kFThreads, 1) flat_kernel(const AttnParams p, 
         drain_wait(&sm.q_full, 0, p.err);
       }
     } else if (warp == kFMmaWarp && lane == 0) {
-      flat_mma<D>(p, t, sm, tmem);
+      flat_mma<D, RAGGED>(p, t, sm, tmem);
       tc::mma_commit(&sm.mma_fin);
       drain_wait(&sm.mma_fin, 0, p.err);
     }

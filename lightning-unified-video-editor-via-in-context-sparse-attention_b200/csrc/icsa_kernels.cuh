@@ -118,6 +118,10 @@ struct AttnParams {
   // and query heads per key/value head (0: one, with kv_lens nullptr)
   const int* kv_lens;
   int kv_group;
+  // [B, key/value heads] or nullptr: where it is a number R, the head's values
+  // are f16 numbers that stand for 2^R of themselves (the probabilities are
+  // f16 then), else bf16
+  const float* v_ref;
 };
 
 struct AttnMaps {

@@ -259,9 +259,48 @@ ICSA_DEV void store8(T* dst, const float (&v)[8]) {
   }
 }
 
-template <typename T, int D>
+ICSA_DEV uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// exponent of a power of two as a float; NaN stays NaN
+ICSA_DEV float scale_log2(float s) { return s != s ? s : float(int(__float_as_uint(s) >> 23) - 127); }
+
+// R of a head for launch_kv8_copy, a CTA each: codes are exact in f16 from
+// 2^-15 to 2^7 of themselves, so where the scales lie within 22 binades
+// R = (log2 of the largest) - 7.  (A NaN scale goes with any R.)
+constexpr int kRefThreads = 256;
+__global__ void __launch_bounds__(kRefThreads) kv8_reference_kernel(const Kv8Cache c, float* v_ref) {
+  const int len = valid_tokens(c, blockIdx.x / c.H), nb = (len + kTokens - 1) / kTokens;
+  const float* scale = c.v_scale + size_t(blockIdx.x) * c.nb;
+  int lo = 1000, hi = -1000;
+  for (int i = threadIdx.x; i < nb; i += kRefThreads) {
+    const float e = scale_log2(scale[i]);
+    if (e == e) {
+      lo = min(lo, int(e));
+      hi = max(hi, int(e));
+    }
+  }
+  __shared__ int part[2][kRefThreads / 32];
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((threadIdx.x & 31) == 0) {
+    part[0][threadIdx.x >> 5] = lo;
+    part[1][threadIdx.x >> 5] = hi;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < kRefThreads / 32; ++i) {
+    lo = min(lo, part[0][i]);
+    hi = max(hi, part[1][i]);
+  }
+  v_ref[blockIdx.x] = hi < lo ? 0.f : hi - lo <= 22 ? float(hi - 7) : __uint_as_float(0x7FC00000u);
+}
+
+// V_REF: the operands of launch_kv8_copy.
+template <typename T, int D, bool V_REF>
 __global__ void __launch_bounds__(FillShape<D>::kThreads)
-    kv8_dequantize_kernel(const Kv8Cache c, T* k_out, T* v_out) {
+    kv8_dequantize_kernel(const Kv8Cache c, T* k_out, T* v_out, const float* v_ref) {
   constexpr int kPerRow = FillShape<D>::kPerRow, kThreads = FillShape<D>::kThreads;
   const int which = k_out == nullptr ? 1 : int(blockIdx.y);
   T* out = which ? v_out : k_out;
@@ -271,7 +310,14 @@ __global__ void __launch_bounds__(FillShape<D>::kThreads)
   const int f0 = (threadIdx.x % kPerRow) * 8, g = threadIdx.x / kPerRow;
   const size_t slot = size_t(bh) * c.nb + blk;
   const bool any = blk * kTokens < len;
-  const float scale = any ? (which ? c.v_scale : c.k_scale)[slot] : 0.f;
+  float scale = any ? (which ? c.v_scale : c.k_scale)[slot] : 0.f;
+  bool f16 = false;
+  if constexpr (V_REF) {
+    wait_prior_grid();
+    const float r = which ? v_ref[bh] : __uint_as_float(0x7FC00000u);
+    f16 = r == r;
+    if (f16) scale *= __uint_as_float(uint32_t(127 - int(r)) << 23);
+  }
   uint32_t code[2][4] = {};  // [features 0-3 | 4-7][token]
   __shared__ uint32_t tile[D][17];
   if (any) {
@@ -320,7 +366,11 @@ __global__ void __launch_bounds__(FillShape<D>::kThreads)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.f;
     }
-    store8<T, D>(out + ((size_t(b) * c.L + tok) * c.H + h) * D + f0, v);
+    T* dst = out + ((size_t(b) * c.L + tok) * c.H + h) * D + f0;
+    if (V_REF && f16)
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]),
+                                                  pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+    else store8<T, D>(dst, v);
   }
 }
 
@@ -334,10 +384,6 @@ ICSA_DEV uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
-}
-ICSA_DEV uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 ICSA_DEV uint4 load_stream16(const void* p) {
   uint4 r;
@@ -358,9 +404,6 @@ ICSA_DEV uint4 keep_bytes(uint4 u, int n) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-// exponent of a power of two as a float; NaN stays NaN
-ICSA_DEV float scale_log2(float s) { return s != s ? s : float(int(__float_as_uint(s) >> 23) - 127); }
 
 // The 8 NQ rows blockIdx.z of (b, cache head): row r is query token r / group,
 // head h * group + r % group.
@@ -683,8 +726,8 @@ template <typename T>
 cudaError_t dequantize_as(const Kv8Cache& c, void* const out[2], cudaStream_t stream) {
   const dim3 grid(unsigned(c.B) * c.H * c.nb, (out[0] != nullptr) + (out[1] != nullptr));
   T *k = static_cast<T*>(out[0]), *v = static_cast<T*>(out[1]);
-  if (c.D == 128) kv8_dequantize_kernel<T, 128><<<grid, FillShape<128>::kThreads, 0, stream>>>(c, k, v);
-  else kv8_dequantize_kernel<T, 64><<<grid, FillShape<64>::kThreads, 0, stream>>>(c, k, v);
+  if (c.D == 128) kv8_dequantize_kernel<T, 128, false><<<grid, FillShape<128>::kThreads, 0, stream>>>(c, k, v, nullptr);
+  else kv8_dequantize_kernel<T, 64, false><<<grid, FillShape<64>::kThreads, 0, stream>>>(c, k, v, nullptr);
   return cudaGetLastError();
 }
 
@@ -696,6 +739,19 @@ cudaError_t launch_kv8_quantize(const Kv8Rows& x, int dtype, const Kv8Cache& c, 
 
 cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out_dtype, cudaStream_t stream) {
   return out_dtype == ICSA_BF16 ? dequantize_as<__nv_bfloat16>(c, out, stream) : dequantize_as<float>(c, out, stream);
+}
+
+cudaError_t launch_kv8_copy(const Kv8Cache& c, void* k, void* v, float* v_ref, cudaStream_t stream) {
+  kv8_reference_kernel<<<c.B * c.H, kRefThreads, 0, stream>>>(c, v_ref);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const dim3 grid(unsigned(c.B) * c.H * c.nb, 2);
+  __nv_bfloat16 *kb = static_cast<__nv_bfloat16*>(k), *vb = static_cast<__nv_bfloat16*>(v);
+  const float* ref = v_ref;
+  return c.D == 128 ? launch_chained(kv8_dequantize_kernel<__nv_bfloat16, 128, true>, grid,
+                                     dim3(FillShape<128>::kThreads), 0, stream, c, kb, vb, ref)
+                    : launch_chained(kv8_dequantize_kernel<__nv_bfloat16, 64, true>, grid,
+                                     dim3(FillShape<64>::kThreads), 0, stream, c, kb, vb, ref);
 }
 
 Kv8DecodePlan kv8_decode_plan(int B, int H, int rows, int L, int D, int num_sms) {

@@ -113,6 +113,10 @@ __device__ __forceinline__ float value_spread(int keys) { return float(78 + __cl
 cudaError_t launch_kv8_quantize(const Kv8Rows& x, int dtype, const Kv8Cache& c, cudaStream_t stream);
 // out[i]: [B, L, H, D] contiguous of out_dtype; rows behind a length are zero
 cudaError_t launch_kv8_dequantize(const Kv8Cache& c, void* const out[2], int out_dtype, cudaStream_t stream);
+// The same as operands of the dense kernels: keys in bf16, the values of a head
+// in f16 as 2^-R of themselves where its scales allow that exactly (R to
+// v_ref[b, h]), else in bf16 (v_ref NaN).
+cudaError_t launch_kv8_copy(const Kv8Cache& c, void* k, void* v, float* v_ref, cudaStream_t stream);
 
 struct Kv8AttnParams {
   const __nv_bfloat16* q;  // [B, Lq, Hq, D]

@@ -259,7 +259,7 @@ struct AttnPlan {
   AttnPath path;
   int splits, groups;            // kDecode
   icsa::Kv8TcPlan tc;    // kPairs
-  size_t v_offset;       // kDense: bf16 copy of the values, behind that of the keys
+  size_t v_offset;       // kDense: 16-bit copy of the values, behind that of the keys; then a float for each head
   size_t bytes;          // workspace
 };
 
@@ -271,8 +271,10 @@ struct AttnPlan {
 //    cut their parts are joined, the more the fewer rounds there are.
 //  * The dense kernels run a 256-row tile per SM pair (D = 128) or SM (D = 64)
 //    at a time, 0.86 / 1.87 us a step of 128 keys, in waves of about 7 us
-//    beside the steps, on a bf16 copy that is written and read (6 bytes an
-//    element).  Their probabilities are bf16, so few rows do without them.
+//    beside the steps, on a 16-bit copy that is written and read (6 bytes an
+//    element).  The values of a head are f16 there, scaled by one power of
+//    two, and so are its probabilities; only where the head's scales do not
+//    let f16 hold the values exactly both are bf16, so few rows do without.
 // Constants fitted to 324 sizes (1, 8 and 2 x 40 heads, D = 64 and 128, 100 to
 // 32000 keys, 16 to 4096 rows): the choice is within 1 % of the best of the
 // three on average, at worst a third slower.  Measured, us, decode / pairs /
@@ -322,7 +324,7 @@ AttnPlan plan_attention(const icsa::Kv8Cache& c, int Lq, int Hq, int sms) {
   if (rows > kNoCopyRows && c.nb <= 16384 && dense_us(c, Lq, Hq, sms) < us) {
     a.path = kDense;
     a.v_offset = align256(size_t(c.B) * c.L * c.H * c.D * 2);
-    a.bytes = 2 * a.v_offset;
+    a.bytes = 2 * a.v_offset + align256(size_t(c.B) * c.H * sizeof(float));
   }
   return a;
 }
@@ -335,7 +337,7 @@ int check_queries(const char* who, const icsa::Kv8Cache& c, int Lq, int Hq) {
   return ICSA_OK;
 }
 
-// The dense tensor core kernels on a bf16 copy of the cache.
+// The dense tensor core kernels on a 16-bit copy of the cache.
 int dense_attention(const icsa::Kv8Cache& c, const AttnPlan& plan, const void* q, const int64_t q_strides[3], void* out,
                     int Lq, int Hq, float scale_log2, void* workspace, cudaStream_t stream) {
   if (q_strides[2] != c.D || q_strides[1] < int64_t(Hq) * c.D || (c.B > 1 && q_strides[0] != Lq * q_strides[1]))
@@ -343,8 +345,9 @@ int dense_attention(const icsa::Kv8Cache& c, const AttnPlan& plan, const void* q
                 "strides of at least Hq * D and a batch stride of Lq tokens", Lq);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   void* const copy[2] = {ws, ws + plan.v_offset};
-  cudaError_t e = icsa::launch_kv8_dequantize(c, copy, ICSA_BF16, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "kv8_attention: bf16 copy of the cache");
+  float* v_ref = reinterpret_cast<float*>(ws + 2 * plan.v_offset);
+  cudaError_t e = icsa::launch_kv8_copy(c, copy[0], copy[1], v_ref, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "kv8_attention: 16-bit copy of the cache");
   const int nbq = (Lq + icsa::kBlock - 1) / icsa::kBlock;
   icsa::AttnMaps maps;
   std::memset(&maps, 0, sizeof(maps));
@@ -364,6 +367,7 @@ int dense_attention(const icsa::Kv8Cache& c, const AttnPlan& plan, const void* q
   a.out = out; a.out_dtype = ICSA_BF16; a.out_tma = 1;
   a.kv_lens = c.lengths;
   a.kv_group = Hq / c.H;
+  a.v_ref = v_ref;
   e = icsa::launch_flat_attention(a, maps, c.D, stream);
   return e == cudaSuccess ? ICSA_OK : cuda_fail(e, "kv8_attention");
 }

@@ -6,7 +6,8 @@ values that the cache holds and "mass" = sum p |v|:
   * one rounding to bf16: 2^-8 of the result;
   * the probabilities' rounding.  In f16 2^-11 of each, and for those below
     2^-14 of the row's largest 2^-25 of that one: 2^-11 mass + 2^-25 max(p)
-    sum |v|.  In bf16, on the copy of the cache, 2^-8 mass;
+    sum |v|.  In bf16, on the copy of a head whose scales lie more than 2^22
+    apart, 2^-8 mass;
   * scores: float32 sums of D products, 16 to an instruction, with sa the
     largest sum |q k| / sqrt(D): at most (16 + D / 16) 2^-23 sa < 2^-18 sa,
     and 2^-18 for the exponential; p moves by as much of itself;
@@ -37,7 +38,7 @@ def on_copy(cache, Lq, Hq):
     """Whether the call runs on a bf16 copy of the cache: told by its workspace."""
     B, H, _, _, D = cache.k.shape
     size = lowp._load().icsa_kv8_attention_workspace_size(ctypes.byref(cache._desc()), Lq, Hq)
-    return size == 2 * (-(-B * cache.L * H * D * 2 // 256) * 256)
+    return size == 2 * (-(-B * cache.L * H * D * 2 // 256) * 256) + -(-B * H * 4 // 256) * 256
 
 
 def check(q, cache, copy=None):
@@ -48,7 +49,7 @@ def check(q, cache, copy=None):
     L, H = k.shape[1:3]
     if copy is not None:
         assert on_copy(cache, Lq, Hq) == copy
-    bits = 8 if on_copy(cache, Lq, Hq) else 11
+    copied = on_copy(cache, Lq, Hq)
     worst = 0.0
     for b in range(B):
         n = L if cache.lengths is None else min(max(int(cache.lengths[b]), 0), L)
@@ -60,6 +61,8 @@ def check(q, cache, copy=None):
             sa = float((qq.abs() @ kk.abs().T).max()) / math.sqrt(D)
             p = torch.softmax(qq @ kk.T / math.sqrt(D), -1)
             want, mass = p @ vv, p @ vv.abs()
+            e = torch.log2(cache.v_scale[b, h * H // Hq, :-(-n // 64)])
+            bits = 8 if copied and float(e.max() - e.min()) > 22 else 11
             tol = (want.abs() * 2.0 ** -8 + mass * (2.0 ** -bits + (sa + 1) * 2.0 ** -18 + (n / 16 + 64) * 2.0 ** -23)
                    + 1e-38)
             if bits == 11:
@@ -135,6 +138,36 @@ def test_probabilities_keep_the_bits_of_their_path(path, D):
     q = torch.randn(3, Lq, H * group, D, generator=g).to(torch.bfloat16).cuda()
     n = torch.tensor([L, 0, L - 77], dtype=torch.int32, device="cuda")
     check(q, lowp.kv8_quantize(k, v, n))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_copied_heads_of_both_kinds(D):
+    """Heads whose scales lie near together and far apart, shared by query heads, with lengths that leave the far
+    blocks of one sequence out; then blocks exactly 22 and 23 binades apart, and a block with a NaN."""
+    g = torch.Generator().manual_seed(9)
+    B, Lq, L, H, group = 2, 4096, 2000, 4, 2
+    k, v = (torch.randn(B, L, H, D, generator=g) for _ in range(2))
+    v[:, :1024, 1] *= 2.0 ** -30
+    v[:, 1024:, 2] *= 2.0 ** 40
+    v[:, 64:128, 3] = 0.0
+    q = torch.randn(B, Lq, H * group, D, generator=g).to(torch.bfloat16).cuda()
+    n = torch.tensor([L, 1000], dtype=torch.int32, device="cuda")
+    check(q, lowp.kv8_quantize(k.cuda(), v.cuda(), n), True)
+    v = torch.randn(B, L, H, D, generator=g).clamp(-3, 3)
+    v[:, ::64] = 3.0                                            # the same scale in every block
+    v[:, 640:704, 0] *= 2.0 ** -22
+    v[:, 640:704, 1] *= 2.0 ** -23
+    cache = lowp.kv8_quantize(k.cuda(), v.cuda(), n)
+    for h, apart in ((0, 22), (1, 23), (2, 0)):
+        e = torch.log2(cache.v_scale[0, h])
+        assert float(e.max() - e.min()) == apart
+    clean = check(q, cache, True)
+    v[0, 700, 2, 5] = math.nan
+    bad = lowp.kv8_attention(q, lowp.kv8_quantize(k.cuda(), v.cuda(), n))
+    assert bool(torch.isnan(bad[0, :, 4:6]).all())
+    rest = torch.ones(B, H * group, dtype=torch.bool)
+    rest[0, 4:6] = False
+    assert all(torch.equal(bad[b, :, h], clean[b, :, h]) for b in range(B) for h in range(H * group) if rest[b, h])
 
 
 def test_a_replayed_call_follows_scales_that_change():
