@@ -148,14 +148,17 @@ ICSA_API int icsa_kv8_dequantize(const icsa_kv8_cache* cache, void* k_out, void*
  * apart have their probabilities in bf16 (off by 2^-8 of themselves).
  *   q: bf16 [B, Lq, Hq, D] with batch, token, head strides (multiples of 8
  *   elements, 16-byte aligned), contiguous features; Hq a multiple of H.
- *   (ICSA_ERR_UNSUPPORTED for many queries over a long cache whose heads are
- *   not contiguous, or whose tokens or batch elements overlap or have gaps
- *   between batch elements: that path reads q as rows.)
+ *   Many queries over a long cache read q as rows: contiguous heads, tokens
+ *   that do not overlap, no gaps between batch elements.  A q of other strides
+ *   takes another kernel then, for which the workspace has to be of
+ *   icsa_kv8_attention_strided_workspace_size() bytes (ICSA_ERR_UNSUPPORTED
+ *   where it is smaller); for every other size that is the same number.
  *   out: bf16 [B, Lq, Hq, D], contiguous
  *   workspace: icsa_kv8_attention_workspace_size() bytes, 256-byte aligned;
  *   its contents do not matter before the call and mean nothing after it
  */
 ICSA_API size_t icsa_kv8_attention_workspace_size(const icsa_kv8_cache* cache, int Lq, int Hq);
+ICSA_API size_t icsa_kv8_attention_strided_workspace_size(const icsa_kv8_cache* cache, int Lq, int Hq);
 ICSA_API int icsa_kv8_attention(const icsa_kv8_cache* cache, const void* q, const int64_t q_strides[3], void* out,
                                 int Lq, int Hq, void* workspace, size_t workspace_bytes, cudaStream_t stream);
 

@@ -337,12 +337,15 @@ int check_queries(const char* who, const icsa::Kv8Cache& c, int Lq, int Hq) {
   return ICSA_OK;
 }
 
+// Whether q is rows of contiguous heads, as the dense kernels read it.
+bool query_rows(const icsa::Kv8Cache& c, const int64_t q_strides[3], int Lq, int Hq) {
+  return q_strides[2] == c.D && q_strides[1] >= int64_t(Hq) * c.D &&
+         (c.B == 1 || q_strides[0] == Lq * q_strides[1]);
+}
+
 // The dense tensor core kernels on a 16-bit copy of the cache.
 int dense_attention(const icsa::Kv8Cache& c, const AttnPlan& plan, const void* q, const int64_t q_strides[3], void* out,
                     int Lq, int Hq, float scale_log2, void* workspace, cudaStream_t stream) {
-  if (q_strides[2] != c.D || q_strides[1] < int64_t(Hq) * c.D || (c.B > 1 && q_strides[0] != Lq * q_strides[1]))
-    return fail(ICSA_ERR_UNSUPPORTED, "kv8_attention: %d query tokens over a long cache need contiguous heads, token "
-                "strides of at least Hq * D and a batch stride of Lq tokens", Lq);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   void* const copy[2] = {ws, ws + plan.v_offset};
   float* v_ref = reinterpret_cast<float*>(ws + 2 * plan.v_offset);
@@ -489,6 +492,16 @@ size_t icsa_kv8_attention_workspace_size(const icsa_kv8_cache* cache, int Lq, in
   return plan_attention(c, Lq, Hq, sms).bytes;
 }
 
+size_t icsa_kv8_attention_strided_workspace_size(const icsa_kv8_cache* cache, int Lq, int Hq) {
+  icsa::Kv8Cache c;
+  int sms = 0;
+  if (check_cache("kv8_attention_strided_workspace_size", cache, &c) != ICSA_OK ||
+      check_queries("kv8_attention_strided_workspace_size", c, Lq, Hq) != ICSA_OK || !sm_count(&sms))
+    return 0;
+  const AttnPlan plan = plan_attention(c, Lq, Hq, sms);
+  return plan.path == kDense ? align256(plan.tc.bytes) : plan.bytes;
+}
+
 int icsa_kv8_attention(const icsa_kv8_cache* cache, const void* q, const int64_t q_strides[3], void* out, int Lq,
                        int Hq, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   icsa::Kv8Cache c;
@@ -504,7 +517,16 @@ int icsa_kv8_attention(const icsa_kv8_cache* cache, const void* q, const int64_t
       return fail(ICSA_ERR_INVALID, "kv8_attention: strides of q must be non-negative multiples of 8 elements");
   int sms = 0;
   if (!sm_count(&sms)) return ICSA_ERR_CUDA;
-  const AttnPlan plan = plan_attention(c, Lq, Hq, sms);
+  AttnPlan plan = plan_attention(c, Lq, Hq, sms);
+  if (plan.path == kDense && !query_rows(c, q_strides, Lq, Hq)) {
+    // the copy path reads q as rows; the pair kernel takes any strides, in its own workspace
+    plan.path = kPairs;
+    plan.bytes = align256(plan.tc.bytes);
+    if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes))
+      return fail(ICSA_ERR_UNSUPPORTED, "kv8_attention: %d query tokens over a long cache need contiguous heads, token "
+                  "strides of at least Hq * D and a batch stride of Lq tokens, or a workspace of "
+                  "icsa_kv8_attention_strided_workspace_size() = %zu bytes", Lq, plan.bytes);
+  }
   if (plan.bytes > 0) {
     if (workspace == nullptr || workspace_bytes < plan.bytes)
       return fail(ICSA_ERR_WORKSPACE, "kv8_attention: workspace of %zu bytes is smaller than the %zu bytes required",

@@ -30,7 +30,7 @@ LOWP_EXPORTED = ("icsa_fp4_data_bytes", "icsa_fp4_scale_bytes", "icsa_fp4_quanti
                  "icsa_fp4_linear_workspace_size", "icsa_fp4_linear", "icsa_fp4_linear_rows_workspace_size",
                  "icsa_fp4_linear_rows", "icsa_fp4_linear_scaled_rows_workspace_size", "icsa_fp4_linear_scaled_rows",
                  "icsa_kv8_quantize", "icsa_kv8_dequantize",
-                 "icsa_kv8_attention_workspace_size", "icsa_kv8_attention")
+                 "icsa_kv8_attention_workspace_size", "icsa_kv8_attention_strided_workspace_size", "icsa_kv8_attention")
 
 FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
 FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
@@ -74,6 +74,7 @@ def _load():
             ("icsa_kv8_quantize", i, [desc, vp, vp, i, st, st, vp]),
             ("icsa_kv8_dequantize", i, [desc, vp, vp, i, vp]),
             ("icsa_kv8_attention_workspace_size", sz, [desc, i, i]),
+            ("icsa_kv8_attention_strided_workspace_size", sz, [desc, i, i]),
             ("icsa_kv8_attention", i, [desc, vp, st, vp, i, i, vp, sz, vp])):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, res
@@ -466,8 +467,14 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace(index, B, H, L, D, Lq, Hq):
-    return _lib.icsa_kv8_attention_workspace_size(ctypes.byref(_Kv8Desc(B, H, L, D)), Lq, Hq)
+def _attention_workspace(index, B, H, L, D, Lq, Hq, strided=False):
+    """Workspace bytes of icsa_kv8_attention; strided: for a q that is not rows,
+    None where that would take another kernel.  The device is current."""
+    desc = ctypes.byref(_Kv8Desc(B, H, L, D))
+    size = _lib.icsa_kv8_attention_workspace_size(desc, Lq, Hq)
+    if strided and size != _lib.icsa_kv8_attention_strided_workspace_size(desc, Lq, Hq):
+        return None
+    return size
 
 
 def _attention(lib, stream, index, q, shape, cache, H):
@@ -476,16 +483,21 @@ def _attention(lib, stream, index, q, shape, cache, H):
     if Lq == 0:
         return out
     sb, st, sh, sd = q.stride()
-    # rows of a wider GEMM output are taken as they are
-    if (sd != 1 or (Hq > 1 and sh != D) or (Lq > 1 and st < Hq * D) or st % 8 or (B > 1 and sb != Lq * st)
-            or q.data_ptr() % 16):
+    # an axis of one has any stride
+    sh = sh if Hq > 1 else D
+    st = st if Lq > 1 else Hq * D
+    sb = sb if B > 1 else Lq * st
+    size = None
+    if sd == 1 and not (sb | st | sh) % 8 and q.data_ptr() % 16 == 0:
+        # rows of a wider GEMM output are taken as they are, other strides wherever the kernel for these sizes does
+        strided = sh != D or st < Hq * D or sb != Lq * st
+        size = _attention_workspace(index, B, H, cache.L, D, Lq, Hq, strided)
+    if size is None:
         q = q.clone(memory_format=torch.contiguous_format)
-        st = Hq * D
-    if Lq == 1 and B == 1:
-        st = Hq * D
-    size = _attention_workspace(index, B, H, cache.L, D, Lq, Hq)
+        sb, st, sh = Lq * Hq * D, Hq * D, D
+        size = _attention_workspace(index, B, H, cache.L, D, Lq, Hq)
     ws, ptr = _bytes(out, size)
-    code = lib.icsa_kv8_attention(ctypes.byref(cache._desc()), q.data_ptr(), _int64x3(Lq * st, st, D), out.data_ptr(),
+    code = lib.icsa_kv8_attention(ctypes.byref(cache._desc()), q.data_ptr(), _int64x3(sb, st, sh), out.data_ptr(),
                                   Lq, Hq, ptr, size, stream)
     if code:
         _capi.check(code, "icsa_kv8_attention")

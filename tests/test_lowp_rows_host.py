@@ -71,3 +71,12 @@ def test_inputs_that_require_a_gradient_are_refused_where_gradients_are_enabled(
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):      # as without one: tensors on the CPU
             call()
+
+
+def test_strided_workspace_size_refuses_what_the_attention_refuses():
+    import ctypes
+    lib = lowp._load()
+    for bad in (dict(D=32), dict(B=0), dict(L=0)):
+        d = {**dict(B=1, H=2, L=5, D=128), **bad}
+        assert lib.icsa_kv8_attention_strided_workspace_size(ctypes.byref(lowp._Kv8Desc(*d.values())), 1, 2) == 0
+    assert lib.icsa_kv8_attention_strided_workspace_size(ctypes.byref(lowp._Kv8Desc(1, 2, 5, 128)), 1, 3) == 0
