@@ -229,6 +229,9 @@ ICSA_DEV void issuer(const Fp4GemmParams& p, Smem& sm, uint32_t tmem) {
 // the tile at M and N, or row by row where the output's rows are not aligned.  (Storing the rows straight from registers, 16 bytes
 // a lane in 32 different lines, took 8600 clk a tile, more than half of a
 // K = 5120 main loop.)
+// SCALED: a's rows have their own global scales (read in the same instance by
+// every call they cost 30 us of 1890 with GELU).
+template <bool SCALED>
 ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm, uint32_t tmem, uint32_t rank) {
   volatile int* abort_flag = &sm.abort_flag;
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
@@ -250,7 +253,7 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
       bias[threadIdx.x & 127] = bv;
       pair::named_sync(1u + uint32_t(w), 128);
     }
-    const float alpha = row0 + lane < p.M ? row_alpha(p, row0 + lane) : 0.f;
+    const float alpha = !SCALED ? p.alpha : row0 + lane < p.M ? row_alpha(p, row0 + lane) : 0.f;
     const bool ok = attn::warp_mbar_wait(&sm.acc_full, uint32_t(count) & 1u, nullptr, kErrAccFull, abort_flag);
     tc::fence_after_sync();
     float acc[128];
@@ -332,7 +335,7 @@ ICSA_DEV void epilogue(const Fp4GemmParams& p, const Fp4GemmMaps& maps, Smem& sm
   if (lane == 0) bulk_wait_read();
 }
 
-template <int FMT>
+template <int FMT, bool SCALED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const Fp4GemmParams p, const __grid_constant__ Fp4GemmMaps maps) {
   extern __shared__ uint8_t smem_raw[];
@@ -365,7 +368,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sm.tmem_base;
   wait_prior_grid();  // the operands are the previous kernels' outputs
   if (warp < 8) {
-    epilogue(p, maps, sm, tmem, rank);
+    epilogue<SCALED>(p, maps, sm, tmem, rank);
   } else if (warp == kProducerWarp) {
     if (lane == 0) {
       int issued = 0;
@@ -448,7 +451,9 @@ cudaError_t launch_fp4_gemm(Fp4GemmParams p, const Fp4GemmMaps& maps, int format
   if (p.units == 0) return cudaSuccess;
   const int clusters = std::max(1, std::min(num_sms / 2, p.units));
   const size_t smem = sizeof(Smem) + 1024;
-  auto kernel = format == ICSA_NVFP4 ? fp4_gemm_kernel<ICSA_NVFP4> : fp4_gemm_kernel<ICSA_MXFP4>;
+  const auto kernel = format == ICSA_MXFP4      ? fp4_gemm_kernel<ICSA_MXFP4, false>
+                      : p.row_scales != nullptr ? fp4_gemm_kernel<ICSA_NVFP4, true>
+                                                : fp4_gemm_kernel<ICSA_NVFP4, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
   e = launch_chained(kernel, dim3(2 * clusters), dim3(kThreads), smem, stream, p, maps);

@@ -141,10 +141,11 @@ ICSA_DEV int cache_length(const Kv8Cache& c, int b) {
 ICSA_DEV int steps_of(int len) { return (len + kStepKeys - 1) / kStepKeys; }
 
 // Work space: the rounds of batch element 0, 1, .. one behind the other, heads
-// outermost, a step of a round of two tiles weighing 12 and of one tile 10
-// (measured: 2.6 us for the two tiles of a step, 2.2 us for one, which the
-// filling of its stage bounds).  A round without keys, and in whole
-// rounds its epilogue, count as a step.
+// outermost, a step of a round of two tiles weighing 12 and of one tile 10: the
+// latter is bound by the filling of its stage.  (1 x 12 heads, 700 rows over
+// 6000 keys, three tiles a head: 12 to 10 61.7 us, 12 to 9 63.6, 12 to 8, the
+// ratio of the times that plan_attention fits over all sizes, 66.8.)  A round
+// without keys, and in whole rounds its epilogue, count as a step.
 constexpr int kWeightTwo = 12, kWeightOne = 10;
 struct Extent {
   int n;             // steps that a round counts for
