@@ -121,9 +121,9 @@ ICSA_DEV uint32_t operand_idesc(uint32_t bf16, bool f16) {
   return RAGGED && f16 ? bf16 & ~((1u << 7) | (1u << 10)) : bf16;
 }
 // 64 probabilities as 16-bit pairs
-template <bool RAGGED>
-ICSA_DEV void pack_probabilities(const float* s, bool f16, uint32_t (&pk)[32]) {
-  if (RAGGED && f16) {
+template <bool F16>
+ICSA_DEV void pack_probabilities(const float* s, uint32_t (&pk)[32]) {
+  if constexpr (F16) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
       const __half2 v = __floats2half2_rn(s[2 * e], s[2 * e + 1]);

@@ -216,7 +216,7 @@ ICSA_DEV void pair_mma(const AttnParams& p, const PTile& t, PSmem& sm, uint32_t 
 // epilogue's named barriers pair them): after a failed wait the abort flag
 // is set, every later wait returns at once, the loop runs on over stale
 // data, and the error code marks the result invalid.
-template <bool RAGGED>
+template <bool RAGGED, bool F16>
 ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTile& t, PSmem& sm, uint32_t tmem) {
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -301,7 +301,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2) {
       uint32_t pk[32];
-      pack_probabilities<RAGGED>(s + 64 * h2, is_f16<RAGGED>(t.v_ref), pk);
+      pack_probabilities<F16>(s + 64 * h2, pk);
       tc::tmem_st32(p_base + uint32_t(h2) * 32u, pk);
     }
     tc::tmem_wait_st();
@@ -324,7 +324,7 @@ ICSA_DEV void pair_softmax(const AttnParams& p, const AttnMaps& maps, const PTil
   const float f0 = (m0 == -INFINITY) ? 0.f : ex2((m0 - m_fin) * sl2);
   const float f1 = (!has1 || m1 == -INFINITY) ? 0.f : ex2((m1 - m_fin) * sl2);
   const float lt = sm.lsum[0][row] * f0 + (has1 ? sm.lsum[1][row] * f1 : 0.f);
-  const float inv = (lt == 0.f ? 0.f : 1.0f / lt) * (is_f16<RAGGED>(t.v_ref) ? ex2(t.v_ref) : 1.f);
+  const float inv = (lt == 0.f ? 0.f : 1.0f / lt) * (F16 ? ex2(t.v_ref) : 1.f);
   const bool none = RAGGED && t.keys == 0;  // no valid key: the accumulators hold NaN, the output is zero
   const int hb = row >> 6;
   const int blk = hb ? t.blk[1] : t.blk[0];  // (no dynamic indexing: keeps the tile in registers)
@@ -470,7 +470,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
   // a warpgroup.
   if (warp < 8) {
     tc::reg_alloc<216>();
-    pair_softmax<RAGGED>(p, maps, t, sm, tmem);
+    if (is_f16<RAGGED>(t.v_ref)) pair_softmax<RAGGED, RAGGED>(p, maps, t, sm, tmem);
+    else pair_softmax<RAGGED, false>(p, maps, t, sm, tmem);
   } else {
     tc::reg_dealloc<72>();
   }

@@ -212,7 +212,7 @@ ICSA_DEV void flat_mma(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32
 // ---------------------------------------------------------------------------
 // Softmax warpgroups (warps 0-3: tile 0, warps 4-7: tile 1) and epilogue.
 // ---------------------------------------------------------------------------
-template <int D, bool RAGGED>
+template <int D, bool RAGGED, bool F16>
 ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, uint32_t tmem) {
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5;
@@ -259,7 +259,7 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
       if ((c & 63) == 60) {
         // 64 probabilities done: pack them and write them over S in TMEM
         uint32_t pk[32];
-        pack_probabilities<RAGGED>(s + (c & ~63), is_f16<RAGGED>(t.v_ref), pk);
+        pack_probabilities<F16>(s + (c & ~63), pk);
         tc::tmem_st32(s_col + (c >> 6) * 32, pk);
       }
     }
@@ -291,7 +291,7 @@ ICSA_DEV void flat_softmax(const AttnParams& p, const FTile& t, FSmem<D>& sm, ui
   const int wr = (q == 0) ? t.write[0] : (q == 1) ? t.write[1] : (q == 2) ? t.write[2] : t.write[3];
   const int token = blk * kBlock + (row & 63);
   const bool write = wr && token < p.S;
-  const float inv = (l == 0.f ? 0.f : 1.0f / l) * (is_f16<RAGGED>(t.v_ref) ? ex2(t.v_ref) : 1.f);
+  const float inv = (l == 0.f ? 0.f : 1.0f / l) * (F16 ? ex2(t.v_ref) : 1.f);
   const bool none = RAGGED && t.keys == 0;  // no valid key: the accumulators hold NaN, the output is zero
   const float* oc = p.outc ? p.outc + (size_t(t.bh) * p.NB + blk) * D : nullptr;  // nullptr: no residual term
   const size_t out_row = ((size_t(t.b) * p.S + token) * p.H + t.h) * D;
@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(kFThreads, 1) flat_kernel(const AttnParams p, 
   // a warpgroup.
   if (warp < 8) {
     tc::reg_alloc<216>();
-    flat_softmax<D, RAGGED>(p, t, sm, tmem);
+    if (is_f16<RAGGED>(t.v_ref)) flat_softmax<D, RAGGED, RAGGED>(p, t, sm, tmem);
+    else flat_softmax<D, RAGGED, false>(p, t, sm, tmem);
   } else {
     tc::reg_dealloc<72>();  // one instance for all four warps of warpgroup 2
     if (warp == kFProducerWarp && lane == 0) {
